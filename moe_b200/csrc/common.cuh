@@ -18,6 +18,7 @@ enum : int {
     ST_BAD_EXPERT = 4,    // routing produced an expert id outside [0, E)
     ST_WAIT_TIMEOUT = 8,  // a bounded wait on a barrier ran out
     ST_BAD_ROW = 16,      // gather index outside its tensor
+    ST_NOT_FINITE = 32,   // a weight that is to be held in 4 bits is an infinity or a NaN
 };
 
 // status[1]: where the FIRST bounded wait ran out (a site number, see WAIT_SITES in ops/core.py); 0 if none.

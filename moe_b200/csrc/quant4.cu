@@ -1,0 +1,223 @@
+// Weights to 4 bits and back (the format: quant4.cuh).
+//
+//   s = max |w| over the group / 7, rounded to five significant bits (nearest, ties to even); q = w / s rounded (ties to even).
+// s may be rounded down by 1 / 33 of itself at most, so |w| / s <= 7 (1 + 1 / 32) < 7.5 and q needs no clamp.  Decisions at a border are
+// exact: the quotient max / 7 is formed in 64 bits (of a 24-bit number: never nearer to a border of five bits than 2^-27 of itself unless on
+// it), and w - q s, which 32 bits hold exactly, says which side of half a step w lies on.  A group whose maximum is below 7 * 2^-126 is
+// held as zeros; one that holds an infinity or a NaN gets the scale NaN, so that products of it are NaN, and sets ST_NOT_FINITE.
+//
+// Both directions are bound by DRAM: a warp takes one strip (16 rows) x 64 k (128 where a group is 128), 8 bytes a load of bfloat16, four
+// lanes a 32-byte sector.
+#include "quant4.cuh"
+
+namespace {
+
+template <typename T>
+__device__ __forceinline__ void load4(const T* row, int k, int K, bool vec, float (&v)[4]) {
+    if (vec && k + 4 <= K) {
+        if constexpr (sizeof(T) == 2) {
+            const uint2 u = __ldg(reinterpret_cast<const uint2*>(row + k));
+            v[0] = __uint_as_float(u.x << 16), v[1] = __uint_as_float(u.x & 0xffff0000u);
+            v[2] = __uint_as_float(u.y << 16), v[3] = __uint_as_float(u.y & 0xffff0000u);
+        } else {
+            const float4 f = __ldg(reinterpret_cast<const float4*>(row + k));
+            v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) v[i] = k + i < K ? ld_f(row + k + i) : 0.f;
+}
+
+// max / 7 to five significant bits; 0 for what is held as zeros, NaN for what is no number
+__device__ __forceinline__ float scale_of(float amax) {
+    if (!(amax <= 3.402823466e38f)) return __uint_as_float(0x7fc00000u);
+    if (amax < 0x1.cp-124f) return 0.f;                                   // 7 * 2^-126
+    const double d = (double)amax / 7.0;
+    unsigned long long u = (unsigned long long)__double_as_longlong(d);
+    u += (1ull << 47) - 1 + ((u >> 48) & 1);                              // 52 - 4 bits go
+    u &= ~((1ull << 48) - 1);
+    return (float)__longlong_as_double((long long)u);
+}
+
+// w / s to the nearest whole number, ties to even
+__device__ __forceinline__ int code_of(float w, float s, float rs) {
+    float q = rintf(w * rs);
+    const float r = fmaf(-q, s, w), h = 0.5f * s, a = fabsf(r);           // exact: q s has eight bits and lies within a step of w
+    if (a > h || (a == h && ((int)q & 1))) q += r > 0.f ? 1.f : -1.f;
+    return (int)q;
+}
+
+__device__ __forceinline__ bool row_of(int strip, int r, int strips, int N, int pair, int* row) {
+    const int half = pair ? N / 2 : N, per = pair ? strips / 2 : strips;
+    const int h = strip / per, in = (strip - h * per) * q4::STRIP + r;
+    *row = h * half + in;
+    return in < half;
+}
+
+template <typename T, int GROUP>
+__global__ void __launch_bounds__(256)
+quantize_kernel(const T* __restrict__ w, int N, int K, int pair, int strips, int blocks, int qgroups, int vec, long long units, uint4* __restrict__ codes,
+                uint32_t* __restrict__ scales, int* status) {
+    constexpr int SPAN = GROUP == 128 ? 2 : 1;                            // blocks of a unit
+    pdl_sync();
+    const int lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
+    const int per_strip = (blocks + SPAN - 1) / SPAN;
+    const long long unit = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (unit >= units) return;
+    const long long gs = unit / per_strip;                                // group and strip
+    const int u = (int)(unit - gs * per_strip), strip = (int)(gs % strips);
+    const T* wg = w + (size_t)(gs / strips) * N * K;
+    float v[2][SPAN][16];
+#pragma unroll
+    for (int half = 0; half < 2; half++) {
+        int row;
+        const bool live = row_of(strip, r + 8 * half, strips, N, pair, &row);
+        const T* p = wg + (size_t)(live ? row : 0) * K;
+#pragma unroll
+        for (int b = 0; b < SPAN; b++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                float x[4];
+                load4(p, live ? (u * SPAN + b) * 64 + 16 * j + 4 * t : K, K, vec, x);
+#pragma unroll
+                for (int i = 0; i < 4; i++) v[half][b][4 * j + i] = x[i];
+            }
+    }
+    constexpr int SETS = GROUP == 32 ? 2 : 1, PER = 16 * SPAN / SETS;     // scales of a unit and row, elements of this lane under one
+    float s[2][SETS], rs[2][SETS];
+    bool bad = false;
+#pragma unroll
+    for (int half = 0; half < 2; half++)
+#pragma unroll
+        for (int g = 0; g < SETS; g++) {
+            float m = 0.f;
+            bool fine = true;
+#pragma unroll
+            for (int i = 0; i < PER; i++) {
+                const float a = fabsf(v[half][(g * PER + i) / 16][(g * PER + i) % 16]);
+                fine = fine && a <= 3.402823466e38f;
+                m = fmaxf(m, a);
+            }
+            if (!fine) m = INFINITY;
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+            s[half][g] = scale_of(m);
+            bad = bad || s[half][g] != s[half][g];
+            rs[half][g] = s[half][g] > 0.f ? 1.f / s[half][g] : 0.f;      // (0 too for NaN: q = 0)
+        }
+    if (bad && status) atomicOr(status, ST_NOT_FINITE);
+    if (t == 0) {
+#pragma unroll
+        for (int g = 0; g < SETS; g++) {
+            const int q = GROUP == 32 ? 2 * u + g : u;
+            if (q < qgroups)
+                scales[((size_t)gs * qgroups + q) * 8 + r] = (__float_as_uint(s[0][g]) >> 16) | (__float_as_uint(s[1][g]) & 0xffff0000u);
+        }
+    }
+#pragma unroll
+    for (int b = 0; b < SPAN; b++) {
+        if (u * SPAN + b >= blocks) break;
+        uint32_t out[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int g = GROUP == 32 ? j / 2 : 0;
+            uint32_t o = 0;
+#pragma unroll
+            for (int i = 0; i < 4; i++)                                   // k 4 t + i: pair i / 2, place i % 2
+#pragma unroll
+                for (int half = 0; half < 2; half++) {
+                    const int q = rs[half][g] > 0.f ? code_of(v[half][b][4 * j + i], s[half][g], rs[half][g]) : 0;
+                    o |= (uint32_t)(q + 8) << (16 * (i & 1) + 8 * (i >> 1) + 4 * half);
+                }
+            out[j] = o;
+        }
+        codes[((size_t)gs * blocks + u * SPAN + b) * 32 + lane] = make_uint4(out[0], out[1], out[2], out[3]);
+    }
+}
+
+template <int GROUP>
+__global__ void __launch_bounds__(256)
+dequantize_kernel(const uint4* __restrict__ codes, const uint32_t* __restrict__ scales, int N, int K, int pair, int strips, int blocks, int qgroups,
+                  int vec, long long units, __nv_bfloat16* __restrict__ out) {
+    pdl_sync();
+    const int lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
+    const long long unit = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (unit >= units) return;
+    const long long gs = unit / blocks;
+    const int b = (int)(unit - gs * blocks), strip = (int)(gs % strips);
+    const uint4 c = __ldg(codes + (size_t)unit * 32 + lane);
+    q4::Scales<GROUP> sc;
+    sc.load(scales + (size_t)gs * qgroups * 8, b, qgroups, r);
+    __nv_bfloat16* og = out + (size_t)(gs / strips) * N * K;
+    int row[2];
+    const bool live[2] = {row_of(strip, r, strips, N, pair, &row[0]), row_of(strip, r + 8, strips, N, pair, &row[1])};
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        uint32_t a[4];
+        q4::unpack(q4::word(c, j), a);
+        const int k = b * 64 + 16 * j + 4 * t;
+#pragma unroll
+        for (int half = 0; half < 2; half++) {
+            const uint32_t s2 = sc.s[GROUP == 32 ? j / 2 : 0];
+            const __nv_bfloat16 s = __ushort_as_bfloat16((unsigned short)(half ? s2 >> 16 : s2 & 0xffffu));
+            const __nv_bfloat162 ss = __halves2bfloat162(s, s);
+            __nv_bfloat162 v[2];
+#pragma unroll
+            for (int p = 0; p < 2; p++) v[p] = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&a[half + 2 * p]), ss);      // exact
+            if (!live[half]) continue;
+            __nv_bfloat16* o = og + (size_t)row[half] * K + k;
+            if (vec && k + 4 <= K)
+                *reinterpret_cast<uint2*>(o) = *reinterpret_cast<const uint2*>(v);
+            else
+                for (int i = 0; i < 4 && k + i < K; i++) o[i] = reinterpret_cast<const __nv_bfloat16*>(v)[i];
+        }
+    }
+}
+
+}  // namespace
+
+#define BY_GROUP(CALL)            \
+    switch (group) {              \
+        case 32: return CALL(32);   \
+        case 64: return CALL(64);   \
+        case 128: return CALL(128); \
+    }                             \
+    return (int)cudaErrorInvalidValue
+
+// w: [G, N, K] float32 (w_dt DT_F32) or bfloat16, contiguous; codes, scales: see quant4.cuh (strips of one G: ceil(N / 16), of a pair
+// 2 ceil(N / 2 / 16)).
+MOE_API int moe_q4_quantize(const void* w, int w_dt, int G, int N, int K, int group, int pair, void* codes, void* scales, int* status, cudaStream_t stream) {
+    if (G <= 0 || N <= 0 || K <= 0) return 0;
+    if (!w || !codes || !scales || (pair && N % 2)) return (int)cudaErrorInvalidValue;
+    const int half = pair ? N / 2 : N, strips = (half + 15) / 16 * (pair ? 2 : 1), blocks = (K + 63) / 64, qgroups = (K + group - 1) / group;
+    const int span = group == 128 ? 2 : 1;
+    const long long units = (long long)G * strips * ((blocks + span - 1) / span), grid = (units + 7) / 8;
+    if (grid > 0x7fffffffll) return (int)cudaErrorInvalidValue;
+    const int vec = K % 4 == 0 && ((uintptr_t)w & 15) == 0;
+#define GO(GR)                                                                                                                                    \
+    (w_dt == DT_BF16 ? launch_pdl(quantize_kernel<__nv_bfloat16, GR>, (unsigned)grid, 256, 0, stream, (const __nv_bfloat16*)w, N, K, pair, strips, blocks, \
+                                  qgroups, vec, units, (uint4*)codes, (uint32_t*)scales, status)                                                  \
+                     : launch_pdl(quantize_kernel<float, GR>, (unsigned)grid, 256, 0, stream, (const float*)w, N, K, pair, strips, blocks, qgroups, vec,  \
+                                  units, (uint4*)codes, (uint32_t*)scales, status))
+    BY_GROUP(GO);
+#undef GO
+}
+
+// out: [G, N, K] bfloat16, the values that the codes stand for
+MOE_API int moe_q4_dequantize(const void* codes, const void* scales, int G, int N, int K, int group, int pair, void* out, cudaStream_t stream) {
+    if (G <= 0 || N <= 0 || K <= 0) return 0;
+    if (!out || !codes || !scales || (pair && N % 2)) return (int)cudaErrorInvalidValue;
+    const int half = pair ? N / 2 : N, strips = (half + 15) / 16 * (pair ? 2 : 1), blocks = (K + 63) / 64, qgroups = (K + group - 1) / group;
+    const long long units = (long long)G * strips * blocks, grid = (units + 7) / 8;
+    if (grid > 0x7fffffffll) return (int)cudaErrorInvalidValue;
+    const int vec = K % 4 == 0 && ((uintptr_t)out & 7) == 0;
+#define GO(GR)                                                                                                                             \
+    launch_pdl(dequantize_kernel<GR>, (unsigned)grid, 256, 0, stream, (const uint4*)codes, (const uint32_t*)scales, N, K, pair, strips, blocks, qgroups, \
+               vec, units, (__nv_bfloat16*)out)
+    BY_GROUP(GO);
+#undef GO
+}
+
+// Programmatic dependent launch on or off for the kernels of this library (on by default).
+MOE_API void moe_q4_set_pdl(int enabled) { g_pdl_enabled = enabled ? 1 : 0; }

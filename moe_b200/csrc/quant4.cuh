@@ -1,0 +1,71 @@
+// Weights held in 4 bits, as every kernel that reads them sees them.
+//
+// W [G, N, K]: `group` (32, 64 or 128) neighbouring k of a row share a scale s of five significant bits, and an element is q s with
+// a whole number q, -7 <= q <= 7.  q has three bits, s five, so q s IS a bfloat16: every product of such a weight, whether the
+// values are formed in front of the tensor core or the scale is applied behind it, is a product of the same numbers.
+//
+// Rows come in strips of 16, k in blocks of 64.  A block of a strip is 512 bytes of codes, 16 for each lane of a warp: lane 4 r + t
+// holds rows r and r + 8 at k = 16 j + 4 t + {0, 1, 2, 3} in its 32-bit word j.  Those are the A fragment of an m16n8k16 product whose
+// k are taken in the order of the fragment (the B operand's are permuted alike: a lane's four k of 16 are neighbours, one 8-byte
+// load), and the registers that a warp hands to tensor memory with tcgen05.st.16x256b.  Word j, low to high: four times 4 bits of the
+// first k of a pair (rows r, r + 8 at k 4 t; rows r, r + 8 at 4 t + 2), then the same of the second (4 t + 1, 4 t + 3), each q + 8.
+//   codes   [G][strips][ceil(K / 64)][32][16 bytes]
+//   scales  [G][strips][ceil(K / group)][8][2] bfloat16: rows r and r + 8 beside one another
+// Rows beyond N have scale 0, k beyond K q = 0.  A pair (gate rows and up rows, N / 2 each) fills whole strips with either half.
+#pragma once
+#include "common.cuh"
+
+namespace q4 {
+
+constexpr int STRIP = 16, BLOCK_K = 64, BLOCK_BYTES = 512;
+
+struct Weight {
+    const uint4* codes;            // [G][strips][blocks][32]
+    const uint32_t* scales;        // [G][strips][qgroups][8], a pair of bfloat16 each
+    int strips, blocks, qgroups;   // of one group
+    int N, K;                      // rows (of both halves of a pair) and k
+};
+
+// The eight elements of a word as bfloat16 pairs, a[0..3] the fragment's registers: 0x4300 | n is 128 + n, less 136 is q, exactly.
+__device__ __forceinline__ void unpack(uint32_t w, uint32_t (&a)[4]) {
+    const __nv_bfloat162 off = __halves2bfloat162(__ushort_as_bfloat16(0x4308), __ushort_as_bfloat16(0x4308));
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const uint32_t v = ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+        const __nv_bfloat162 q = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), off);
+        a[i] = *reinterpret_cast<const uint32_t*>(&q);
+    }
+}
+__device__ __forceinline__ float scale_lo(uint32_t s) { return __uint_as_float(s << 16); }            // row r
+__device__ __forceinline__ float scale_hi(uint32_t s) { return __uint_as_float(s & 0xffff0000u); }    // row r + 8
+
+// D += A B of one 16 x 16 tile of weights and eight columns of tokens
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], const uint2 b) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y));
+}
+
+// Weights are read once: past L1.
+__device__ __forceinline__ uint4 ld_codes(const uint4* p) {
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint32_t word(const uint4& v, int j) { return j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w; }
+
+// Scales of a block of 64 k: two where a group is 32, one otherwise (the same for two blocks where it is 128).
+template <int GROUP>
+struct Scales {
+    static constexpr int N = GROUP == 32 ? 2 : 1;
+    uint32_t s[N];
+    __device__ __forceinline__ void load(const uint32_t* strip, int block, int qgroups, int r) {      // strip: scales of the strip
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const int q = GROUP == 32 ? 2 * block + i : GROUP == 64 ? block : block >> 1;
+            s[i] = q < qgroups ? __ldg(strip + (size_t)q * 8 + r) : 0u;
+        }
+    }
+};
+
+}  // namespace q4

@@ -185,6 +185,7 @@ STATUS_BITS = {
     4: "routing produced an expert id outside the expert range",
     8: "a bounded wait inside a kernel ran out",
     16: "a gather index lies outside its tensor",
+    32: "a weight to be held in 4 bits is not finite",
 }
 
 

@@ -1,0 +1,228 @@
+"""Python face of the kernel library ``q4``: weights held in 4 bits and the products over them.
+
+A ``Weight4`` stands for a matrix [N, K] or a stack of them [G, N, K].  ``group`` (32, 64 or 128) neighbouring elements of a
+row share a scale s = max |w| / 7 rounded to five significant bits; an element is q s with q = w / s rounded, a whole number from -7 to 7.  q s
+has at most eight significant bits, so it is a bfloat16: a product over a ``Weight4`` is the product over ``dequantize`` of it, but for the
+order of the 32-bit sums.  0.5 + 2 / group bytes an element.
+
+    w4 = quantize(w, group=64)                 # w: float32 or bfloat16, on the device
+    gemm4(x, w4, out, bias=b)                  # out = x w^T (+ b); x bfloat16 [M, K], any M
+    gemm4(x, pair4, out, swiglu=True)          # out = silu(x gate^T) * (x up^T); pair4 = quantize(cat([gate, up]), pair=True)
+    gemm4(xs, stack4, out, group_offsets=o)    # rows [o[g], o[g + 1]) of xs meet stack4[g]
+    experts4(x, idx, w, gate_up4, down4, out)  # a layer of routed experts for up to 8 tokens, in two launches
+
+Everything launches on the current stream of the current device, and a tensor on another device is refused.  The functions may be
+called while a CUDA graph is captured.
+"""
+from __future__ import annotations
+
+import os
+from ctypes import c_float, c_int, c_longlong, c_void_p
+from typing import Optional, Tuple
+
+import torch
+
+from . import build, core
+
+GROUPS = (32, 64, 128)
+EXPERTS_TOKENS = 8            # tokens that ``experts4`` takes
+
+_lib = None
+
+
+def lib():
+    global _lib
+    if _lib is None:
+        L = build.load("q4")
+        P, I, F = c_void_p, c_int, c_float
+        for name, args in (("moe_q4_quantize", [P, I, I, I, I, I, I, P, P, P, P]),
+                           ("moe_q4_dequantize", [P, P, I, I, I, I, I, P, P]),
+                           ("moe_gemm_q4", [P, I, I, P, P, I, I, I, I, I, P, I, I, P, P, I, F, P]),
+                           ("moe_experts_q4", [P, I, I, I, P, P, I, I, I, P, P, P, P, I, P, P, P, P, P, I, P, P, I, I, P, P])):
+            fn = getattr(L, name)
+            fn.argtypes, fn.restype = args, c_int
+        L.moe_experts_q4_scratch.argtypes, L.moe_experts_q4_scratch.restype = [I] * 5, c_longlong
+        L.moe_q4_set_pdl.argtypes, L.moe_q4_set_pdl.restype = [I], None
+        if os.environ.get("MOE_B200_PDL", "1") == "0":      # programmatic dependent launch off
+            L.moe_q4_set_pdl(0)
+        _lib = L
+    return _lib
+
+
+class Weight4:
+    """A matrix ``shape`` = (N, K), or a stack (G, N, K), in 4 bits.
+
+    ``codes``: uint8 [G, strips, ceil(K / 64), 8, 4, 4, 2, 2] (any shape of that many elements): strips of 16 rows; the byte at
+    [.., strip, block, r, t, j, h, p] holds k = 64 block + 16 j + 4 t + 2 p + h of rows r (low four bits) and r + 8 (high four bits) of the
+    strip, each as q + 8.  ``scales``: bfloat16 [G, strips, ceil(K / group), 8, 2], rows r and r + 8 beside one another, each of at most five
+    significant bits.  Rows beyond N have scale 0, elements beyond K q = 0.  With ``pair`` the rows are a gated feed-forward's, N / 2 of
+    the gate and N / 2 of up, and either half fills whole strips; a pair is what products with ``swiglu`` take."""
+
+    __slots__ = ("codes", "scales", "shape", "group", "pair", "G", "N", "K")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, shape: Tuple[int, ...], group: int = 64, pair: bool = False):
+        if len(shape) not in (2, 3) or min(shape) < 1:
+            raise core.KernelError(f"Weight4: the shape is (N, K) or (G, N, K), not {tuple(shape)}")
+        if group not in GROUPS:
+            raise core.KernelError(f"Weight4: the group is one of {GROUPS}, not {group}")
+        self.G, self.N, self.K = (1, *shape) if len(shape) == 2 else shape
+        if pair and self.N % 2:
+            raise core.KernelError("Weight4: a pair has as many gate rows as up rows")
+        strips = self.G * _strips(self.N, pair)
+        if (codes.dtype != torch.uint8 or scales.dtype != torch.bfloat16 or not codes.is_contiguous() or not scales.is_contiguous()
+                or codes.numel() != strips * -(-self.K // 64) * 512 or scales.numel() != strips * -(-self.K // group) * 16
+                or codes.data_ptr() % 16 or scales.data_ptr() % 4 or codes.device != scales.device):
+            raise core.KernelError(f"Weight4: codes and scales of {tuple(shape)} in groups of {group} are contiguous uint8 and bfloat16 tensors "
+                                   f"of {strips * -(-self.K // 64) * 512} and {strips * -(-self.K // group) * 16} elements on one device")
+        self.codes, self.scales, self.shape, self.group, self.pair = codes, scales, tuple(shape), int(group), bool(pair)
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+    @property
+    def nbytes(self) -> int:
+        return self.codes.numel() + 2 * self.scales.numel()
+
+    def __repr__(self):
+        return f"Weight4({'x'.join(map(str, self.shape))}, groups of {self.group}{', pair' if self.pair else ''})"
+
+
+def _strips(N: int, pair: bool) -> int:
+    return 2 * -(-(N // 2) // 16) if pair else -(-N // 16)
+
+
+def _here(device: torch.device, what: str):
+    """A kernel launches on the current device's current stream: its tensors have to lie there."""
+    if device.type != "cuda":
+        raise core.KernelError(f"{what}: expected CUDA tensors; there is no CPU path")
+    if core._raw_device is not None and device.index != core._raw_device():
+        raise core.KernelError(f"{what}: tensors on {device}, but the current device is cuda:{core._raw_device()}")
+
+
+def _on(t: Optional[torch.Tensor], device, name: str, dtype, numel: Optional[int] = None):
+    if t is None:
+        return None
+    if t.dtype != dtype or t.device != device or not t.is_contiguous() or (numel is not None and t.numel() != numel):
+        raise core.KernelError(f"{name}: expected a contiguous {dtype} tensor{'' if numel is None else f' of {numel} elements'} on {device}, got "
+                               f"{t.dtype} {tuple(t.shape)} on {t.device}")
+    return t.data_ptr()
+
+
+def _matrix(t: torch.Tensor, device, name: str, dtypes):
+    if t.dtype not in dtypes or t.device != device or t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise core.KernelError(f"{name}: expected a matrix of {' or '.join(map(str, dtypes))} with dense rows on {device}, got {t.dtype} "
+                               f"{tuple(t.shape)} with strides {t.stride()} on {t.device}")
+
+
+def quantize(w: torch.Tensor, group: int = 64, *, pair: bool = False, status=None) -> Weight4:
+    """The matrix or stack ``w`` (float32 or bfloat16, contiguous) in 4 bits.  A group that holds an infinity or a NaN is marked so that
+    products over it are NaN, and reported through ``status``."""
+    core._chk(w, "w")
+    core._dt(w)
+    _here(w.device, "quantize")
+    if w.dim() not in (2, 3) or not w.numel():
+        raise core.KernelError(f"quantize: a matrix or a stack of matrices, not {tuple(w.shape)}")
+    if group not in GROUPS:
+        raise core.KernelError(f"quantize: the group is one of {GROUPS}, not {group}")
+    G, N, K = (1, *w.shape) if w.dim() == 2 else w.shape
+    if pair and N % 2:
+        raise core.KernelError("quantize: a pair has as many gate rows as up rows")
+    strips = _strips(N, pair)
+    codes = torch.empty((G, strips, -(-K // 64), 8, 4, 4, 2, 2), dtype=torch.uint8, device=w.device)
+    scales = torch.empty((G, strips, -(-K // group), 8, 2), dtype=torch.bfloat16, device=w.device)
+    core._ok(lib().moe_q4_quantize(w.data_ptr(), core._dt(w), G, N, K, group, 1 if pair else 0, codes.data_ptr(), scales.data_ptr(),
+                                   _on(status, w.device, "status", torch.int32), core._stream()), "quantize")
+    return Weight4(codes, scales, tuple(w.shape), group, pair)
+
+
+def dequantize(w: Weight4, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The values that ``w`` stands for, exactly, as bfloat16 of ``w.shape``."""
+    _here(w.device, "dequantize")
+    if out is None:
+        out = torch.empty(w.shape, dtype=torch.bfloat16, device=w.device)
+    elif tuple(out.shape) != w.shape:
+        raise core.KernelError(f"dequantize: out is {tuple(out.shape)}, the weight {w.shape}")
+    core._ok(lib().moe_q4_dequantize(w.codes.data_ptr(), w.scales.data_ptr(), w.G, w.N, w.K, w.group, 1 if w.pair else 0,
+                                     _on(out, w.device, "out", torch.bfloat16), core._stream()), "dequantize")
+    return out
+
+
+def gemm4(x: torch.Tensor, w: Weight4, out: torch.Tensor, *, swiglu: bool = False, bias: Optional[torch.Tensor] = None,
+          group_offsets: Optional[torch.Tensor] = None, act: str = "silu", act_param: float = 0.0, status=None) -> torch.Tensor:
+    """out = x w^T (+ bias), or act(x gate^T) * (x up^T) with ``swiglu`` and a pair; ``act``: as in ``tc.gemm_tc``.
+
+    x: bfloat16 [M, K], dense rows of any pitch; out: float32 or bfloat16 [M, N] (a pair: [M, N / 2]), dense rows of any pitch.
+    A stack needs ``group_offsets`` (int32 [G + 1], ascending): rows [offsets[g], offsets[g + 1]) of x meet w[g]; rows that no group
+    has are left as they were."""
+    dev = x.device
+    _here(dev, "gemm4")
+    _matrix(x, dev, "x", (torch.bfloat16,))
+    _matrix(out, dev, "out", (torch.float32, torch.bfloat16))
+    M, N = x.shape[0], w.N // 2 if swiglu else w.N
+    if w.device != dev or x.shape[1] != w.K or out.shape[0] != M or out.shape[1] != N:
+        raise core.KernelError(f"gemm4: shapes x{tuple(x.shape)} w{w.shape} out{tuple(out.shape)}, on {dev} and {w.device}")
+    if swiglu != w.pair:
+        raise core.KernelError("gemm4: a pair is multiplied with swiglu, another weight without")
+    if swiglu and (bias is not None or act not in core.GLU_ACTS):
+        raise core.KernelError("gemm4: a gated product takes no bias and an activation of core.GLU_ACTS")
+    if not swiglu and act != "silu" and act not in core.PLAIN_ACTS:
+        raise core.KernelError("gemm4: the activation of an ungated product is one of core.PLAIN_ACTS")
+    if group_offsets is None and w.G != 1:
+        raise core.KernelError("gemm4: a stack needs group_offsets")
+    code = core.GLU_ACTS[act] if swiglu else core.PLAIN_ACTS.get(act, 0)
+    if not M:
+        return out
+    core._ok(lib().moe_gemm_q4(x.data_ptr(), x.stride(0), M, w.codes.data_ptr(), w.scales.data_ptr(), w.G, w.N, w.K, w.group, 1 if w.pair else 0,
+                               out.data_ptr(), 1 if out.dtype == torch.bfloat16 else 0, out.stride(0), _on(bias, dev, "bias", torch.float32, N),
+                               _on(group_offsets, dev, "group_offsets", torch.int32, w.G + 1), code, float(act_param), core._stream()), "gemm4")
+    return out
+
+
+def experts4(x: torch.Tensor, topk_idx: torch.Tensor, topk_w: torch.Tensor, gate_up: Weight4, down: Weight4, out: torch.Tensor, *,
+             shared_gate_up: Optional[Weight4] = None, shared_down: Optional[Weight4] = None, shared_gate: Optional[torch.Tensor] = None,
+             status=None) -> bool:
+    """A layer of routed experts for up to 8 tokens, in two launches:
+
+        out_t = sum_j w_tj down_e(silu(gate_e x_t) * (up_e x_t)) + gate_t shared(x_t),   e = idx_tj
+
+    x: bfloat16 [T, H]; topk_idx int32 and topk_w float32 [T, k]; gate_up: a pair's stack [E, 2 I, H], down: [E, H, I]; the shared expert's two
+    likewise without the stack, shared_gate float32 [T] (None: 1); out: float32 or bfloat16 [T, H].  An index of -1 is no pick
+    (all of a row's: zeros but for the shared expert), any other outside [0, E) is reported through ``status`` and taken for none.  False, with
+    nothing launched, for more tokens, 1,024 experts or 512 picks than that."""
+    dev = x.device
+    _here(dev, "experts4")
+    _matrix(x, dev, "x", (torch.bfloat16,))
+    _matrix(out, dev, "out", (torch.float32, torch.bfloat16))
+    T, H = x.shape
+    E, size, k = gate_up.G, gate_up.N // 2, topk_idx.shape[-1] if topk_idx.dim() == 2 else 0
+    if (not gate_up.pair or down.pair or gate_up.K != H or down.G != E or down.N != H or down.K != size or tuple(out.shape) != (T, H)
+            or tuple(topk_idx.shape) != (T, k) or topk_w.shape != topk_idx.shape or gate_up.device != dev or down.device != dev):
+        raise core.KernelError(f"experts4: shapes x{tuple(x.shape)} gate_up{gate_up.shape} down{down.shape} picks{tuple(topk_idx.shape)} "
+                               f"weights{tuple(topk_w.shape)} out{tuple(out.shape)}")
+    shared = 0
+    if (shared_gate_up is None) != (shared_down is None) or (shared_gate is not None and shared_down is None):
+        raise core.KernelError("experts4: the shared expert is a pair and its down projection, its gate goes with them")
+    if shared_gate_up is not None:
+        shared = shared_gate_up.N // 2
+        if (not shared_gate_up.pair or shared_down.pair or shared_gate_up.shape != (2 * shared, H) or shared_down.shape != (H, shared)
+                or shared_gate_up.device != dev or shared_down.device != dev):
+            raise core.KernelError(f"experts4: shapes of the shared expert {shared_gate_up.shape} {shared_down.shape}, on {dev}")
+    if any(w is not None and w.group != gate_up.group for w in (down, shared_gate_up, shared_down)):
+        raise core.KernelError("experts4: the weights of a layer have one group size")
+    pi, pw = _on(topk_idx, dev, "topk_idx", torch.int32), _on(topk_w, dev, "topk_w", torch.float32)
+    pg, ps = _on(shared_gate, dev, "shared_gate", torch.float32, T), _on(status, dev, "status", torch.int32)
+    if T > EXPERTS_TOKENS or E > 1024 or T * k > 512:
+        return False
+    if not T:
+        return True
+    L = lib()
+    scratch = torch.empty(L.moe_experts_q4_scratch(T, k, E, size, shared), dtype=torch.bfloat16, device=dev)
+    s = (None, None, None, None) if not shared else (shared_gate_up.codes.data_ptr(), shared_gate_up.scales.data_ptr(),
+                                                     shared_down.codes.data_ptr(), shared_down.scales.data_ptr())
+    code = L.moe_experts_q4(x.data_ptr(), x.stride(0), T, H, pi, pw, k, E, size, gate_up.codes.data_ptr(), gate_up.scales.data_ptr(),
+                            down.codes.data_ptr(), down.scales.data_ptr(), shared, *s, pg, gate_up.group, scratch.data_ptr(), out.data_ptr(),
+                            1 if out.dtype == torch.bfloat16 else 0, out.stride(0), ps, core._stream())
+    core._ok(code, "experts4")
+    core.launches += 1            # (two kernels)
+    return True
