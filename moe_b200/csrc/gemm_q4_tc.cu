@@ -1,0 +1,487 @@
+// Products of many rows over weights held in 4 bits (the format: quant4.cuh), on the 5th-generation tensor cores.
+//
+// The weight is the MMA's A operand and is read from TENSOR MEMORY: a warp takes the codes of a strip (16 features x 64 k) as they lie in
+// global memory, forms the bfloat16 values q s (exact) in registers and hands them over with tcgen05.st.16x256b, whose register layout is that
+// of the codes.  Nothing of a weight passes through shared memory, which carries the activations alone (TMA, 128-byte swizzle): with A
+// in shared memory too it is what bounds a tile of one SM.  128 features x up to 192 rows a tile; two accumulators (2 x 192 columns) and
+// four stages of A (4 x 32 columns) fill the 512 columns, so the epilogue of a tile runs under the next one's products.
+//
+//   warps 0-7    two groups of four: the codes of every other block of 64 k to values in tensor memory, PREFETCH blocks ahead in registers
+//   warps 8-15   epilogue: accumulator -> registers -> global memory (warp w: lanes 32 (w % 4).., half of the tile's rows)
+//   warp 16      TMA producer of the rows of x, STAGES tiles of [rows x 64]
+//   warp 17      allocates tensor memory and issues the products
+//
+// One CTA an SM walks over the tiles.  A gated pair's tile holds 64 features: gate strips in lanes 32 i.., up strips in lanes 32 i + 16.. .
+// Groups (routed experts): rows [offsets[g], offsets[g + 1]) meet the weights of g.  Where a dense product has too few tiles for the
+// SMs, up to 8 CTAs of a cluster share a tile's k; each leaves its rows of the partial sums in their owners' shared memory and the owner
+// adds them up in the order of the splits.
+//
+// Every wait on a barrier is bounded; one that runs out sets ST_WAIT_TIMEOUT, the roles drain and the CTA frees its tensor memory.
+#include <cuda.h>
+
+#include <mutex>
+
+#include "quant4.cuh"
+
+namespace {
+
+using q4::Weight;
+
+constexpr int FEATURES = 128, BK = 64, BN = 192, STAGES = 8, A_STAGES = 4, A_COLS = 32, NBUF = 2, PREFETCH = 3;
+constexpr int STAGE_BYTES = BN * BK * 2, SMEM = STAGES * STAGE_BYTES + 1024 + 256;
+constexpr int A_COL0 = NBUF * BN, TMEM_COLS = 512, MAX_GROUPS = 1024, MAX_CLUSTER = 8;
+constexpr int DEQUANT_WARPS = 8, EPI_WARPS = 8, WARPS = DEQUANT_WARPS + EPI_WARPS + 2, THREADS = WARPS * 32;
+static_assert(A_COL0 + A_STAGES * A_COLS <= TMEM_COLS, "tensor memory");
+
+struct Args {
+    Weight w;
+    void* out;
+    int out_bf16, ldo;
+    const float* bias;
+    const int* offsets;
+    int G, M, N;                   // N: output features
+    int bn;                        // rows of a tile, a multiple of 16
+    int n_tiles;                   // tiles of features
+    int splits, kb_per_split;
+    int act;
+    float act_param;
+    int* status;
+    uint32_t wait_limit;
+    int test_fault;                // 0; the wait test: 1 nothing is loaded, 2 no product is issued, 3 no value is formed
+};
+
+// ---- PTX wrappers ----------------------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count)); }
+__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok != 0;
+}
+// false: the barrier did not complete in time, or another role gave up
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, const Args& p, int site) {
+    if (mbar_try(bar, parity)) return true;
+    const unsigned long long t0 = global_ns();
+    for (uint32_t i = 1;; i++) {
+        if (mbar_try(bar, parity)) return true;
+        if ((i & 31u) == 0) {
+            if (abort_flag && *abort_flag) return false;
+            if (global_ns() - t0 > (unsigned long long)p.wait_limit * 1000ull) break;
+        }
+    }
+    wait_ran_out(p.status, site);
+    return false;
+}
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst), "l"(map), "r"(x), "r"(y),
+                 "r"(bar)
+                 : "memory");
+}
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+// D[128, N] (+)= A[128, 16] B[N, 16]^T, A in tensor memory (a lane a row, two k a column), B in shared memory
+__device__ __forceinline__ void umma(uint32_t d, uint32_t a, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b_desc), "r"(idesc),
+                 "r"(accumulate)
+                 : "memory");
+}
+__device__ __forceinline__ void umma_commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[16]) {
+    uint32_t r[16];
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
+                   "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(taddr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 16; i++) v[i] = __uint_as_float(r[i]);
+}
+// 16 rows x 64 k of bfloat16: of each 16 k, registers 0 and 1 hold row lane / 4 at k 4 (lane % 4)..., registers 2 and 3 row lane / 4 + 8
+__device__ __forceinline__ void tmem_st_strip(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.16x256b.x4.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
+                 "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// K-major tile with 128-byte swizzle: rows of 128 bytes, groups of 8 rows 1024 bytes apart
+__device__ __forceinline__ uint64_t smem_desc(uint32_t addr) {
+    return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+// 32-bit sums, bfloat16 operands, both K-major
+__device__ __forceinline__ uint32_t instr_desc(int n) { return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(FEATURES >> 4) << 24); }
+
+struct Tile {
+    int g, row0, rows, ft;         // group, first row, rows, tile of features
+};
+__device__ __forceinline__ Tile tile_of(int item, int m_tiles, const Args& p, const int* prefix, const int* offs) {
+    Tile t;
+    if (!p.offsets) {              // all row tiles of a feature tile first: CTAs that run together share its codes in L2
+        t.ft = item / m_tiles, t.g = 0, t.row0 = (item % m_tiles) * p.bn, t.rows = min(p.bn, p.M - t.row0);
+        return t;
+    }
+    const int m = item / p.n_tiles;      // all feature tiles of a row tile first: they share its rows
+    t.ft = item % p.n_tiles;
+    int lo = 0, hi = p.G;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (prefix[mid] <= m) lo = mid; else hi = mid;
+    }
+    t.g = lo, t.row0 = offs[lo] + (m - prefix[lo]) * p.bn, t.rows = min(p.bn, offs[lo + 1] - t.row0);
+    return t;
+}
+
+__device__ __forceinline__ void put(const Args& p, int row, int n, float v) {
+    if (p.out_bf16)
+        ((__nv_bfloat16*)p.out)[(size_t)row * p.ldo + n] = __float2bfloat16_rn(v);
+    else
+        ((float*)p.out)[(size_t)row * p.ldo + n] = v;
+}
+
+template <int GROUP, bool PAIR>
+__global__ void __launch_bounds__(THREADS, 1)
+gemm_q4_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ Args p) {
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ volatile int s_abort;
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_offs[MAX_GROUPS + 1], s_prefix[MAX_GROUPS + 1];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u, bars = base + STAGES * STAGE_BYTES;
+    auto b_full = [&](int s) { return bars + 8u * s; };
+    auto b_empty = [&](int s) { return bars + 8u * (STAGES + s); };
+    auto a_full = [&](int s) { return bars + 8u * (2 * STAGES + s); };
+    auto a_empty = [&](int s) { return bars + 8u * (2 * STAGES + A_STAGES + s); };
+    auto acc_full = [&](int b) { return bars + 8u * (2 * STAGES + 2 * A_STAGES + b); };
+    auto acc_empty = [&](int b) { return bars + 8u * (2 * STAGES + 2 * A_STAGES + NBUF + b); };
+    const uint32_t drained = bars + 8u * (2 * STAGES + 2 * A_STAGES + 2 * NBUF);
+    if (threadIdx.x == 0) {
+        s_abort = 0;
+        for (int s = 0; s < STAGES; s++) mbar_init(b_full(s), 1), mbar_init(b_empty(s), 1);
+        for (int s = 0; s < A_STAGES; s++) mbar_init(a_full(s), 4), mbar_init(a_empty(s), 1);
+        for (int b = 0; b < NBUF; b++) mbar_init(acc_full(b), 1), mbar_init(acc_empty(b), EPI_WARPS);
+        mbar_init(drained, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == WARPS - 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(TMEM_COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    int m_tiles = (p.M + p.bn - 1) / p.bn;
+    if (p.offsets) {
+        pdl_sync();
+        for (int i = threadIdx.x; i <= p.G; i += THREADS) s_offs[i] = min(p.M, max(0, p.offsets[i]));
+        __syncthreads();
+        if (warp == 0) {                                 // row tiles of the groups before each
+            int run = 0;
+            for (int g0 = 0; g0 < p.G; g0 += 32) {
+                const int g = g0 + lane, n = g < p.G ? max(0, s_offs[g + 1] - s_offs[g] + p.bn - 1) / p.bn : 0;
+                int upto = n;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int v = __shfl_up_sync(0xffffffffu, upto, o);
+                    if (lane >= o) upto += v;
+                }
+                if (g < p.G) s_prefix[g] = run + upto - n;
+                run += __shfl_sync(0xffffffffu, upto, 31);
+            }
+            if (lane == 0) s_prefix[p.G] = run;
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = s_tmem;
+    if (p.offsets) m_tiles = s_prefix[p.G];
+    const int items = m_tiles * p.n_tiles, rank = p.splits > 1 ? (int)cluster_ctarank() : 0;
+    const int kb0 = rank * p.kb_per_split, kbs = min(p.w.blocks, kb0 + p.kb_per_split) - kb0;
+    const int mine = (int)blockIdx.x < items ? (items - 1 - (int)blockIdx.x) / (int)gridDim.x + 1 : 0;      // tiles of this CTA
+    const int total = mine * kbs;
+
+    if (warp < DEQUANT_WARPS) {
+        // ---- codes to values: block `it` of the CTA's sequence by the warps of group it % 2 --------------------------------------------
+        const int q = warp & 3, r = lane >> 2;
+        uint4 code[PREFETCH][2];
+        q4::Scales<GROUP> sc[PREFETCH][2];
+        int next = warp >> 2, next_item = -1;
+        Tile t;
+        auto load = [&](int d) {                         // the block `next` into place d
+            if (next < total) {
+                const int li = next / kbs, kb = kb0 + next - li * kbs;
+                if (li != next_item) t = tile_of(blockIdx.x + li * gridDim.x, m_tiles, p, s_prefix, s_offs), next_item = li;
+                const int half = PAIR ? p.w.strips / 2 : p.w.strips;
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const int strip = PAIR ? t.ft * 4 + q : t.ft * 8 + 2 * q + i;
+                    if (strip < half) {
+                        const size_t s = (size_t)t.g * p.w.strips + strip + (PAIR && i ? half : 0);
+                        code[d][i] = __ldg(p.w.codes + (s * p.w.blocks + kb) * 32 + lane);
+                        sc[d][i].load(p.w.scales + s * p.w.qgroups * 8, kb, p.w.qgroups, r);
+                    } else {
+                        code[d][i] = make_uint4(0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u);
+                        sc[d][i] = q4::Scales<GROUP>{};
+                    }
+                }
+            }
+            next += 2;
+        };
+#pragma unroll
+        for (int d = 0; d < PREFETCH; d++) load(d);
+        bool ok = p.test_fault != 3;
+        for (int it0 = warp >> 2; it0 < total && ok; it0 += 2 * PREFETCH) {
+#pragma unroll
+            for (int d = 0; d < PREFETCH; d++) {
+                const int it = it0 + 2 * d;
+                if (it >= total || !ok) break;
+                const int s = it % A_STAGES;
+                uint32_t v[2][16];
+#pragma unroll
+                for (int i = 0; i < 2; i++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        uint32_t a[4];
+                        q4::unpack(q4::word(code[d][i], j), a);
+                        const uint32_t s2 = sc[d][i].s[GROUP == 32 ? j / 2 : 0];
+                        const uint32_t lo2 = __byte_perm(s2, 0, 0x1010), hi2 = __byte_perm(s2, 0, 0x3232);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {      // registers of the fragment: rows r, r + 8, r, r + 8; of the store: r, r, r + 8, r + 8
+                            const uint32_t m = (e & 1) ? hi2 : lo2;
+                            const __nv_bfloat162 y = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&a[e]), *reinterpret_cast<const __nv_bfloat162*>(&m));
+                            v[i][4 * j + 2 * (e & 1) + (e >> 1)] = *reinterpret_cast<const uint32_t*>(&y);
+                        }
+                    }
+                ok = mbar_wait(a_empty(s), ((it / A_STAGES) & 1) ^ 1, &s_abort, p, 0x56);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t at = tmem + A_COL0 + s * A_COLS + ((uint32_t)(q * 32) << 16);
+                tmem_st_strip(at, v[0]);
+                tmem_st_strip(at + (16u << 16), v[1]);
+                load(d);
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(a_full(s));
+            }
+        }
+        if (!ok && p.test_fault != 3) s_abort = 1;
+    } else if (warp < DEQUANT_WARPS + EPI_WARPS) {
+        // ---- epilogue -------------------------------------------------------------------------------------------------------------------
+        if (p.splits == 1) {
+            const int q = warp & 3, h = (warp - DEQUANT_WARPS) >> 2;
+            bool ok = true;
+            for (int li = 0; li < mine && ok; li++) {
+                const Tile t = tile_of(blockIdx.x + li * gridDim.x, m_tiles, p, s_prefix, s_offs);
+                const int b = li % NBUF;
+                ok = mbar_wait(acc_full(b), (li / NBUF) & 1, &s_abort, p, 0x55);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t taddr = tmem + b * BN + ((uint32_t)(q * 32) << 16);
+                const bool upper = PAIR && (lane & 16);
+                const int n = PAIR ? t.ft * 64 + q * 16 + (lane & 15) : t.ft * FEATURES + q * 32 + lane;
+                const float bias = !PAIR && p.bias && n < p.N ? p.bias[n] : 0.f;
+                const int part = ((t.rows + 31) / 32) * 16, lo = h * part, hi = min(t.rows, lo + part);
+                for (int c0 = lo; c0 < hi; c0 += 16) {
+                    float a[16];
+                    __syncwarp();
+                    tmem_ld16(taddr + c0, a);
+                    if (PAIR) {
+#pragma unroll
+                        for (int j = 0; j < 16; j += 2) {
+                            const float recv = __shfl_xor_sync(0xffffffffu, upper ? a[j] : a[j + 1], 16);
+                            const float g = upper ? recv : a[j], u = upper ? a[j + 1] : recv;
+                            const int c = c0 + j + (upper ? 1 : 0);
+                            if (c < hi && n < p.N) put(p, t.row0 + c, n, glu_mul(p.act, p.act_param, g, u));
+                        }
+                    } else if (n < p.N) {
+#pragma unroll
+                        for (int j = 0; j < 16; j++)
+                            if (c0 + j < hi) put(p, t.row0 + c0 + j, n, plain_act(p.act, a[j] + bias));
+                    }
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(acc_empty(b));
+            }
+            if (!ok) s_abort = 1;
+        }
+    } else if (warp == WARPS - 2) {
+        // ---- rows of x -------------------------------------------------------------------------------------------------------------------
+        if (lane == 0) {
+            if (!p.offsets) pdl_sync();
+            int it = 0;
+            bool ok = p.test_fault != 1;
+            for (int li = 0; li < mine && ok; li++) {
+                const Tile t = tile_of(blockIdx.x + li * gridDim.x, m_tiles, p, s_prefix, s_offs);
+                const int boxes = (t.rows + 63) / 64;
+                for (int kb = 0; kb < kbs; kb++, it++) {
+                    const int s = it % STAGES;
+                    ok = mbar_wait(b_empty(s), ((it / STAGES) & 1) ^ 1, &s_abort, p, 0x51);
+                    if (!ok) break;
+                    mbar_expect_tx(b_full(s), boxes * 64 * BK * 2);
+                    for (int c = 0; c < boxes; c++) tma_load_2d(base + s * STAGE_BYTES + c * 64 * BK * 2, &tmX, (kb0 + kb) * BK, t.row0 + c * 64, b_full(s));
+                }
+            }
+            if (!ok && p.test_fault != 1) {
+                s_abort = 1;
+                for (int i = max(0, it - STAGES); i < it; i++) mbar_wait(b_full(i % STAGES), (i / STAGES) & 1, nullptr, p, 0x52);      // copies in flight must land
+            }
+        }
+    } else {
+        // ---- products --------------------------------------------------------------------------------------------------------------------
+        if (lane == 0) {
+            int it = 0;
+            bool ok = p.test_fault != 2;
+            for (int li = 0; li < mine && ok; li++) {
+                const Tile t = tile_of(blockIdx.x + li * gridDim.x, m_tiles, p, s_prefix, s_offs);
+                const uint32_t idesc = instr_desc((t.rows + 15) & ~15);
+                const int b = li % NBUF;
+                ok = mbar_wait(acc_empty(b), ((li / NBUF) & 1) ^ 1, &s_abort, p, 0x53);
+                if (!ok) break;
+                for (int kb = 0; kb < kbs; kb++, it++) {
+                    const int s = it % STAGES, a = it % A_STAGES;
+                    ok = mbar_wait(b_full(s), (it / STAGES) & 1, &s_abort, p, 0x54) && mbar_wait(a_full(a), (it / A_STAGES) & 1, &s_abort, p, 0x57);
+                    if (!ok) break;
+                    tc_fence_after();
+#pragma unroll
+                    for (int k4 = 0; k4 < BK / 16; k4++)
+                        umma(tmem + b * BN, tmem + A_COL0 + a * A_COLS + k4 * 8, smem_desc(base + s * STAGE_BYTES + k4 * 32), idesc, kb > 0 || k4 > 0);
+                    umma_commit(b_empty(s));
+                    umma_commit(a_empty(a));
+                }
+                if (ok) umma_commit(acc_full(b));
+            }
+            if (!ok && p.test_fault != 2) s_abort = 1;
+            umma_commit(drained);                        // tensor memory is given back only behind the last product
+            mbar_wait(drained, 0, nullptr, p, 0x58);
+        }
+        __syncwarp();
+    }
+    if (p.splits > 1) {
+        // ---- a tile's k splits: rows [r cpo, (r + 1) cpo) of the tile belong to rank r ------------------------------------------------------
+        tc_fence_before();
+        __syncthreads();
+        tc_fence_after();
+        cluster_sync_all();                              // every CTA's products are done: the stages are free to receive
+        const Tile t = tile_of(blockIdx.x, m_tiles, p, s_prefix, s_offs);
+        const int S = p.splits, cpo = (t.rows + S - 1) / S;
+        const bool fine = !s_abort;
+        if (warp >= DEQUANT_WARPS && warp < DEQUANT_WARPS + EPI_WARPS && fine) {
+            const int q = warp & 3, h = (warp - DEQUANT_WARPS) >> 2;
+            const uint32_t taddr = tmem + ((uint32_t)(q * 32) << 16);
+            const int part = ((t.rows + 31) / 32) * 16, lo = h * part, hi = min(t.rows, lo + part);
+            for (int c0 = lo; c0 < hi; c0 += 16) {
+                float a[16];
+                __syncwarp();
+                tmem_ld16(taddr + c0, a);
+#pragma unroll
+                for (int j = 0; j < 16; j++) {
+                    const int c = c0 + j, owner = c / cpo;
+                    if (c < hi) st_cluster_f32(mapa_cluster(base + (uint32_t)((rank * cpo + c - owner * cpo) * FEATURES + q * 32 + lane) * 4u, owner), a[j]);
+                }
+            }
+        }
+        __syncwarp();
+        cluster_sync_all();
+        const float* recv = reinterpret_cast<const float*>(smem_raw + (base - smem_u32(smem_raw)));
+        const int first = rank * cpo, cols = min(cpo, t.rows - first), per = PAIR ? 64 : FEATURES;
+        for (int i = threadIdx.x; i < cols * per && fine; i += THREADS) {
+            const int c = i / per, f = i - c * per, n = t.ft * per + f;
+            if (n >= p.N) continue;
+            const int l = PAIR ? (f >> 4) * 32 + (f & 15) : f;
+            float a = 0.f, b = 0.f;
+            for (int s = 0; s < S; s++) {
+                a += recv[(s * cpo + c) * FEATURES + l];
+                if (PAIR) b += recv[(s * cpo + c) * FEATURES + l + 16];
+            }
+            const float v = PAIR ? glu_mul(p.act, p.act_param, a, b) : plain_act(p.act, p.bias ? a + p.bias[n] : a);
+            put(p, t.row0 + first + c, n, v);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == WARPS - 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
+    }
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
+                                  CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiledFn encode_fn() {
+    static EncodeTiledFn fn = [] {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult st;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &st) != cudaSuccess || st != cudaDriverEntryPointSuccess) return (EncodeTiledFn) nullptr;
+        return (EncodeTiledFn)f;
+    }();
+    return fn;
+}
+
+uint32_t g_wait_limit = WAIT_LIMIT_US;
+int g_test_fault = 0;
+
+template <int GROUP, bool PAIR>
+int launch(const CUtensorMap& map, const Args& p, unsigned ctas, cudaStream_t stream) {
+    // (the attribute belongs to a device's copy of the kernel: set per launch it costs a fraction of a microsecond and is right on every device)
+    const cudaError_t e = cudaFuncSetAttribute(gemm_q4_tc_kernel<GROUP, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+    if (e != cudaSuccess) return (int)e;
+    return launch_pdl_cluster(gemm_q4_tc_kernel<GROUP, PAIR>, dim3(ctas, 1, p.splits), dim3(THREADS), (size_t)SMEM, stream, p.splits, map, p);
+}
+
+}  // namespace
+
+// The same product as moe_gemm_q4 by the kernel above.  Returns -1, with nothing launched, for what it does not take: K or a row pitch of x that is no
+// multiple of 8, an unaligned x, more than 1,024 groups.
+MOE_API int moe_gemm_q4_tc(const void* x, int ldx, int M, const void* codes, const void* scales, int G, int N, int K, int group, int pair, void* out,
+                           int out_bf16, int ldo, const float* bias, const int* offsets, int act, float act_param, int splits, int* status, cudaStream_t stream) {
+    if (M <= 0 || N <= 0) return 0;
+    if (!x || !codes || !scales || !out || !status || K <= 0 || G <= 0 || (G > 1 && !offsets) || (pair && N % 2)) return (int)cudaErrorInvalidValue;
+    if (K % 8 || ldx % 8 || ((uintptr_t)x & 15) || G > MAX_GROUPS || !encode_fn()) return -1;
+    CUtensorMap map;
+    const cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)M}, strides[1] = {(cuuint64_t)ldx * 2};
+    const cuuint32_t box[2] = {BK, 64}, estr[2] = {1, 1};
+    if (encode_fn()(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(x), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+        return -1;
+    Args p = {};
+    p.w.codes = (const uint4*)codes, p.w.scales = (const uint32_t*)scales, p.w.N = N, p.w.K = K;
+    p.N = pair ? N / 2 : N;
+    p.w.strips = (p.N + 15) / 16 * (pair ? 2 : 1), p.w.blocks = (K + 63) / 64, p.w.qgroups = (K + group - 1) / group;
+    p.out = out, p.out_bf16 = out_bf16, p.ldo = ldo, p.bias = bias, p.offsets = offsets, p.G = G, p.M = M;
+    p.act = act, p.act_param = act_param, p.status = status, p.wait_limit = g_wait_limit, p.test_fault = g_test_fault;
+    p.n_tiles = pair ? (p.N + 63) / 64 : (p.N + FEATURES - 1) / FEATURES;
+    // rows of a tile: as few tiles as 192 rows allow, of equal height
+    const int mt = (M + BN - 1) / BN;
+    p.bn = offsets ? BN : ((M + mt - 1) / mt + 15) / 16 * 16;
+    int dev = 0, sms = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    if (e != cudaSuccess) return (int)e;
+    const long long tiles = (offsets ? (long long)(M < G ? M : G) + M / BN : (long long)((M + p.bn - 1) / p.bn)) * p.n_tiles;
+    if (tiles > 0x3fffffff) return -1;
+    if (offsets || splits < 1) splits = 1;
+    if (splits > MAX_CLUSTER) splits = MAX_CLUSTER;
+    if (splits > p.w.blocks) splits = p.w.blocks;
+    p.kb_per_split = (p.w.blocks + splits - 1) / splits;
+    p.splits = (p.w.blocks + p.kb_per_split - 1) / p.kb_per_split;
+    const unsigned ctas = p.splits > 1 ? (unsigned)tiles : (unsigned)(tiles < sms ? tiles : sms);
+    switch (group) {
+        case 32: return pair ? launch<32, true>(map, p, ctas, stream) : launch<32, false>(map, p, ctas, stream);
+        case 64: return pair ? launch<64, true>(map, p, ctas, stream) : launch<64, false>(map, p, ctas, stream);
+        case 128: return pair ? launch<128, true>(map, p, ctas, stream) : launch<128, false>(map, p, ctas, stream);
+    }
+    return (int)cudaErrorInvalidValue;
+}
+
+// For the test of the bounded waits only: ``fault`` 1: nothing of x is loaded, 2: no product is issued, 3: no values are formed, so that the other
+// roles' waits run out after ``wait_limit`` microseconds (0: the normal limit).  (0, 0) restores the normal behaviour.
+MOE_API void moe_q4_set_wait_test(int fault, unsigned wait_limit) {
+    g_test_fault = fault >= 1 && fault <= 3 ? fault : 0;
+    g_wait_limit = wait_limit ? wait_limit : WAIT_LIMIT_US;
+}

@@ -39,7 +39,7 @@ LIBRARIES: Dict[str, List[str]] = {
     # tcgen05 / TMA kernels of the bfloat16 path; a float32 model never builds or loads them
     "tc": ["gemm_tc.cu", "attention_prefill.cu", "attention_prefill_tc.cu"],
     # weights held in 4 bits; only a model that has them builds or loads it
-    "q4": ["quant4.cu", "gemm_q4.cu"],
+    "q4": ["quant4.cu", "gemm_q4.cu", "gemm_q4_tc.cu"],
     # host side of a step (cache ledger, step packing): plain C++, no CUDA
     "host": ["host_runtime.cpp"],
 }

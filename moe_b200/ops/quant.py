@@ -17,7 +17,7 @@ called while a CUDA graph is captured.
 from __future__ import annotations
 
 import os
-from ctypes import c_float, c_int, c_longlong, c_void_p
+from ctypes import c_float, c_int, c_longlong, c_uint, c_void_p
 from typing import Optional, Tuple
 
 import torch
@@ -26,6 +26,7 @@ from . import build, core
 
 GROUPS = (32, 64, 128)
 EXPERTS_TOKENS = 8            # tokens that ``experts4`` takes
+FEW_ROWS = 16                 # rows up to which a product streams its weights through registers
 
 _lib = None
 
@@ -38,10 +39,12 @@ def lib():
         for name, args in (("moe_q4_quantize", [P, I, I, I, I, I, I, P, P, P, P]),
                            ("moe_q4_dequantize", [P, P, I, I, I, I, I, P, P]),
                            ("moe_gemm_q4", [P, I, I, P, P, I, I, I, I, I, P, I, I, P, P, I, F, P]),
+                           ("moe_gemm_q4_tc", [P, I, I, P, P, I, I, I, I, I, P, I, I, P, P, I, F, I, P, P]),
                            ("moe_experts_q4", [P, I, I, I, P, P, I, I, I, P, P, P, P, I, P, P, P, P, P, I, P, P, I, I, P, P])):
             fn = getattr(L, name)
             fn.argtypes, fn.restype = args, c_int
         L.moe_experts_q4_scratch.argtypes, L.moe_experts_q4_scratch.restype = [I] * 5, c_longlong
+        L.moe_q4_set_wait_test.argtypes, L.moe_q4_set_wait_test.restype = [I, c_uint], None
         L.moe_q4_set_pdl.argtypes, L.moe_q4_set_pdl.restype = [I], None
         if os.environ.get("MOE_B200_PDL", "1") == "0":      # programmatic dependent launch off
             L.moe_q4_set_pdl(0)
@@ -173,10 +176,26 @@ def gemm4(x: torch.Tensor, w: Weight4, out: torch.Tensor, *, swiglu: bool = Fals
     code = core.GLU_ACTS[act] if swiglu else core.PLAIN_ACTS.get(act, 0)
     if not M:
         return out
-    core._ok(lib().moe_gemm_q4(x.data_ptr(), x.stride(0), M, w.codes.data_ptr(), w.scales.data_ptr(), w.G, w.N, w.K, w.group, 1 if w.pair else 0,
-                               out.data_ptr(), 1 if out.dtype == torch.bfloat16 else 0, out.stride(0), _on(bias, dev, "bias", torch.float32, N),
-                               _on(group_offsets, dev, "group_offsets", torch.int32, w.G + 1), code, float(act_param), core._stream()), "gemm4")
+    args = (x.data_ptr(), x.stride(0), M, w.codes.data_ptr(), w.scales.data_ptr(), w.G, w.N, w.K, w.group, 1 if w.pair else 0, out.data_ptr(),
+            1 if out.dtype == torch.bfloat16 else 0, out.stride(0), _on(bias, dev, "bias", torch.float32, N),
+            _on(group_offsets, dev, "group_offsets", torch.int32, w.G + 1), code, float(act_param))
+    st = _on(status, dev, "status", torch.int32)
+    if M > FEW_ROWS and st is not None:
+        done = lib().moe_gemm_q4_tc(*args, 1 if group_offsets is not None else _splits(M, N, w, dev), st, core._stream())
+        if done != -1:
+            core._ok(done, "gemm4")
+            return out
+    core._ok(lib().moe_gemm_q4(*args, core._stream()), "gemm4")
     return out
+
+
+def _splits(M: int, N: int, w: Weight4, device) -> int:
+    """K splits of a tensor-core product: as many as find SMs for all tiles of 128 features (64 of a pair) and up to 192 rows, 4 blocks of 64 k
+    and more each."""
+    from . import tc
+
+    tiles = -(-M // 192) * -(-N // (64 if w.pair else 128))
+    return max(1, min(8, tc.num_sms(device) // tiles, -(-w.K // 64) // 4))
 
 
 def experts4(x: torch.Tensor, topk_idx: torch.Tensor, topk_w: torch.Tensor, gate_up: Weight4, down: Weight4, out: torch.Tensor, *,
