@@ -2,221 +2,123 @@
 //
 //   y[m, n] = sum_k x[m, k] q[n, k] s[n, k / group] (+ b[n]), or act(gate) * up of a pair's two rows.
 //
-// What bounds them is the stream of codes, 0.53 bytes an element, and close behind it the issue slots: 6.5 TB/s are 46 elements a cycle and
-// SM.  So an element costs about two thirds of an instruction: the weights are the A operand of m16n8k16 products straight from the registers
-// that they were loaded to (two shifts, masks and subtractions a pair of elements, no shared memory), a product takes eight rows of x for the price of
-// one, and the scale is applied to the sums of a group's 64 k (four products from zero, then one multiply-add an output), which also keeps
-// the sums in plain 32-bit additions but for those 64.  A warp takes every W-th block of 64 k of its strip, so a block of W warps reads
-// W * 512 neighbouring bytes; D blocks a warp are in flight, the first ones asked for before the wait on the predecessor.  The warps'
-// sums are added up through shared memory in the order of the warps.
+// What bounds them is the stream of codes, 0.53 bytes an element, and close behind it the issue slots and the logic unit: 6.5 TB/s are 46
+// elements a cycle and SM.  So the weights are the A operand of m16n8k16 products straight from the registers that they come in (a shift,
+// a mask and a subtraction a pair of elements), a product takes eight rows of x for the price of one, and the scale is applied to the sums
+// of a group's k (up to four products from zero, then one multiply-add an output), which also keeps the sums in plain 32-bit additions but
+// for those 64.  The warps that share a strip's k add their sums up through shared memory in the order of the warps.
+//
+//   gemm_q4_direct_kernel    few strips: a block of eight warps a strip, codes and rows straight to registers, all asked for at once
+//   gemm_q4_stream_kernel    many: one block an SM, its codes by bulk copies into stages, the rows' fragments in shared memory
+//   experts_down_kernel      the second half of a layer of experts
 #include "quant4.cuh"
 
 namespace {
 
 using q4::Weight;
+using q4::lds16;
+using q4::lds4;
+using q4::smem_u32;
+using q4::sts8;
 
-struct Rows {
-    const __nv_bfloat16* x;        // [M, K], pitch ldx
-    int ldx, vec;                  // vec: rows of whole 8-byte units
-};
+// Four neighbouring k of a row, zeros beyond K or where there is no row.
+__device__ __forceinline__ uint2 row4(const __nv_bfloat16* row, int k, int K, int vec) {
+    if (!row || k >= K) return make_uint2(0u, 0u);
+    if (vec) return *reinterpret_cast<const uint2*>(row + k);
+    uint32_t e[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) e[i] = k + i < K ? (uint32_t)__bfloat16_as_ushort(row[k + i]) : 0u;
+    return make_uint2(e[0] | (e[1] << 16), e[2] | (e[3] << 16));
+}
 
-// The four B registers pairs of a block of 64 k for the lane's row (null: zeros)
-__device__ __forceinline__ void load_rows(const __nv_bfloat16* row, int k0, int K, int vec, int t, uint2 (&b)[4]) {
+// acc += 64 k of MT strips against NT tiles of eight rows (x[n][j]: the B registers of 16 k), the group's scale on the sums of its k.  The strips'
+// products alternate: one waits for itself.
+template <int MT, int NT, int GROUP>
+__device__ __forceinline__ void block_product(const uint4 (&code)[MT], const uint32_t (&sc)[MT][q4::Scales<GROUP>::N], const uint2 (&x)[NT][4], const q4::Bits& bits,
+                                              float (&acc)[MT][NT][4]) {
+    constexpr int SETS = q4::Scales<GROUP>::N, WORDS = 4 / SETS;
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-        const int k = k0 + 16 * j + 4 * t;
-        b[j] = make_uint2(0u, 0u);
-        if (!row) continue;
-        if (vec) {
-            if (k < K) b[j] = *reinterpret_cast<const uint2*>(row + k);
-        } else {
-            uint32_t e[4];
+    for (int h = 0; h < SETS; h++) {
+        float c[MT][NT][4];
 #pragma unroll
-            for (int i = 0; i < 4; i++) e[i] = k + i < K ? (uint32_t)__bfloat16_as_ushort(row[k + i]) : 0u;
-            b[j] = make_uint2(e[0] | (e[1] << 16), e[2] | (e[3] << 16));
+        for (int i = 0; i < WORDS; i++) {
+            const int j = h * WORDS + i;
+#pragma unroll
+            for (int m = 0; m < MT; m++) {
+                uint32_t a[4];
+                q4::unpack(q4::word(code[m], j), bits, a);
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    if (i == 0)
+                        q4::mma(c[m][n], a, x[n][j].x, x[n][j].y, 0.f, 0.f, 0.f, 0.f);
+                    else
+                        q4::mma(c[m][n], a, x[n][j].x, x[n][j].y, c[m][n][0], c[m][n][1], c[m][n][2], c[m][n][3]);
+                }
+            }
+        }
+#pragma unroll
+        for (int m = 0; m < MT; m++) {
+            const float lo = q4::scale_lo(sc[m][h]), hi = q4::scale_hi(sc[m][h]);
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                acc[m][n][0] = fmaf(lo, c[m][n][0], acc[m][n][0]), acc[m][n][1] = fmaf(lo, c[m][n][1], acc[m][n][1]);
+                acc[m][n][2] = fmaf(hi, c[m][n][2], acc[m][n][2]), acc[m][n][3] = fmaf(hi, c[m][n][3], acc[m][n][3]);
+            }
         }
     }
 }
 
-// acc += one block of 64 k of MT strips against NT tiles of eight rows
-template <int MT, int NT, int GROUP>
-__device__ __forceinline__ void block_product(const uint4 (&code)[MT], const q4::Scales<GROUP> (&sc)[MT], const uint2 (&b)[NT][4], float (&acc)[MT][NT][4]) {
-#pragma unroll
-    for (int m = 0; m < MT; m++)
-#pragma unroll
-        for (int h = 0; h < q4::Scales<GROUP>::N; h++) {
-            constexpr int WORDS = 4 / q4::Scales<GROUP>::N;
-            float c[NT][4];
-#pragma unroll
-            for (int n = 0; n < NT; n++) c[n][0] = c[n][1] = c[n][2] = c[n][3] = 0.f;
-#pragma unroll
-            for (int i = 0; i < WORDS; i++) {
-                uint32_t a[4];
-                q4::unpack(q4::word(code[m], h * WORDS + i), a);
-#pragma unroll
-                for (int n = 0; n < NT; n++) q4::mma(c[n], a, b[n][h * WORDS + i]);
-            }
-            const float lo = q4::scale_lo(sc[m].s[h]), hi = q4::scale_hi(sc[m].s[h]);
-#pragma unroll
-            for (int n = 0; n < NT; n++) {
-                acc[m][n][0] = fmaf(lo, c[n][0], acc[m][n][0]), acc[m][n][1] = fmaf(lo, c[n][1], acc[m][n][1]);
-                acc[m][n][2] = fmaf(hi, c[n][2], acc[m][n][2]), acc[m][n][3] = fmaf(hi, c[n][3], acc[m][n][3]);
-            }
-        }
-}
-
-// The sums of W warps, added up in order: red [W][MT][8 NT][16 + 1]; thread i gets output i of MT * 8 NT * 16 (rows of the strip fastest)
-template <int MT, int NT>
-__device__ __forceinline__ void leave_sums(float* red, int warp, int lane, const float (&acc)[MT][NT][4]) {
+// The sums of a team's warps over one tile of eight rows: red [W][MT][8][17] (features of the strip fastest)
+template <int MT>
+__device__ __forceinline__ void leave_sums(float* red, int warp, int lane, int m, const float (&acc)[4]) {
     const int r = lane >> 2, t = lane & 3;
 #pragma unroll
-    for (int m = 0; m < MT; m++)
-#pragma unroll
-        for (int n = 0; n < NT; n++)
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-                red[((warp * MT + m) * 8 * NT + 8 * n + 2 * t + (i & 1)) * 17 + r + 8 * (i >> 1)] = acc[m][n][i];
+    for (int i = 0; i < 4; i++) red[((warp * MT + m) * 8 + 2 * t + (i & 1)) * 17 + r + 8 * (i >> 1)] = acc[i];
 }
-template <int W, int MT, int NT>
+template <int W, int MT>
 __device__ __forceinline__ float sum_of(const float* red, int m, int col, int row) {
     float v = 0.f;
 #pragma unroll
-    for (int w = 0; w < W; w++) v += red[((w * MT + m) * 8 * NT + col) * 17 + row];
+    for (int w = 0; w < W; w++) v += red[((w * MT + m) * 8 + col) * 17 + row];
     return v;
 }
-
-struct GemmArgs {
-    Weight w;
-    Rows rows;
-    void* out;
-    int out_bf16, ldo;
-    const float* bias;
-    const int* offsets;            // null: one group of M rows
-    int M, N;                      // N: output features (of a pair: of one half)
-    int act;
-    float act_param;
-};
-
-constexpr int DEPTH = 4;           // blocks of a warp in flight
-
-// Grid: (strips of the output, groups, 1).  MT 2: a pair's gate and up strip.
-template <int W, int MT, int NT, int GROUP>
-__global__ void __launch_bounds__(W * 32)
-gemm_q4_kernel(const __grid_constant__ GemmArgs p) {
-    __shared__ float red[W * MT * 8 * NT * 17];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
-    const int strip = blockIdx.x, g = blockIdx.y, blocks = p.w.blocks;
-    const uint4* codes[MT];
-    const uint32_t* scales[MT];
-#pragma unroll
-    for (int m = 0; m < MT; m++) {
-        const size_t s = (size_t)g * p.w.strips + strip + m * (p.w.strips / 2);
-        codes[m] = p.w.codes + s * blocks * 32 + lane;
-        scales[m] = p.w.scales + s * p.w.qgroups * 8;
-    }
-    int row0 = 0, row_end = p.M;
-    bool waited = false;
-    if (p.offsets) {                                     // (written by an earlier kernel, maybe the predecessor)
-        pdl_sync();
-        waited = true;
-        row0 = max(0, p.offsets[g]), row_end = min(p.M, p.offsets[g + 1]);
-        if (row0 >= row_end) return;
-    }
-    for (; row0 < row_end; row0 += 8 * NT) {
-        uint4 code[DEPTH][MT];
-        q4::Scales<GROUP> sc[DEPTH][MT];
-        float acc[MT][NT][4];
-#pragma unroll
-        for (int m = 0; m < MT; m++)
-#pragma unroll
-            for (int n = 0; n < NT; n++) acc[m][n][0] = acc[m][n][1] = acc[m][n][2] = acc[m][n][3] = 0.f;
-        auto load = [&](int d, int b) {
-#pragma unroll
-            for (int m = 0; m < MT; m++) {
-                code[d][m] = q4::ld_codes(codes[m] + (size_t)b * 32);
-                sc[d][m].load(scales[m], b, p.w.qgroups, r);
-            }
-        };
-#pragma unroll
-        for (int d = 0; d < DEPTH; d++)
-            if (warp + d * W < blocks) load(d, warp + d * W);
-        if (!waited) pdl_sync();
-        waited = true;
-        const __nv_bfloat16* xr[NT];
-#pragma unroll
-        for (int n = 0; n < NT; n++) xr[n] = row0 + 8 * n + r < row_end ? p.rows.x + (size_t)(row0 + 8 * n + r) * p.rows.ldx : nullptr;
-        for (int b0 = warp; b0 < blocks; b0 += DEPTH * W) {
-#pragma unroll
-            for (int d = 0; d < DEPTH; d++) {
-                const int b = b0 + d * W;
-                if (b >= blocks) break;
-                uint2 x[NT][4];
-#pragma unroll
-                for (int n = 0; n < NT; n++) load_rows(xr[n], b * 64, p.w.K, p.rows.vec, t, x[n]);
-                block_product<MT, NT, GROUP>(code[d], sc[d], x, acc);
-                if (b + DEPTH * W < blocks) load(d, b + DEPTH * W);
-            }
-        }
-        leave_sums<MT, NT>(red, warp, lane, acc);
-        __syncthreads();
-        for (int i = threadIdx.x; i < 8 * NT * 16; i += W * 32) {
-            const int col = i >> 4, f = i & 15, n = strip * 16 + f, row = row0 + col;
-            if (n >= p.N || row >= row_end) continue;
-            float v = sum_of<W, MT, NT>(red, 0, col, f);
-            if (MT == 2)
-                v = glu_mul(p.act, p.act_param, v, sum_of<W, MT, NT>(red, MT - 1, col, f));
-            else
-                v = plain_act(p.act, p.bias ? v + p.bias[n] : v);
-            if (p.out_bf16)
-                ((__nv_bfloat16*)p.out)[(size_t)row * p.ldo + n] = __float2bfloat16_rn(v);
-            else
-                ((float*)p.out)[(size_t)row * p.ldo + n] = v;
-        }
-        __syncthreads();
-    }
+template <int THREADS>
+__device__ __forceinline__ void team_sync(int id) {
+    asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(THREADS) : "memory");
 }
 
-// ---- a layer of routed experts of few tokens -----------------------------------------------------------------------------------------
-//   out_t = sum_e w_te Wd_e a_te + gate_t Wd_s a_t,  a = silu(Wg h_t) * (Wu h_t),  w_te the sum of t's weights for expert e
-// in two launches.  The eight columns of a product are the step's tokens whatever the expert, so that nothing is gathered: an expert's
-// block forms all tokens' rows and keeps those of the tokens that picked it, and the second product takes zeros for the others.  Both
-// kernels find the list of picked experts (in order of their numbers) from the picks themselves.  The second takes one strip of the output through
-// ALL picked experts and the shared one, w_te on the sums of each block: nothing is left to combine.
-constexpr int EXPERTS_MAX = 1024, FEW = 8, PAIRS_MAX = 512;
+// the same, and whether every warp says so
+template <int THREADS>
+__device__ __forceinline__ bool team_sync_and(int id, bool mine) {
+    int all;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.s32 q, %1, 0;\n\tbar.red.and.pred p, %2, %3, q;\n\tselp.s32 %0, 1, 0, p;\n\t}" : "=r"(all) : "r"((int)mine), "r"(id), "n"(THREADS) : "memory");
+    return all != 0;
+}
 
-struct LayerArgs {
-    const __nv_bfloat16* x;        // [T, H], pitch ldx
-    int ldx, vec, T, H, E, top_k;
-    const int* idx;                // [T, top_k]; -1: none
-    const float* wk;               // [T, top_k]
-    const float* gate;             // [T] or null (1)
-    Weight gu, down, sgu, sdown;   // sgu.codes null: no shared expert
-    __nv_bfloat16* act;            // [slots][8][pitch]
-    __nv_bfloat16* sact;           // [8][spitch]
-    int pitch, spitch;             // whole strips
-    void* out;
-    int out_bf16, ldo;
-    int* status;
-};
-
-// The picked experts' bits, and the number of those below each word.  By all threads; ends with a barrier.
+// ---- the picked experts of a step of few tokens -------------------------------------------------------------------------------------------
+constexpr int EXPERTS_MAX = 1024, FEW = 8, PAIRS_MAX = 128;
 struct Picked {
     uint32_t bits[EXPERTS_MAX / 32];
-    int before[EXPERTS_MAX / 32 + 1];
-    int idx[PAIRS_MAX];
+    int before[EXPERTS_MAX / 32 + 1];      // picked experts below each word
+    short pick[PAIRS_MAX];                 // the expert of a pair, -1 for none
+    short expert[PAIRS_MAX];               // of a slot: the picked experts in order of their numbers
+    uint32_t takes[PAIRS_MAX];             // of a slot: the tokens that picked it
+    __device__ __forceinline__ int slot_of(int e) const { return before[e >> 5] + __popc(bits[e >> 5] & ((1u << (e & 31)) - 1)); }
 };
-__device__ __forceinline__ void find_picked(const LayerArgs& p, Picked& s, bool tell) {
-    const int pairs = p.T * p.top_k;
+// By all threads of the block; ends with a barrier.
+__device__ __forceinline__ void find_picked(const int* idx, int T, int top_k, int E, int* status, Picked& s) {
+    const int pairs = T * top_k;
     for (int i = threadIdx.x; i < EXPERTS_MAX / 32; i += blockDim.x) s.bits[i] = 0;
+    for (int i = threadIdx.x; i < pairs; i += blockDim.x) s.takes[i] = 0;
     __syncthreads();
     for (int i = threadIdx.x; i < pairs; i += blockDim.x) {
-        int e = p.idx[i];
-        if (e < 0 || e >= p.E) {
-            if (e != -1 && tell && p.status) atomicOr(p.status, ST_BAD_EXPERT);
+        int e = idx[i];
+        if (e < 0 || e >= E) {
+            if (e != -1 && status) atomicOr(status, ST_BAD_EXPERT);
             e = -1;
         } else
             atomicOr(&s.bits[e >> 5], 1u << (e & 31));
-        s.idx[i] = e;
+        s.pick[i] = (short)e;
     }
     __syncthreads();
     if (threadIdx.x < 32) {
@@ -231,162 +133,604 @@ __device__ __forceinline__ void find_picked(const LayerArgs& p, Picked& s, bool 
         if (threadIdx.x == 31) s.before[32] = upto;
     }
     __syncthreads();
-}
-// the slot-th picked expert
-__device__ __forceinline__ int expert_of(const Picked& s, int slot) {
-    int w = 0;
-    while (s.before[w + 1] <= slot) w++;
-    return w * 32 + (int)__fns(s.bits[w], 0, slot - s.before[w] + 1);
-}
-
-template <int W, int GROUP>
-__global__ void __launch_bounds__(W * 32)
-experts_up_kernel(const __grid_constant__ LayerArgs p) {
-    __shared__ float red[W * 2 * 8 * 17];
-    __shared__ Picked picked;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
-    const int shared_strips = p.sgu.codes ? p.sgu.strips / 2 : 0;
-    const bool shared = (int)blockIdx.x < shared_strips;
-    Weight w;
-    int strip, slot = 0;
-    size_t first = 0;
-    if (shared) {
-        w = p.sgu, strip = blockIdx.x;
-    } else {
-        pdl_sync();
-        find_picked(p, picked, (int)blockIdx.x == shared_strips);
-        const int u = blockIdx.x - shared_strips;
-        w = p.gu, slot = u / (w.strips / 2), strip = u - slot * (w.strips / 2);
-        if (slot >= picked.before[32]) return;
-        first = (size_t)expert_of(picked, slot) * w.strips;
+    for (int i = threadIdx.x; i < pairs; i += blockDim.x) {
+        const int e = s.pick[i];
+        if (e < 0) continue;
+        const int slot = s.slot_of(e);
+        s.expert[slot] = (short)e;
+        atomicOr(&s.takes[slot], 1u << (i / top_k));
     }
-    const int blocks = w.blocks;
-    const uint4* codes[2];
-    const uint32_t* scales[2];
-#pragma unroll
-    for (int m = 0; m < 2; m++) {
-        const size_t s = first + strip + m * (w.strips / 2);
-        codes[m] = w.codes + s * blocks * 32 + lane;
-        scales[m] = w.scales + s * w.qgroups * 8;
-    }
-    uint4 code[DEPTH][2];
-    q4::Scales<GROUP> sc[DEPTH][2];
-    float acc[2][1][4] = {};
-    auto load = [&](int d, int b) {
-#pragma unroll
-        for (int m = 0; m < 2; m++) {
-            code[d][m] = q4::ld_codes(codes[m] + (size_t)b * 32);
-            sc[d][m].load(scales[m], b, w.qgroups, r);
-        }
-    };
-#pragma unroll
-    for (int d = 0; d < DEPTH; d++)
-        if (warp + d * W < blocks) load(d, warp + d * W);
-    if (shared) pdl_sync();
-    const __nv_bfloat16* xr = r < p.T ? p.x + (size_t)r * p.ldx : nullptr;
-    for (int b0 = warp; b0 < blocks; b0 += DEPTH * W) {
-#pragma unroll
-        for (int d = 0; d < DEPTH; d++) {
-            const int b = b0 + d * W;
-            if (b >= blocks) break;
-            uint2 x[1][4];
-            load_rows(xr, b * 64, w.K, p.vec, t, x[0]);
-            block_product<2, 1, GROUP>(code[d], sc[d], x, acc);
-            if (b + DEPTH * W < blocks) load(d, b + DEPTH * W);
-        }
-    }
-    leave_sums<2, 1>(red, warp, lane, acc);
     __syncthreads();
-    for (int i = threadIdx.x; i < 8 * 16; i += W * 32) {
-        const int col = i >> 4, f = i & 15;
-        if (col >= p.T) continue;
-        const float v = glu_mul(ACT_SILU, 0.f, sum_of<W, 2, 1>(red, 0, col, f), sum_of<W, 2, 1>(red, 1, col, f));
-        // (rounded once, as what every product over weights of these reads)
-        __nv_bfloat16* a = shared ? p.sact + (size_t)col * p.spitch : p.act + ((size_t)slot * FEW + col) * p.pitch;
-        a[strip * 16 + f] = __float2bfloat16_rn(v);
+}
+
+struct Args {
+    Weight w, shared;              // shared: EXPERTS, codes null where there is none
+    const __nv_bfloat16* x;        // [M, K], pitch ldx; vec: rows of whole 8-byte units
+    int ldx, vec, M;
+    void* out;
+    int out_bf16, ldo, N;          // N: output features (of a pair: of one half)
+    const float* bias;
+    const int* offsets;
+    int G;
+    int act;
+    float act_param;
+    const int* idx;                // EXPERTS: the picks, [M, top_k]
+    int top_k, E;
+    uint8_t *frag, *sfrag;         // EXPERTS: [slot][frag_blocks] of 2 KB, see experts_down_kernel; the shared expert's
+    int frag_blocks;
+    q4::Bits bits;
+    q4::Waits waits;
+};
+
+__device__ __forceinline__ void put(const Args& p, int row, int n, float y) {
+    const size_t o = (size_t)row * p.ldo + n;
+    if (p.out_bf16)
+        ((__nv_bfloat16*)p.out)[o] = __float2bfloat16_rn(y);
+    else
+        ((float*)p.out)[o] = y;
+}
+
+// ---- few strips -----------------------------------------------------------------------------------------------------------------------------
+// Grid: strips of the output (of a pair: of one half).  Warp w takes blocks w, w + 8, ... of 64 k, DEPTH of them in flight; the codes are asked for
+// before the wait on the predecessor, the rows behind it.
+template <int MT, int NT, int GROUP>
+__global__ void __launch_bounds__(256, NT == 1 ? 2 : 1)
+gemm_q4_direct_kernel(const __grid_constant__ Args p) {
+    constexpr int W = 8, DEPTH = NT == 1 ? 4 : 2, NS = q4::Scales<GROUP>::N;
+    __shared__ float red[W * MT * 8 * 17];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3, strip = blockIdx.x, blocks = p.w.blocks;
+    const uint4* codes[MT];
+    const uint32_t* scales[MT];
+#pragma unroll
+    for (int m = 0; m < MT; m++) {
+        const size_t s = strip + m * (p.w.strips / 2);
+        codes[m] = p.w.codes + s * blocks * 32 + lane;
+        scales[m] = p.w.scales + s * p.w.qgroups * 8;
+    }
+    bool waited = false;
+    for (int row0 = 0; row0 < p.M; row0 += 8 * NT) {
+        uint4 code[DEPTH][MT];
+        uint32_t sc[DEPTH][MT][NS];
+        uint2 x[DEPTH][NT][4];
+        const __nv_bfloat16* xr[NT];
+#pragma unroll
+        for (int n = 0; n < NT; n++) xr[n] = row0 + 8 * n + r < p.M ? p.x + (size_t)(row0 + 8 * n + r) * p.ldx : nullptr;
+        auto ask = [&](int d, int b) {
+#pragma unroll
+            for (int m = 0; m < MT; m++) {
+                asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                             : "=r"(code[d][m].x), "=r"(code[d][m].y), "=r"(code[d][m].z), "=r"(code[d][m].w)
+                             : "l"(codes[m] + (size_t)b * 32));
+                q4::Scales<GROUP> s;
+                s.load(scales[m], b, p.w.qgroups, r);
+#pragma unroll
+                for (int i = 0; i < NS; i++) sc[d][m][i] = s.s[i];
+            }
+        };
+        auto ask_rows = [&](int d, int b) {
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) x[d][n][j] = row4(xr[n], b * 64 + 16 * j + 4 * t, p.w.K, p.vec);
+        };
+        float acc[MT][NT][4];
+#pragma unroll
+        for (int m = 0; m < MT; m++)
+#pragma unroll
+            for (int n = 0; n < NT; n++) acc[m][n][0] = acc[m][n][1] = acc[m][n][2] = acc[m][n][3] = 0.f;
+#pragma unroll
+        for (int d = 0; d < DEPTH; d++)
+            if (warp + d * W < blocks) ask(d, warp + d * W);
+        if (!waited) pdl_sync();
+        waited = true;
+#pragma unroll
+        for (int d = 0; d < DEPTH; d++)
+            if (warp + d * W < blocks) ask_rows(d, warp + d * W);
+        for (int b0 = warp; b0 < blocks; b0 += DEPTH * W) {
+#pragma unroll
+            for (int d = 0; d < DEPTH; d++) {
+                const int b = b0 + d * W;
+                if (b >= blocks) break;
+                block_product<MT, NT, GROUP>(code[d], sc[d], x[d], p.bits, acc);
+                if (b + DEPTH * W < blocks) ask(d, b + DEPTH * W), ask_rows(d, b + DEPTH * W);
+            }
+        }
+#pragma unroll
+        for (int n8 = 0; n8 < NT; n8++) {
+#pragma unroll
+            for (int m = 0; m < MT; m++) leave_sums<MT>(red, warp, lane, m, acc[m][n8]);
+            __syncthreads();
+            const int i = threadIdx.x, col = i >> 4, f = i & 15, n = strip * 16 + f, row = row0 + 8 * n8 + col;
+            if (i < 128 && n < p.N && row < p.M) {
+                float y = sum_of<W, MT>(red, 0, col, f);
+                y = MT == 2 ? glu_mul(p.act, p.act_param, y, sum_of<W, MT>(red, MT - 1, col, f)) : plain_act(p.act, p.bias ? y + p.bias[n] : y);
+                put(p, row, n, y);
+            }
+            __syncthreads();
+        }
     }
 }
 
-template <int W, int GROUP>
-__global__ void __launch_bounds__(W * 32)
-experts_down_kernel(const __grid_constant__ LayerArgs p) {
-    __shared__ float red[W * 8 * 17];
+// ---- many strips ----------------------------------------------------------------------------------------------------------------------------
+// DENSE   one weight, up to 8 NT rows
+// GROUPED rows [offsets[g], offsets[g + 1]) meet weight g, eight at a time
+// EXPERTS the gate and up rows of a layer of routed experts: the eight rows of a unit are the step's tokens whatever the expert, so
+//         that nothing is gathered; the shared expert's strips come first.  What comes out lies as the B fragments of the next
+//         product, as two bfloat16 terms (rounded to one, the layer's output would be as far off again as its own rounding).
+//
+// A unit is two strips (a pair's gate and up strip, or neighbours) and up to 8 NT rows.  A block takes a run of neighbouring units; its four teams of
+// four warps take them in turn, and the warps of a team every fourth block of 64 k.  One more warp a team has its codes copied (cp.async.bulk) into
+// stages of KC blocks, across the borders of units.  The fragments of the rows lie in shared memory for all teams; where the
+// rows change (GROUPED), all teams meet.
+enum { DENSE = 0, GROUPED = 1, EXPERTS = 2 };
+constexpr int GROUPS_MAX = 1024, TEAM_W = 4, TEAMS = 4, KC = 8, STREAM_THREADS = TEAMS * (TEAM_W + 1) * 32, STAGES_MAX = 8;
+
+template <int NT, int GROUP>
+struct Stream {
+    static constexpr int SCALE_BLOCK = GROUP == 32 ? 64 : GROUP == 64 ? 32 : 16;      // bytes a block of 64 k (128: a pair of blocks has 32)
+    static constexpr int CODES = KC * 512, SCALES = KC * SCALE_BLOCK, STAGE = 2 * (CODES + SCALES);
+    static constexpr int RED_BUFFERS = NT == 1 ? 2 : 1, RED_FLOATS = TEAM_W * 2 * 8 * 17;      // of a team
+    static constexpr int RED = TEAMS * RED_BUFFERS * RED_FLOATS * 4;
+    static int bytes(int blocks, int stages) { return TEAMS * stages * STAGE + RED + blocks * NT * 1024; }
+};
+
+struct Unit {
+    int strip, g, slot;            // first strip (of the half); group; EXPERTS: slot, -1: the shared expert
+};
+
+template <int MODE, int NT, int GROUP, bool PAIR>
+__global__ void __launch_bounds__(STREAM_THREADS, 1)
+gemm_q4_stream_kernel(const __grid_constant__ Args p, const int stages) {
+    using S = Stream<NT, GROUP>;
+    constexpr int UM = PAIR ? 1 : 2;                      // strips of the output a unit
+    extern __shared__ __align__(128) uint8_t smem[];     // the teams' stages, the teams' sums, the rows' fragments [blocks][NT][2][32] x 16 bytes
+    __shared__ int s_first[MODE == GROUPED ? GROUPS_MAX + 1 : 1], s_off[MODE == GROUPED ? GROUPS_MAX + 1 : 1];
     __shared__ Picked picked;
-    __shared__ __align__(16) float wt[PAIRS_MAX + 1][FEW];   // a slot's weight of each token; the last one's: the shared expert's gate
-    __shared__ uint32_t takes[PAIRS_MAX + 1];         // the tokens that picked it
-    __shared__ short expert[PAIRS_MAX];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3, strip = blockIdx.x;
+    __shared__ __align__(8) unsigned long long s_bars[TEAMS][2][STAGES_MAX];
+    __shared__ volatile int s_abort;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int blocks = p.w.blocks, half = PAIR ? p.w.strips / 2 : p.w.strips, per = (half + UM - 1) / UM;      // units of a weight and row chunk
+    if (threadIdx.x < TEAMS * stages) {
+        const int q = threadIdx.x / stages, s = threadIdx.x % stages;
+        q4::mbar_init(smem_u32(&s_bars[q][0][s]), 1), q4::mbar_init(smem_u32(&s_bars[q][1][s]), TEAM_W);
+    }
+    if (threadIdx.x == 0) {
+        s_abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    int units, shared_units = 0;
+    if (MODE == DENSE)
+        units = per;
+    else {
+        pdl_sync();
+        if (MODE == EXPERTS) {
+            find_picked(p.idx, p.M, p.top_k, p.E, blockIdx.x == 0 ? p.waits.status : nullptr, picked);
+            shared_units = p.shared.codes ? p.shared.strips / 2 : 0;
+            units = shared_units + picked.before[32] * per;
+        } else {
+            for (int i = threadIdx.x; i <= p.G; i += STREAM_THREADS) s_off[i] = min(p.M, max(0, p.offsets[i]));
+            __syncthreads();
+            if (warp == 0) {                             // row chunks of the groups before each
+                int run = 0;
+                for (int g0 = 0; g0 < p.G; g0 += 32) {
+                    const int g = g0 + lane, n = g < p.G ? max(0, s_off[g + 1] - s_off[g] + 8 * NT - 1) / (8 * NT) : 0;
+                    int upto = n;
+#pragma unroll
+                    for (int o = 1; o < 32; o <<= 1) {
+                        const int v = __shfl_up_sync(0xffffffffu, upto, o);
+                        if (lane >= o) upto += v;
+                    }
+                    if (g < p.G) s_first[g] = run + upto - n;
+                    run += __shfl_sync(0xffffffffu, upto, 31);
+                }
+                if (lane == 0) s_first[p.G] = run;
+            }
+            __syncthreads();
+            units = s_first[p.G] * per;
+        }
+    }
+    __syncthreads();
+    const int u0 = (int)((long long)units * blockIdx.x / gridDim.x), u1 = (int)((long long)units * (blockIdx.x + 1) / gridDim.x);      // this block's units
+    auto locate = [&](int u) {
+        Unit v;
+        v.g = 0, v.slot = 0;
+        if (MODE == EXPERTS) {
+            if (u < shared_units)
+                v.slot = -1, v.strip = u;
+            else
+                u -= shared_units, v.slot = u / per, v.strip = u - v.slot * per, v.g = picked.expert[v.slot];
+        } else {
+            const int c = u / per;
+            v.strip = (u - c * per) * UM;
+            if (MODE == GROUPED) {
+                int lo = 0, hi = p.G;
+                while (hi - lo > 1) {
+                    const int mid = (lo + hi) >> 1;
+                    if (s_first[mid] <= c) lo = mid; else hi = mid;
+                }
+                v.g = lo;
+            }
+        }
+        return v;
+    };
+    // the unit TEAMS further on, u
+    auto step = [&](Unit& v, int u) {
+        v.strip += TEAMS * UM;
+        if (v.strip >= (MODE == EXPERTS && v.slot < 0 ? shared_units : half)) v = locate(u);
+    };
+    // A run: units of the same rows.  GROUPED: a chunk's; else all.
+    auto run_end = [&](int u) { return MODE == GROUPED ? min(u1, (u / per + 1) * per) : u1; };
+    const int unit_stages = (blocks + KC - 1) / KC;
+
+    if (warp >= TEAMS * TEAM_W) {
+        // ---- copies of team q ---------------------------------------------------------------------------------------------------------------
+        if (lane || u0 >= u1 || p.waits.test_fault == 1) return;
+        const int q = warp - TEAMS * TEAM_W;
+        int u = u0 + q, end = run_end(u0), s = 0, it = 0;
+        uint32_t parity = 1;
+        const uint32_t base = smem_u32(smem) + q * stages * S::STAGE, bars = smem_u32(&s_bars[q][0][0]);
+        bool ok = true;
+        while (ok) {
+            while (u >= end && end < u1) u = end + q, end = run_end(end);      // past its run: the team's first unit of the next one
+            if (u >= end) break;
+            for (Unit v = locate(u); ok && u < end;) {
+                const Weight& w = MODE == EXPERTS && v.slot < 0 ? p.shared : p.w;
+                const size_t s0 = (size_t)v.g * w.strips + v.strip, s1 = PAIR ? s0 + w.strips / 2 : v.strip + 1 < half ? s0 + 1 : s0;
+                const uint8_t *c0 = (const uint8_t*)(w.codes + s0 * blocks * 32), *c1 = (const uint8_t*)(w.codes + s1 * blocks * 32);
+                const uint8_t *q0 = (const uint8_t*)(w.scales + s0 * w.qgroups * 8), *q1 = (const uint8_t*)(w.scales + s1 * w.qgroups * 8);
+                int groups = w.qgroups;                  // left
+                for (int kb = 0; kb < blocks; kb += KC) {
+                    if (it >= stages && !(ok = q4::mbar_wait(bars + 8 * (STAGES_MAX + s), parity, &s_abort, p.waits.limit_us, p.waits.status, 0x61))) break;
+                    const int n = min(KC, blocks - kb) * 512, qn = min(groups, S::SCALES / 32) * 32;
+                    const uint32_t to = base + s * S::STAGE, full = bars + 8 * s;
+                    q4::mbar_expect_tx(full, 2 * (n + qn));
+                    q4::bulk_copy(to, c0, n, full);
+                    q4::bulk_copy(to + S::CODES, c1, n, full);
+                    q4::bulk_copy(to + 2 * S::CODES, q0, qn, full);
+                    q4::bulk_copy(to + 2 * S::CODES + S::SCALES, q1, qn, full);
+                    c0 += S::CODES, c1 += S::CODES, q0 += S::SCALES, q1 += S::SCALES, groups -= S::SCALES / 32;
+                    it++;
+                    if (++s == stages) s = 0, parity ^= 1;
+                }
+                u += TEAMS;
+                if (u < end) step(v, u);
+            }
+        }
+        if (!ok) {
+            s_abort = 1;
+            for (int i = max(0, it - stages); i < it; i++)      // copies in flight must land
+                q4::mbar_wait(bars + 8 * (i % stages), (i / stages) & 1, nullptr, p.waits.limit_us, p.waits.status, 0x62);
+        }
+        return;
+    }
+
+    // ---- products ---------------------------------------------------------------------------------------------------------------------------
+    const int team = warp / TEAM_W, tw = warp % TEAM_W, r = lane >> 2;
+    const uint32_t base = smem_u32(smem) + team * stages * S::STAGE, xs = smem_u32(smem) + TEAMS * stages * S::STAGE + S::RED;
+    float* red = reinterpret_cast<float*>(smem + TEAMS * stages * S::STAGE) + team * S::RED_BUFFERS * S::RED_FLOATS;
+    if (MODE == DENSE) pdl_sync();
+    int s = 0, turn = 0;
+    uint32_t parity = 0;
+    bool ok = true;
+    for (int first = u0; first < u1; first = run_end(first)) {
+        int row0 = 0, rows = p.M;
+        if (MODE == GROUPED) {
+            const int c = first / per;
+            const Unit v = locate(first);
+            row0 = s_off[v.g] + (c - s_first[v.g]) * 8 * NT, rows = min(8 * NT, s_off[v.g + 1] - row0);
+            if (first > u0) team_sync<TEAMS * TEAM_W * 32>(TEAMS + 1);      // the rows before are done with
+        }
+        const int b16 = blocks * 16;
+        for (int i = threadIdx.x; i < b16 * 8 * NT; i += TEAMS * TEAM_W * 32) {
+            const int c = i / b16, k4 = i - c * b16;     // row, four k
+            const __nv_bfloat16* row = c < rows ? p.x + (size_t)(row0 + c) * p.ldx : nullptr;
+            const int b = k4 >> 4, j = (k4 >> 2) & 3, tt = k4 & 3;
+            sts8(xs + ((b * NT + (c >> 3)) * 2 + (j >> 1)) * 512 + ((c & 7) * 4 + tt) * 16 + (j & 1) * 8, row4(row, k4 * 4, p.w.K, p.vec));
+        }
+        team_sync<TEAMS * TEAM_W * 32>(TEAMS + 1);
+        const int end = run_end(first);
+        Unit v;
+        if (first + team < end) v = locate(first + team);
+        for (int u = first + team; u < end && ok; u += TEAMS) {
+            if (u > first + team) step(v, u);
+            float acc[2][NT][4];
+#pragma unroll
+            for (int m = 0; m < 2; m++)
+#pragma unroll
+                for (int n = 0; n < NT; n++) acc[m][n][0] = acc[m][n][1] = acc[m][n][2] = acc[m][n][3] = 0.f;
+            uint32_t xa = xs + tw * NT * 1024 + lane * 16;
+            int left = blocks - tw;                      // blocks from this warp's first on
+            for (int st = 0; st < unit_stages; st++) {
+                ok = q4::mbar_wait(smem_u32(&s_bars[team][0][s]), parity, &s_abort, p.waits.limit_us, p.waits.status, 0x64);
+                if (!ok) break;
+                const uint32_t at = base + s * S::STAGE + tw * 512 + lane * 16, as = base + s * S::STAGE + 2 * S::CODES + r * 4;
+#pragma unroll
+                for (int i = 0; i < KC / TEAM_W; i++) {
+                    if (left > i * TEAM_W) {
+                        uint4 code[2];
+                        uint32_t sc[2][q4::Scales<GROUP>::N];
+                        uint2 x[NT][4];
+#pragma unroll
+                        for (int m = 0; m < 2; m++) {
+                            code[m] = lds16(at + m * S::CODES + i * TEAM_W * 512);
+                            const uint32_t a = as + m * S::SCALES + (GROUP == 128 ? (tw + i * TEAM_W) / 2 * 32 : (tw + i * TEAM_W) * S::SCALE_BLOCK);
+                            sc[m][0] = lds4(a);
+                            // (a second group that begins beyond K was not copied; its q are 0)
+                            if (GROUP == 32) sc[m][q4::Scales<GROUP>::N - 1] = (st * KC + i * TEAM_W + tw) * 64 + 32 < p.w.K ? lds4(a + 32) : 0u;
+                        }
+#pragma unroll
+                        for (int n = 0; n < NT; n++)
+#pragma unroll
+                            for (int h = 0; h < 2; h++) {
+                                const uint4 y = lds16(xa + i * TEAM_W * NT * 1024 + (n * 2 + h) * 512);
+                                x[n][2 * h] = make_uint2(y.x, y.y), x[n][2 * h + 1] = make_uint2(y.z, y.w);
+                            }
+                        block_product<2, NT, GROUP>(code, sc, x, p.bits, acc);
+                    }
+                }
+                left -= KC, xa += KC * NT * 1024;
+                __syncwarp();
+                if (lane == 0) q4::mbar_arrive(smem_u32(&s_bars[team][1][s]));
+                if (++s == stages) s = 0, parity ^= 1;
+            }
+#pragma unroll
+            for (int n8 = 0; n8 < NT; n8++) {
+                float* sums = red + (S::RED_BUFFERS == 2 ? turn : 0) * S::RED_FLOATS;
+                turn ^= 1;
+#pragma unroll
+                for (int m = 0; m < 2; m++) leave_sums<2>(sums, tw, lane, m, acc[m][n8]);
+                // (two buffers: this one is written again only behind the next one's barrier.  A team gives up as a whole.)
+                if (n8 == 0)
+                    ok = team_sync_and<TEAM_W * 32>(team + 1, ok);
+                else
+                    team_sync<TEAM_W * 32>(team + 1);
+                if (!ok) s_abort = 1;
+#pragma unroll
+                for (int m = 0; m < UM; m++) {
+                    const int i = tw * 32 + lane, col = i >> 4, f = i & 15, n = (v.strip + m) * 16 + f;
+                    if (MODE == EXPERTS) {
+                        const bool takes = col < p.M && (v.slot < 0 || ((picked.takes[v.slot] >> col) & 1));
+                        float a = 0.f;
+                        if (takes) a = glu_mul(ACT_SILU, 0.f, sum_of<TEAM_W, 2>(sums, 0, col, f), sum_of<TEAM_W, 2>(sums, 1, col, f));
+                        const __nv_bfloat16 h = __float2bfloat16_rn(a), l = __float2bfloat16_rn(a - __bfloat162float(h));
+                        uint8_t* to = (v.slot < 0 ? p.sfrag : p.frag + (size_t)v.slot * p.frag_blocks * 2048) + (size_t)v.strip * 512;
+                        __nv_bfloat16* e = reinterpret_cast<__nv_bfloat16*>(to + (col * 4 + (f >> 2)) * 16) + (f & 3);
+                        e[0] = h, e[4] = l;
+                        // the strips that fill the last block of 64
+                        if (v.strip == (v.slot < 0 ? shared_units : half) - 1)
+                            for (int z = v.strip + 1; z & 3; z++) *reinterpret_cast<uint32_t*>(to + (size_t)(z - v.strip) * 512 + i * 4) = 0u;
+                        continue;
+                    }
+                    if (n >= p.N || n8 * 8 + col >= rows) continue;
+                    float y = sum_of<TEAM_W, 2>(sums, m, col, f);
+                    y = PAIR ? glu_mul(p.act, p.act_param, y, sum_of<TEAM_W, 2>(sums, 1, col, f)) : plain_act(p.act, p.bias ? y + p.bias[n] : y);
+                    put(p, row0 + n8 * 8 + col, n, y);
+                }
+                if (S::RED_BUFFERS == 1) team_sync<TEAM_W * 32>(team + 1);
+            }
+        }
+    }
+}
+
+// ---- the down products of a layer of routed experts ---------------------------------------------------------------------------------------
+//   out_t = sum_e w_te Wd_e a_te + gate_t Wd_s a_t,  w_te the sum of t's weights for expert e
+// Four strips of the output go through ALL picked experts and the shared one, w_te on the sums of each block of 64 k: nothing is left to
+// combine.  Tokens that did not pick an expert meet it with the zeros that the first kernel left.  A block of 64 k of the rows is 2 KB: for each 16 k a
+// B fragment of 32 lanes x (four k rounded to bfloat16, what that left rounded likewise).  Grid: (fours of strips, 1, S); the S blocks of a unit are
+// a cluster and share its blocks of 64 k, sixteen a stage and one a warp; the first block adds their sums up in order.
+constexpr int DOWN_W = 16, DOWN_MT = 4, DOWN_STAGES = 3, DOWN_THREADS = DOWN_W * 32 + 32;
+struct DownArgs {
+    Weight down, shared;           // shared.codes null: none
+    const uint8_t *frag, *sfrag;
+    int T, H, E, top_k, S;
+    const int* idx;
+    const float* wk;
+    const float* gate;
+    void* out;
+    int out_bf16, ldo;
+    q4::Bits bits;
+    q4::Waits waits;
+};
+template <int GROUP>
+struct DownStage {
+    static constexpr int SCALE_BLOCK = GROUP == 32 ? 64 : 32;      // (128: each block has its own copy)
+    static constexpr int CODES = DOWN_W * 512, SCALES = DOWN_W * SCALE_BLOCK, X = DOWN_W * 2048;
+    static constexpr int STAGE = DOWN_MT * (CODES + SCALES) + X, BYTES = DOWN_STAGES * STAGE;
+    static constexpr int RED_FLOATS = DOWN_W * DOWN_MT * 8 * 17;   // lies over the stages, and the other blocks' sums behind it
+    static_assert(RED_FLOATS * 4 + 8 * DOWN_MT * 128 * 4 <= BYTES, "sums");
+};
+
+template <int GROUP>
+__global__ void __launch_bounds__(DOWN_THREADS, 1)
+experts_down_kernel(const __grid_constant__ DownArgs p) {
+    using D = DownStage<GROUP>;
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ Picked picked;
+    __shared__ float wk[PAIRS_MAX];
+    __shared__ __align__(16) float wt[PAIRS_MAX + 1][FEW];      // a slot's weight of each token; the last one's: the shared expert's gate
+    __shared__ __align__(8) unsigned long long s_bars[2][DOWN_STAGES];
+    __shared__ volatile int s_abort;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3, strip0 = blockIdx.x * DOWN_MT, rank = blockIdx.z;
+    if (threadIdx.x == 0) {
+        s_abort = 0;
+        for (int s = 0; s < DOWN_STAGES; s++) q4::mbar_init(smem_u32(&s_bars[0][s]), 1), q4::mbar_init(smem_u32(&s_bars[1][s]), DOWN_W);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
     // The picks were written at least two kernels ago (this one's predecessor let it in behind its own wait): they, and the weights, are
     // read before the wait.
-    find_picked(p, picked, false);
+    find_picked(p.idx, p.T, p.top_k, p.E, nullptr, picked);
     const int slots = picked.before[32];
-    for (int i = threadIdx.x; i < slots; i += W * 32) {
-        const int e = expert_of(picked, i);
-        expert[i] = (short)e;
-        uint32_t m = 0;
-        for (int c = 0; c < p.T; c++) {
-            float v = 0.f;
-            for (int j = 0; j < p.top_k; j++)
-                if (picked.idx[c * p.top_k + j] == e) v += p.wk[c * p.top_k + j], m |= 1u << c;
-            wt[i][c] = v;
-        }
-        for (int c = p.T; c < FEW; c++) wt[i][c] = 0.f;
-        takes[i] = m;
-    }
-    if (threadIdx.x < FEW) wt[slots][threadIdx.x] = (int)threadIdx.x < p.T && p.sdown.codes ? (p.gate ? p.gate[threadIdx.x] : 1.f) : 0.f;
-    if (threadIdx.x == FEW) takes[slots] = (1u << p.T) - 1;
+    for (int i = threadIdx.x; i < slots * FEW; i += DOWN_THREADS) wt[i >> 3][i & 7] = 0.f;
+    const int pairs = p.T * p.top_k;
+    if (threadIdx.x < pairs) wk[threadIdx.x] = p.wk[threadIdx.x];
     __syncthreads();
-    const int nb = p.down.blocks, total = slots * nb + (p.sdown.codes ? p.sdown.blocks : 0);
-    auto where = [&](int i, int* slot, int* b) {
-        *slot = min(i / nb, slots), *b = i - *slot * nb;
-    };
-    uint4 code[DEPTH][1];
-    q4::Scales<GROUP> sc[DEPTH][1];
-    auto load = [&](int d, int i) {
-        int slot, b;
-        where(i, &slot, &b);
-        const Weight& w = slot < slots ? p.down : p.sdown;
-        const size_t s = (size_t)(slot < slots ? expert[slot] : 0) * w.strips + strip;
-        code[d][0] = q4::ld_codes(w.codes + (s * w.blocks + b) * 32 + lane);
-        sc[d][0].load(w.scales + s * w.qgroups * 8, b, w.qgroups, r);
-    };
-#pragma unroll
-    for (int d = 0; d < DEPTH; d++)
-        if (warp + d * W < total) load(d, warp + d * W);
-    pdl_sync();
-    float acc[1][1][4] = {};
-    for (int i0 = warp; i0 < total; i0 += DEPTH * W) {
-#pragma unroll
-        for (int d = 0; d < DEPTH; d++) {
-            const int i = i0 + d * W;
-            if (i >= total) break;
+    if (threadIdx.x < pairs && picked.pick[threadIdx.x] >= 0) {
+        const int e = picked.pick[threadIdx.x], c = threadIdx.x / p.top_k;
+        float v = 0.f;
+        bool first = true;                                      // an expert may be picked twice: the first of the picks adds them up
+        for (int j = c * p.top_k; j < (c + 1) * p.top_k; j++)
+            if (picked.pick[j] == e) first = first && j >= (int)threadIdx.x, v += wk[j];
+        if (first) wt[picked.slot_of(e)][c] = v;
+    }
+    if (threadIdx.x < FEW) wt[slots][threadIdx.x] = (int)threadIdx.x < p.T && p.shared.codes ? (p.gate ? p.gate[threadIdx.x] : 1.f) : 0.f;
+    __syncthreads();
+    const int nb = p.down.blocks, total = slots * nb + (p.shared.codes ? p.shared.blocks : 0);
+    const int lo = (int)((long long)total * rank / p.S), hi = (int)((long long)total * (rank + 1) / p.S), count = (hi - lo + DOWN_W - 1) / DOWN_W;
+    bool ok = true;
+
+    if (warp == DOWN_W) {
+        // ---- copies.  The pieces of a stage that lie in one expert are neighbours in memory: a lane for each of its strips' codes and scales, one for
+        // the rows' fragments.
+        ok = p.waits.test_fault != 1;
+        int done = 0;
+        struct Place {
             int slot, b;
-            where(i, &slot, &b);
-            uint2 x[1][4];
-            const bool mine = (takes[slot] >> r) & 1;
-            const __nv_bfloat16* row = slot < slots ? p.act + ((size_t)slot * FEW + r) * p.pitch : p.sact + (size_t)r * p.spitch;
-            load_rows(mine ? row : nullptr, b * 64, slot < slots ? p.pitch : p.spitch, 1, t, x[0]);
-            float part[1][1][4] = {};
-            block_product<1, 1, GROUP>(code[d], sc[d], x, part);
-            const float2 w2 = *reinterpret_cast<const float2*>(&wt[slot][2 * t]);
-            acc[0][0][0] = fmaf(w2.x, part[0][0][0], acc[0][0][0]), acc[0][0][1] = fmaf(w2.y, part[0][0][1], acc[0][0][1]);
-            acc[0][0][2] = fmaf(w2.x, part[0][0][2], acc[0][0][2]), acc[0][0][3] = fmaf(w2.y, part[0][0][3], acc[0][0][3]);
-            if (i + DEPTH * W < total) load(d, i + DEPTH * W);
+        };
+        const int strip = min(strip0 + (lane & 3), p.down.strips - 1);
+        // one stage from `at` on; where it ends
+        auto copy_stage = [&](int st, Place at, bool codes, bool rows) {
+            const uint32_t base = smem_u32(smem) + st % DOWN_STAGES * D::STAGE, bar = smem_u32(&s_bars[0][st % DOWN_STAGES]);
+            const int all = min(DOWN_W, hi - lo - st * DOWN_W);
+            for (int i = 0; i < all;) {
+                const bool own = at.slot < slots;
+                const Weight& w = own ? p.down : p.shared;
+                const int n = min(all - i, w.blocks - at.b);
+                if (codes && lane < DOWN_MT) {
+                    const size_t row = (size_t)(own ? picked.expert[at.slot] : 0) * w.strips + strip;
+                    q4::bulk_copy(base + lane * D::CODES + i * 512, w.codes + (row * w.blocks + at.b) * 32, n * 512, bar);
+                    const uint32_t sc = base + DOWN_MT * D::CODES + lane * D::SCALES + i * D::SCALE_BLOCK;
+                    const uint32_t* from = w.scales + row * w.qgroups * 8;
+                    if (GROUP == 128)
+                        for (int j = 0; j < n; j++) q4::bulk_copy(sc + j * 32, from + (size_t)((at.b + j) >> 1) * 8, 32, bar);
+                    else if (GROUP == 64)
+                        q4::bulk_copy(sc, from + (size_t)at.b * 8, n * 32, bar);
+                    else
+                        q4::bulk_copy(sc, from + (size_t)at.b * 16, min(2 * n, w.qgroups - 2 * at.b) * 32, bar);
+                }
+                if (rows && lane == DOWN_MT)
+                    q4::bulk_copy(base + DOWN_MT * (D::CODES + D::SCALES) + i * 2048, (own ? p.frag + (size_t)at.slot * nb * 2048 : p.sfrag) + (size_t)at.b * 2048, n * 2048, bar);
+                i += n, at.b += n;
+                if (own && at.b == nb) at.b = 0, at.slot++;
+            }
+            return at;
+        };
+        auto expect = [&](int st, Place at) {
+            const int all = min(DOWN_W, hi - lo - st * DOWN_W);
+            int bytes = all * (DOWN_MT * (512 + (GROUP == 32 ? 64 : 32)) + 2048);
+            if (GROUP == 32)                             // (a last block of no more than 32 k has one group)
+                for (int i = 0; i < all; i++) {
+                    if (2 * at.b + 1 >= (at.slot < slots ? p.down.qgroups : p.shared.qgroups)) bytes -= DOWN_MT * 32;
+                    if (++at.b == nb && at.slot < slots) at.b = 0, at.slot++;
+                }
+            if (lane == 0) q4::mbar_expect_tx(smem_u32(&s_bars[0][st % DOWN_STAGES]), bytes);
+            __syncwarp();
+        };
+        Place codes_at, rows_at;
+        codes_at.slot = min(lo / nb, slots), codes_at.b = lo - codes_at.slot * nb;
+        rows_at = codes_at;
+        for (int st = 0; st < min(count, DOWN_STAGES) && ok; st++) {
+            expect(st, codes_at);
+            codes_at = copy_stage(st, codes_at, true, false);
+        }
+        pdl_sync();
+        for (; done < count && ok; done++) {
+            if (done < DOWN_STAGES)
+                rows_at = copy_stage(done, rows_at, false, true);
+            else {
+                ok = q4::mbar_wait(smem_u32(&s_bars[1][done % DOWN_STAGES]), ((done / DOWN_STAGES) & 1) ^ 1, &s_abort, p.waits.limit_us, p.waits.status, 0x71);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                expect(done, codes_at);
+                codes_at = copy_stage(done, codes_at, true, true);
+            }
+            __syncwarp();
+        }
+        if (!ok && p.waits.test_fault != 1) {
+            s_abort = 1;
+            for (int i = max(0, done - DOWN_STAGES); i < done; i++)      // copies in flight must land
+                q4::mbar_wait(smem_u32(&s_bars[0][i % DOWN_STAGES]), (i / DOWN_STAGES) & 1, nullptr, p.waits.limit_us, p.waits.status, 0x72);
         }
     }
-    leave_sums<1, 1>(red, warp, lane, acc);
+    float acc[DOWN_MT][4] = {};
+    if (warp < DOWN_W) {
+        int slot = min((lo + warp) / nb, slots), b = lo + warp - slot * nb;      // this warp's block of the stage
+        for (int st = 0; st < count && ok; st++) {
+            const int s = st % DOWN_STAGES;
+            ok = q4::mbar_wait(smem_u32(&s_bars[0][s]), (st / DOWN_STAGES) & 1, &s_abort, p.waits.limit_us, p.waits.status, 0x74);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            if (lo + st * DOWN_W + warp < hi) {
+                const uint32_t base = smem_u32(smem) + s * D::STAGE, xa = base + DOWN_MT * (D::CODES + D::SCALES) + warp * 2048 + lane * 16;
+                float c[DOWN_MT][4], sum[DOWN_MT][4];
+                uint4 code[DOWN_MT];
+#pragma unroll
+                for (int m = 0; m < DOWN_MT; m++) code[m] = lds16(base + m * D::CODES + warp * 512 + lane * 16);
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const uint4 x = lds16(xa + j * 512);
+                    const bool fresh = GROUP == 32 ? j % 2 == 0 : j == 0, last = GROUP == 32 ? j % 2 == 1 : j == 3;
+#pragma unroll
+                    for (int m = 0; m < DOWN_MT; m++) {
+                        uint32_t a[4];
+                        q4::unpack(q4::word(code[m], j), p.bits, a);
+                        if (fresh)
+                            q4::mma(c[m], a, x.x, x.y, 0.f, 0.f, 0.f, 0.f);
+                        else
+                            q4::mma(c[m], a, x.x, x.y, c[m][0], c[m][1], c[m][2], c[m][3]);
+                        q4::mma(c[m], a, x.z, x.w, c[m][0], c[m][1], c[m][2], c[m][3]);
+                    }
+                    if (last)
+#pragma unroll
+                        for (int m = 0; m < DOWN_MT; m++) {
+                            uint32_t sc = lds4(base + DOWN_MT * D::CODES + m * D::SCALES + warp * D::SCALE_BLOCK + (GROUP == 32 ? j / 2 * 32 : 0) + r * 4);
+                            if (GROUP == 32 && j == 3 && 2 * b + 1 >= (slot < slots ? p.down.qgroups : p.shared.qgroups)) sc = 0u;      // (not copied; its q are 0)
+                            const float l = q4::scale_lo(sc), h = q4::scale_hi(sc);
+                            const bool one = GROUP != 32 || j == 1;
+                            sum[m][0] = one ? l * c[m][0] : fmaf(l, c[m][0], sum[m][0]), sum[m][1] = one ? l * c[m][1] : fmaf(l, c[m][1], sum[m][1]);
+                            sum[m][2] = one ? h * c[m][2] : fmaf(h, c[m][2], sum[m][2]), sum[m][3] = one ? h * c[m][3] : fmaf(h, c[m][3], sum[m][3]);
+                        }
+                }
+                const float2 w2 = *reinterpret_cast<const float2*>(&wt[slot][2 * t]);
+#pragma unroll
+                for (int m = 0; m < DOWN_MT; m++) {
+                    acc[m][0] = fmaf(w2.x, sum[m][0], acc[m][0]), acc[m][1] = fmaf(w2.y, sum[m][1], acc[m][1]);
+                    acc[m][2] = fmaf(w2.x, sum[m][2], acc[m][2]), acc[m][3] = fmaf(w2.y, sum[m][3], acc[m][3]);
+                }
+            }
+            __syncwarp();
+            if (lane == 0) q4::mbar_arrive(smem_u32(&s_bars[1][s]));
+            b += DOWN_W;
+            while (slot < slots && b >= nb) b -= nb, slot++;
+        }
+        if (!ok) s_abort = 1;
+    }
+    __syncthreads();                                            // every stage has been copied and read: the sums lie over them
+    float* red = reinterpret_cast<float*>(smem);
+    if (warp < DOWN_W)
+#pragma unroll
+        for (int m = 0; m < DOWN_MT; m++) leave_sums<DOWN_MT>(red, warp, lane, m, acc[m]);
     __syncthreads();
-    for (int i = threadIdx.x; i < 8 * 16; i += W * 32) {
-        const int col = i >> 4, f = i & 15, n = strip * 16 + f;
-        if (col >= p.T || n >= p.H) continue;
-        const float v = sum_of<W, 1, 1>(red, 0, col, f);
+    const int i = threadIdx.x, m = i >> 7, col = (i >> 4) & 7, f = i & 15, n = (strip0 + m) * 16 + f;
+    const bool live = i < DOWN_MT * 128;
+    float y = live ? sum_of<DOWN_W, DOWN_MT>(red, m, col, f) : 0.f;
+    if (p.S > 1) {
+        const uint32_t part = smem_u32(smem) + D::RED_FLOATS * 4;
+        cluster_sync_all();                                     // (the first block's stages are free)
+        if (rank && live) st_cluster_f32(mapa_cluster(part + (rank * DOWN_MT * 128 + i) * 4, 0), y);
+        cluster_sync_all();
+        if (rank) return;
+        if (live)
+            for (int k = 1; k < p.S; k++) y += reinterpret_cast<const float*>(smem)[D::RED_FLOATS + k * DOWN_MT * 128 + i];
+    }
+    if (live && col < p.T && n < p.H) {
         if (p.out_bf16)
-            ((__nv_bfloat16*)p.out)[(size_t)col * p.ldo + n] = __float2bfloat16_rn(v);
+            ((__nv_bfloat16*)p.out)[(size_t)col * p.ldo + n] = __float2bfloat16_rn(y);
         else
-            ((float*)p.out)[(size_t)col * p.ldo + n] = v;
+            ((float*)p.out)[(size_t)col * p.ldo + n] = y;
     }
 }
 
+// ---- host -----------------------------------------------------------------------------------------------------------------------------------
 Weight weight(const void* codes, const void* scales, int N, int K, int group, int pair) {
     Weight w = {};
     w.codes = (const uint4*)codes, w.scales = (const uint32_t*)scales, w.N = N, w.K = K;
@@ -394,6 +738,66 @@ Weight weight(const void* codes, const void* scales, int N, int K, int group, in
     w.strips = (half + 15) / 16 * (pair ? 2 : 1), w.blocks = (K + 63) / 64, w.qgroups = (K + group - 1) / group;
     return w;
 }
+
+int sm_count() {
+    int dev = 0, n = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
+    return n;
+}
+
+// Stages of a team beside the fragments of the rows: 0 where there is no room for two.
+template <int MODE, int NT, int GROUP>
+int stream_stages(int blocks) {
+    const long long room = 227 * 1024 - 2048 - (MODE == GROUPED ? 8 * (GROUPS_MAX + 1) : 0) - Stream<NT, GROUP>::RED - (long long)blocks * NT * 1024;
+    const long long n = room / (TEAMS * Stream<NT, GROUP>::STAGE);
+    return n < 2 ? 0 : n < 5 ? (int)n : 5;
+}
+
+// max_units: the units of the launch, or more (blocks without one leave at once)
+template <int MODE, int NT, int GROUP, bool PAIR>
+int launch_stream(const Args& p, long long max_units, cudaStream_t stream) {
+    const int stages = stream_stages<MODE, NT, GROUP>(p.w.blocks), bytes = Stream<NT, GROUP>::bytes(p.w.blocks, stages);
+    auto kernel = gemm_q4_stream_kernel<MODE, NT, GROUP, PAIR>;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) return (int)e;
+    const int sms = sm_count();
+    return launch_pdl(kernel, dim3((unsigned)(max_units < sms ? max_units : sms)), dim3(STREAM_THREADS), (size_t)bytes, stream, p, stages);
+}
+
+template <int GROUP>
+int run_gemm(const Args& p, bool pair, cudaStream_t stream) {
+    const int half = pair ? p.w.strips / 2 : p.w.strips;
+    if (p.offsets) {
+        if (!stream_stages<GROUPED, 1, GROUP>(p.w.blocks)) return -1;
+        const long long chunks = (long long)min(p.M, p.G) + p.M / 8;
+        if (pair) return launch_stream<GROUPED, 1, GROUP, true>(p, chunks * half, stream);
+        return launch_stream<GROUPED, 1, GROUP, false>(p, chunks * ((half + 1) / 2), stream);
+    }
+    const bool two = p.M > 8;
+    const long long units = pair ? half : (half + 1) / 2;
+    if (p.M <= (two ? 16 : 8) && units >= 4 * sm_count() && (two ? stream_stages<DENSE, 2, GROUP>(p.w.blocks) : stream_stages<DENSE, 1, GROUP>(p.w.blocks)))
+        return pair ? (two ? launch_stream<DENSE, 2, GROUP, true>(p, units, stream) : launch_stream<DENSE, 1, GROUP, true>(p, units, stream))
+                    : (two ? launch_stream<DENSE, 2, GROUP, false>(p, units, stream) : launch_stream<DENSE, 1, GROUP, false>(p, units, stream));
+    const dim3 grid(half);
+    return pair ? (two ? launch_pdl(gemm_q4_direct_kernel<2, 2, GROUP>, grid, 256, 0, stream, p) : launch_pdl(gemm_q4_direct_kernel<2, 1, GROUP>, grid, 256, 0, stream, p))
+                : (two ? launch_pdl(gemm_q4_direct_kernel<1, 2, GROUP>, grid, 256, 0, stream, p) : launch_pdl(gemm_q4_direct_kernel<1, 1, GROUP>, grid, 256, 0, stream, p));
+}
+
+template <int GROUP>
+int run_experts(const Args& up, const DownArgs& down, cudaStream_t stream) {
+    if (!stream_stages<EXPERTS, 1, GROUP>(up.w.blocks)) return -1;
+    const long long pairs = (long long)up.M * up.top_k, slots = pairs < up.E ? pairs : up.E;
+    const long long units = slots * (up.w.strips / 2) + (up.shared.codes ? up.shared.strips / 2 : 0);
+    int e = launch_stream<EXPERTS, 1, GROUP, true>(up, units, stream);
+    if (e) return e;
+    e = (int)cudaFuncSetAttribute(experts_down_kernel<GROUP>, cudaFuncAttributeMaxDynamicSharedMemorySize, DownStage<GROUP>::BYTES);
+    if (e) return e;
+    return launch_pdl_cluster(experts_down_kernel<GROUP>, dim3((down.down.strips + DOWN_MT - 1) / DOWN_MT, 1, down.S), dim3(DOWN_THREADS),
+                              (size_t)DownStage<GROUP>::BYTES, stream, down.S, down);
+}
+
+uint32_t g_wait_limit = WAIT_LIMIT_US;
+int g_test_fault = 0;
 
 }  // namespace
 
@@ -407,35 +811,31 @@ Weight weight(const void* codes, const void* scales, int N, int K, int group, in
 
 // x: [M, K] bfloat16, row pitch ldx; codes, scales: a weight of G groups of N rows (a pair's: both halves) and K columns; out: [M, N] (a pair:
 // [M, N / 2] act(gate) * up) float32 or bfloat16, row pitch ldo; offsets: null (G must be 1) or [G + 1], rows [offsets[g], offsets[g + 1]) meet group g.
+// Returns -1, with nothing launched, for more than 1,024 groups, or groups of rows that shared memory does not hold (K beyond 7,000 or so).
 MOE_API int moe_gemm_q4(const void* x, int ldx, int M, const void* codes, const void* scales, int G, int N, int K, int group, int pair, void* out,
-                        int out_bf16, int ldo, const float* bias, const int* offsets, int act, float act_param, cudaStream_t stream) {
+                        int out_bf16, int ldo, const float* bias, const int* offsets, int act, float act_param, int* status, cudaStream_t stream) {
     if (M <= 0 || N <= 0) return 0;
-    if (!x || !codes || !scales || !out || K <= 0 || G <= 0 || (G > 1 && !offsets) || (pair && N % 2) || G > 65535) return (int)cudaErrorInvalidValue;
-    GemmArgs p = {};
+    if (!x || !codes || !scales || !out || K <= 0 || G <= 0 || (G > 1 && !offsets) || (pair && N % 2)) return (int)cudaErrorInvalidValue;
+    if (G > GROUPS_MAX) return -1;
+    Args p = {};
     p.w = weight(codes, scales, N, K, group, pair);
-    p.rows.x = (const __nv_bfloat16*)x, p.rows.ldx = ldx, p.rows.vec = K % 4 == 0 && ldx % 4 == 0 && ((uintptr_t)x & 7) == 0;
-    p.out = out, p.out_bf16 = out_bf16, p.ldo = ldo, p.bias = bias, p.offsets = offsets, p.M = M, p.N = pair ? N / 2 : N;
-    p.act = act, p.act_param = act_param;
-    const dim3 grid(pair ? p.w.strips / 2 : p.w.strips, G);
-    constexpr int W = 8;
-    const bool two = offsets ? true : M > 8;
-#define GO(GR)                                                                                            \
-    (pair ? (two ? launch_pdl(gemm_q4_kernel<W, 2, 2, GR>, grid, W * 32, 0, stream, p)                    \
-                 : launch_pdl(gemm_q4_kernel<W, 2, 1, GR>, grid, W * 32, 0, stream, p))                   \
-          : (two ? launch_pdl(gemm_q4_kernel<W, 1, 2, GR>, grid, W * 32, 0, stream, p)                    \
-                 : launch_pdl(gemm_q4_kernel<W, 1, 1, GR>, grid, W * 32, 0, stream, p)))
+    p.x = (const __nv_bfloat16*)x, p.ldx = ldx, p.M = M, p.vec = K % 4 == 0 && ldx % 4 == 0 && ((uintptr_t)x & 7) == 0;
+    p.out = out, p.out_bf16 = out_bf16, p.ldo = ldo, p.bias = bias, p.offsets = offsets, p.G = G, p.N = pair ? N / 2 : N;
+    p.act = act, p.act_param = act_param, p.bits = q4::bits(), p.waits = q4::Waits{status, g_wait_limit, g_test_fault};
+#define GO(GR) run_gemm<GR>(p, pair != 0, stream)
     BY_GROUP(GO);
 #undef GO
 }
 
-// bfloat16 elements of scratch that moe_experts_q4 wants
+// Bytes of scratch that moe_experts_q4 wants, 16-byte aligned
 MOE_API long long moe_experts_q4_scratch(int T, int top_k, int E, int size, int shared) {
     const long long slots = (long long)T * top_k < E ? (long long)T * top_k : E;
-    return slots * FEW * ((size + 15) / 16 * 16) + (long long)FEW * ((shared + 15) / 16 * 16);
+    return (slots * ((size + 63) / 64) + (shared + 63) / 64) * 2048;
 }
 
 // x: [T, H] bfloat16, row pitch ldx; idx, wk: [T, top_k]; gate: [T] or null; gu [E, 2 size, H] and sgu [2 shared, H] pairs, down [E, H, size], sdown
-// [H, shared]; shared 0: no shared expert.  Returns -1 for what it does not take: more than 8 tokens, 1,024 experts or 512 picks.
+// [H, shared]; shared 0: no shared expert.  Returns -1 for what it does not take: more than 8 tokens, 1,024 experts or 128 picks, rows that shared
+// memory does not hold (H beyond 7,000 or so).
 MOE_API int moe_experts_q4(const void* x, int ldx, int T, int H, const int* idx, const float* wk, int top_k, int E, int size, const void* gu_codes,
                            const void* gu_scales, const void* down_codes, const void* down_scales, int shared, const void* sgu_codes,
                            const void* sgu_scales, const void* sdown_codes, const void* sdown_scales, const float* gate, int group, void* scratch,
@@ -444,22 +844,20 @@ MOE_API int moe_experts_q4(const void* x, int ldx, int T, int H, const int* idx,
     if (T > FEW || E > EXPERTS_MAX || (long long)T * top_k > PAIRS_MAX) return -1;
     if (!x || !idx || !wk || !scratch || !out || E <= 0 || top_k <= 0 || size <= 0 || ((uintptr_t)scratch & 15) || (shared > 0 && (!sgu_codes || !sdown_codes)))
         return (int)cudaErrorInvalidValue;
-    LayerArgs p = {};
-    p.x = (const __nv_bfloat16*)x, p.ldx = ldx, p.vec = H % 4 == 0 && ldx % 4 == 0 && ((uintptr_t)x & 7) == 0;
-    p.T = T, p.H = H, p.E = E, p.top_k = top_k, p.idx = idx, p.wk = wk, p.gate = gate;
-    p.gu = weight(gu_codes, gu_scales, 2 * size, H, group, 1), p.down = weight(down_codes, down_scales, H, size, group, 0);
-    if (shared > 0) p.sgu = weight(sgu_codes, sgu_scales, 2 * shared, H, group, 1), p.sdown = weight(sdown_codes, sdown_scales, H, shared, group, 0);
-    p.pitch = (size + 15) / 16 * 16, p.spitch = (shared + 15) / 16 * 16;
+    Args up = {};
+    DownArgs d = {};
+    up.x = (const __nv_bfloat16*)x, up.ldx = ldx, up.vec = H % 4 == 0 && ldx % 4 == 0 && ((uintptr_t)x & 7) == 0, up.M = T;
+    up.idx = idx, up.top_k = top_k, up.E = E, up.bits = q4::bits(), up.waits = q4::Waits{status, g_wait_limit, g_test_fault};
+    up.w = weight(gu_codes, gu_scales, 2 * size, H, group, 1), d.down = weight(down_codes, down_scales, H, size, group, 0);
+    if (shared > 0) up.shared = weight(sgu_codes, sgu_scales, 2 * shared, H, group, 1), d.shared = weight(sdown_codes, sdown_scales, H, shared, group, 0);
     const long long slots = (long long)T * top_k < E ? (long long)T * top_k : E;
-    p.act = (__nv_bfloat16*)scratch, p.sact = p.act + slots * FEW * p.pitch;
-    p.out = out, p.out_bf16 = out_bf16, p.ldo = ldo, p.status = status;
-    const long long up = p.spitch / 16 + slots * (p.pitch / 16);
-    if (up > 0x7fffffffll) return -1;
-    auto run = [&](auto up_kernel, auto down_kernel) {
-        const int e = launch_pdl(up_kernel, dim3((unsigned)up), 256, 0, stream, p);
-        return e ? e : launch_pdl(down_kernel, dim3(p.down.strips), 512, 0, stream, p);
-    };
-#define GO(GR) run(experts_up_kernel<8, GR>, experts_down_kernel<16, GR>)
+    up.frag = (uint8_t*)scratch, up.frag_blocks = d.down.blocks, up.sfrag = up.frag + slots * d.down.blocks * 2048;
+    d.frag = up.frag, d.sfrag = up.sfrag, d.bits = up.bits, d.waits = up.waits;
+    d.T = T, d.H = H, d.E = E, d.top_k = top_k, d.idx = idx, d.wk = wk, d.gate = gate, d.out = out, d.out_bf16 = out_bf16, d.ldo = ldo;
+    d.S = max(1, min(8, sm_count() / ((d.down.strips + DOWN_MT - 1) / DOWN_MT)));      // one block an SM
+#define GO(GR) run_experts<GR>(up, d, stream)
     BY_GROUP(GO);
 #undef GO
 }
+
+void q4::few_rows_wait_test(int fault, uint32_t wait_limit) { g_test_fault = fault, g_wait_limit = wait_limit; }

@@ -47,34 +47,17 @@ struct Args {
     float act_param;
     int* status;
     uint32_t wait_limit;
+    q4::Bits bits;
     int test_fault;                // 0; the wait test: 1 nothing is loaded, 2 no product is issued, 3 no value is formed
 };
 
 // ---- PTX wrappers ----------------------------------------------------------------------------------------------------------------------
-__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count)); }
-__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void mbar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
-__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
-    return ok != 0;
-}
-// false: the barrier did not complete in time, or another role gave up
+using q4::mbar_arrive;
+using q4::mbar_expect_tx;
+using q4::mbar_init;
+using q4::smem_u32;
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, const Args& p, int site) {
-    if (mbar_try(bar, parity)) return true;
-    const unsigned long long t0 = global_ns();
-    for (uint32_t i = 1;; i++) {
-        if (mbar_try(bar, parity)) return true;
-        if ((i & 31u) == 0) {
-            if (abort_flag && *abort_flag) return false;
-            if (global_ns() - t0 > (unsigned long long)p.wait_limit * 1000ull) break;
-        }
-    }
-    wait_ran_out(p.status, site);
-    return false;
+    return q4::mbar_wait(bar, parity, abort_flag, p.wait_limit, p.status, site);
 }
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst), "l"(map), "r"(x), "r"(y),
@@ -244,7 +227,7 @@ gemm_q4_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
                         uint32_t a[4];
-                        q4::unpack(q4::word(code[d][i], j), a);
+                        q4::unpack(q4::word(code[d][i], j), p.bits, a);
                         const uint32_t s2 = sc[d][i].s[GROUP == 32 ? j / 2 : 0];
                         const uint32_t lo2 = __byte_perm(s2, 0, 0x1010), hi2 = __byte_perm(s2, 0, 0x3232);
 #pragma unroll
@@ -454,7 +437,7 @@ MOE_API int moe_gemm_q4_tc(const void* x, int ldx, int M, const void* codes, con
     p.N = pair ? N / 2 : N;
     p.w.strips = (p.N + 15) / 16 * (pair ? 2 : 1), p.w.blocks = (K + 63) / 64, p.w.qgroups = (K + group - 1) / group;
     p.out = out, p.out_bf16 = out_bf16, p.ldo = ldo, p.bias = bias, p.offsets = offsets, p.G = G, p.M = M;
-    p.act = act, p.act_param = act_param, p.status = status, p.wait_limit = g_wait_limit, p.test_fault = g_test_fault;
+    p.act = act, p.act_param = act_param, p.status = status, p.wait_limit = g_wait_limit, p.test_fault = g_test_fault, p.bits = q4::bits();
     p.n_tiles = pair ? (p.N + 63) / 64 : (p.N + FEATURES - 1) / FEATURES;
     // rows of a tile: as few tiles as 192 rows allow, of equal height
     const int mt = (M + BN - 1) / BN;
@@ -484,4 +467,5 @@ MOE_API int moe_gemm_q4_tc(const void* x, int ldx, int M, const void* codes, con
 MOE_API void moe_q4_set_wait_test(int fault, unsigned wait_limit) {
     g_test_fault = fault >= 1 && fault <= 3 ? fault : 0;
     g_wait_limit = wait_limit ? wait_limit : WAIT_LIMIT_US;
+    q4::few_rows_wait_test(g_test_fault, g_wait_limit);
 }

@@ -139,7 +139,7 @@ quantize_kernel(const T* __restrict__ w, int N, int K, int pair, int strips, int
 template <int GROUP>
 __global__ void __launch_bounds__(256)
 dequantize_kernel(const uint4* __restrict__ codes, const uint32_t* __restrict__ scales, int N, int K, int pair, int strips, int blocks, int qgroups,
-                  int vec, long long units, __nv_bfloat16* __restrict__ out) {
+                  int vec, long long units, const q4::Bits bits, __nv_bfloat16* __restrict__ out) {
     pdl_sync();
     const int lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
     const long long unit = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
@@ -155,7 +155,7 @@ dequantize_kernel(const uint4* __restrict__ codes, const uint32_t* __restrict__ 
 #pragma unroll
     for (int j = 0; j < 4; j++) {
         uint32_t a[4];
-        q4::unpack(q4::word(c, j), a);
+        q4::unpack(q4::word(c, j), bits, a);
         const int k = b * 64 + 16 * j + 4 * t;
 #pragma unroll
         for (int half = 0; half < 2; half++) {
@@ -214,7 +214,7 @@ MOE_API int moe_q4_dequantize(const void* codes, const void* scales, int G, int 
     const int vec = K % 4 == 0 && ((uintptr_t)out & 7) == 0;
 #define GO(GR)                                                                                                                             \
     launch_pdl(dequantize_kernel<GR>, (unsigned)grid, 256, 0, stream, (const uint4*)codes, (const uint32_t*)scales, N, K, pair, strips, blocks, qgroups, \
-               vec, units, (__nv_bfloat16*)out)
+               vec, units, q4::bits(), (__nv_bfloat16*)out)
     BY_GROUP(GO);
 #undef GO
 }

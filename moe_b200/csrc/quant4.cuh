@@ -26,12 +26,19 @@ struct Weight {
     int N, K;                      // rows (of both halves of a pair) and k
 };
 
-// The eight elements of a word as bfloat16 pairs, a[0..3] the fragment's registers: 0x4300 | n is 128 + n, less 136 is q, exactly.
-__device__ __forceinline__ void unpack(uint32_t w, uint32_t (&a)[4]) {
+// The eight elements of a word as bfloat16 pairs, a[0..3] the fragment's registers: 0x4300 | n is 128 + n, less 136 is q, exactly.  The
+// mask and the exponent come as kernel arguments: (w & mask) | exponent is then ONE instruction (with both as literals it is two, and
+// the logic unit is what bounds these kernels).
+struct Bits {
+    uint32_t mask, exponent;
+};
+inline Bits bits() { return Bits{0x000f000fu, 0x43004300u}; }
+__device__ __forceinline__ void unpack(uint32_t w, const Bits& k, uint32_t (&a)[4]) {
     const __nv_bfloat162 off = __halves2bfloat162(__ushort_as_bfloat16(0x4308), __ushort_as_bfloat16(0x4308));
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        const uint32_t v = ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+        uint32_t v;
+        asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(v) : "r"(w >> (4 * i)), "r"(k.mask), "r"(k.exponent));
         const __nv_bfloat162 q = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), off);
         a[i] = *reinterpret_cast<const uint32_t*>(&q);
     }
@@ -39,19 +46,13 @@ __device__ __forceinline__ void unpack(uint32_t w, uint32_t (&a)[4]) {
 __device__ __forceinline__ float scale_lo(uint32_t s) { return __uint_as_float(s << 16); }            // row r
 __device__ __forceinline__ float scale_hi(uint32_t s) { return __uint_as_float(s & 0xffff0000u); }    // row r + 8
 
-// D += A B of one 16 x 16 tile of weights and eight columns of tokens
-__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], const uint2 b) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y));
+// D = A B + C of one 16 x 16 tile of weights and eight columns of tokens
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float c0, float c1, float c2, float c3) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
 }
 
-// Weights are read once: past L1.
-__device__ __forceinline__ uint4 ld_codes(const uint4* p) {
-    uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-    return v;
-}
 __device__ __forceinline__ uint32_t word(const uint4& v, int j) { return j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w; }
 
 // Scales of a block of 64 k: two where a group is 32, one otherwise (the same for two blocks where it is 128).
@@ -67,5 +68,62 @@ struct Scales {
         }
     }
 };
+
+// ---- barriers and bulk copies ------------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count)); }
+__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok != 0;
+}
+// the same without suspending the thread
+__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok != 0;
+}
+// false: the barrier did not complete within limit_us (the site is recorded), or another role of the block gave up
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, uint32_t limit_us, int* status, int site) {
+    if (mbar_try(bar, parity)) return true;
+    const unsigned long long t0 = global_ns();
+    for (uint32_t i = 1;; i++) {
+        if (mbar_try(bar, parity)) return true;
+        if ((i & 31u) == 0) {
+            if (abort_flag && *abort_flag) return false;
+            if (global_ns() - t0 > (unsigned long long)limit_us * 1000ull) break;
+        }
+    }
+    wait_ran_out(status, site);
+    return false;
+}
+// `bytes` (a multiple of 16) from global memory, counted by a barrier of this block
+__device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+__device__ __forceinline__ uint4 lds16(uint32_t a) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+    return v;
+}
+__device__ __forceinline__ uint32_t lds4(uint32_t a) {
+    uint32_t v;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a));
+    return v;
+}
+__device__ __forceinline__ void sts8(uint32_t a, uint2 v) { asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(a), "r"(v.x), "r"(v.y) : "memory"); }
+
+// Limits and faults of the waits, set for all kernels of the library by moe_q4_set_wait_test.
+struct Waits {
+    int* status;
+    uint32_t limit_us;
+    int test_fault;
+};
+
+void few_rows_wait_test(int fault, uint32_t wait_limit);      // gemm_q4.cu
 
 }  // namespace q4

@@ -38,7 +38,7 @@ def lib():
         P, I, F = c_void_p, c_int, c_float
         for name, args in (("moe_q4_quantize", [P, I, I, I, I, I, I, P, P, P, P]),
                            ("moe_q4_dequantize", [P, P, I, I, I, I, I, P, P]),
-                           ("moe_gemm_q4", [P, I, I, P, P, I, I, I, I, I, P, I, I, P, P, I, F, P]),
+                           ("moe_gemm_q4", [P, I, I, P, P, I, I, I, I, I, P, I, I, P, P, I, F, P, P]),
                            ("moe_gemm_q4_tc", [P, I, I, P, P, I, I, I, I, I, P, I, I, P, P, I, F, I, P, P]),
                            ("moe_experts_q4", [P, I, I, I, P, P, I, I, I, P, P, P, P, I, P, P, P, P, P, I, P, P, I, I, P, P])):
             fn = getattr(L, name)
@@ -74,7 +74,7 @@ class Weight4:
         strips = self.G * _strips(self.N, pair)
         if (codes.dtype != torch.uint8 or scales.dtype != torch.bfloat16 or not codes.is_contiguous() or not scales.is_contiguous()
                 or codes.numel() != strips * -(-self.K // 64) * 512 or scales.numel() != strips * -(-self.K // group) * 16
-                or codes.data_ptr() % 16 or scales.data_ptr() % 4 or codes.device != scales.device):
+                or codes.data_ptr() % 16 or scales.data_ptr() % 16 or codes.device != scales.device):
             raise core.KernelError(f"Weight4: codes and scales of {tuple(shape)} in groups of {group} are contiguous uint8 and bfloat16 tensors "
                                    f"of {strips * -(-self.K // 64) * 512} and {strips * -(-self.K // group) * 16} elements on one device")
         self.codes, self.scales, self.shape, self.group, self.pair = codes, scales, tuple(shape), int(group), bool(pair)
@@ -180,12 +180,15 @@ def gemm4(x: torch.Tensor, w: Weight4, out: torch.Tensor, *, swiglu: bool = Fals
             1 if out.dtype == torch.bfloat16 else 0, out.stride(0), _on(bias, dev, "bias", torch.float32, N),
             _on(group_offsets, dev, "group_offsets", torch.int32, w.G + 1), code, float(act_param))
     st = _on(status, dev, "status", torch.int32)
-    if M > FEW_ROWS and st is not None:
+    if st is not None and (M > FEW_ROWS if group_offsets is None else M > 16 * w.G):
         done = lib().moe_gemm_q4_tc(*args, 1 if group_offsets is not None else _splits(M, N, w, dev), st, core._stream())
         if done != -1:
             core._ok(done, "gemm4")
             return out
-    core._ok(lib().moe_gemm_q4(*args, core._stream()), "gemm4")
+    done = lib().moe_gemm_q4(*args, st, core._stream())
+    if done == -1:
+        raise core.KernelError("gemm4: more than 1,024 weights in a stack, or K too large for one")
+    core._ok(done, "gemm4")
     return out
 
 
@@ -208,7 +211,7 @@ def experts4(x: torch.Tensor, topk_idx: torch.Tensor, topk_w: torch.Tensor, gate
     x: bfloat16 [T, H]; topk_idx int32 and topk_w float32 [T, k]; gate_up: a pair's stack [E, 2 I, H], down: [E, H, I]; the shared expert's two
     likewise without the stack, shared_gate float32 [T] (None: 1); out: float32 or bfloat16 [T, H].  An index of -1 is no pick
     (all of a row's: zeros but for the shared expert), any other outside [0, E) is reported through ``status`` and taken for none.  False, with
-    nothing launched, for more tokens, 1,024 experts or 512 picks than that."""
+    nothing launched, for more tokens, 1,024 experts or 128 picks than that."""
     dev = x.device
     _here(dev, "experts4")
     _matrix(x, dev, "x", (torch.bfloat16,))
@@ -231,12 +234,12 @@ def experts4(x: torch.Tensor, topk_idx: torch.Tensor, topk_w: torch.Tensor, gate
         raise core.KernelError("experts4: the weights of a layer have one group size")
     pi, pw = _on(topk_idx, dev, "topk_idx", torch.int32), _on(topk_w, dev, "topk_w", torch.float32)
     pg, ps = _on(shared_gate, dev, "shared_gate", torch.float32, T), _on(status, dev, "status", torch.int32)
-    if T > EXPERTS_TOKENS or E > 1024 or T * k > 512:
+    if T > EXPERTS_TOKENS or E > 1024 or T * k > 128:
         return False
     if not T:
         return True
     L = lib()
-    scratch = torch.empty(L.moe_experts_q4_scratch(T, k, E, size, shared), dtype=torch.bfloat16, device=dev)
+    scratch = torch.empty(L.moe_experts_q4_scratch(T, k, E, size, shared), dtype=torch.uint8, device=dev)
     s = (None, None, None, None) if not shared else (shared_gate_up.codes.data_ptr(), shared_gate_up.scales.data_ptr(),
                                                      shared_down.codes.data_ptr(), shared_down.scales.data_ptr())
     code = L.moe_experts_q4(x.data_ptr(), x.stride(0), T, H, pi, pw, k, E, size, gate_up.codes.data_ptr(), gate_up.scales.data_ptr(),
