@@ -21,6 +21,13 @@ using q4::lds4;
 using q4::smem_u32;
 using q4::sts8;
 
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
 // Four neighbouring k of a row, zeros beyond K or where there is no row.
 __device__ __forceinline__ uint2 row4(const __nv_bfloat16* row, int k, int K, int vec) {
     if (!row || k >= K) return make_uint2(0u, 0u);
@@ -105,42 +112,41 @@ struct Picked {
     uint32_t takes[PAIRS_MAX];             // of a slot: the tokens that picked it
     __device__ __forceinline__ int slot_of(int e) const { return before[e >> 5] + __popc(bits[e >> 5] & ((1u << (e & 31)) - 1)); }
 };
-// By all threads of the block; ends with a barrier.
-__device__ __forceinline__ void find_picked(const int* idx, int T, int top_k, int E, int* status, Picked& s) {
+// By one warp; the block's other threads read it behind a barrier.
+__device__ __forceinline__ void find_picked(const int* idx, int T, int top_k, int E, int* status, Picked& s, int lane) {
     const int pairs = T * top_k;
-    for (int i = threadIdx.x; i < EXPERTS_MAX / 32; i += blockDim.x) s.bits[i] = 0;
-    for (int i = threadIdx.x; i < pairs; i += blockDim.x) s.takes[i] = 0;
-    __syncthreads();
-    for (int i = threadIdx.x; i < pairs; i += blockDim.x) {
+    s.bits[lane] = 0;
+    __syncwarp();
+    for (int i = lane; i < pairs; i += 32) {
         int e = idx[i];
-        if (e < 0 || e >= E) {
+        s.takes[i] = 0;
+        if (e >= 0 && e < E)
+            atomicOr(&s.bits[e >> 5], 1u << (e & 31));
+        else {
             if (e != -1 && status) atomicOr(status, ST_BAD_EXPERT);
             e = -1;
-        } else
-            atomicOr(&s.bits[e >> 5], 1u << (e & 31));
+        }
         s.pick[i] = (short)e;
     }
-    __syncthreads();
-    if (threadIdx.x < 32) {
-        const int n = __popc(s.bits[threadIdx.x]);
-        int upto = n;
+    __syncwarp();
+    const int n = __popc(s.bits[lane]);
+    int upto = n;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int v = __shfl_up_sync(0xffffffffu, upto, o);
-            if ((int)threadIdx.x >= o) upto += v;
-        }
-        s.before[threadIdx.x] = upto - n;
-        if (threadIdx.x == 31) s.before[32] = upto;
+    for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += v;
     }
-    __syncthreads();
-    for (int i = threadIdx.x; i < pairs; i += blockDim.x) {
+    s.before[lane] = upto - n;
+    if (lane == 31) s.before[32] = upto;
+    __syncwarp();
+    for (int i = lane; i < pairs; i += 32) {
         const int e = s.pick[i];
         if (e < 0) continue;
         const int slot = s.slot_of(e);
         s.expert[slot] = (short)e;
         atomicOr(&s.takes[slot], 1u << (i / top_k));
     }
-    __syncthreads();
+    __syncwarp();
 }
 
 struct Args {
@@ -304,7 +310,8 @@ gemm_q4_stream_kernel(const __grid_constant__ Args p, const int stages) {
     else {
         pdl_sync();
         if (MODE == EXPERTS) {
-            find_picked(p.idx, p.M, p.top_k, p.E, blockIdx.x == 0 ? p.waits.status : nullptr, picked);
+            if (warp == 0) find_picked(p.idx, p.M, p.top_k, p.E, blockIdx.x == 0 ? p.waits.status : nullptr, picked, lane);
+            __syncthreads();
             shared_units = p.shared.codes ? p.shared.strips / 2 : 0;
             units = shared_units + picked.before[32] * per;
         } else {
@@ -420,12 +427,14 @@ gemm_q4_stream_kernel(const __grid_constant__ Args p, const int stages) {
             row0 = s_off[v.g] + (c - s_first[v.g]) * 8 * NT, rows = min(8 * NT, s_off[v.g + 1] - row0);
             if (first > u0) team_sync<TEAMS * TEAM_W * 32>(TEAMS + 1);      // the rows before are done with
         }
-        const int b16 = blocks * 16;
-        for (int i = threadIdx.x; i < b16 * 8 * NT; i += TEAMS * TEAM_W * 32) {
-            const int c = i / b16, k4 = i - c * b16;     // row, four k
-            const __nv_bfloat16* row = c < rows ? p.x + (size_t)(row0 + c) * p.ldx : nullptr;
+        // a thread's four k of all rows are asked for at once
+        for (int k4 = threadIdx.x; k4 < blocks * 16; k4 += TEAMS * TEAM_W * 32) {
+            uint2 y[8 * NT];
+#pragma unroll
+            for (int c = 0; c < 8 * NT; c++) y[c] = row4(c < rows ? p.x + (size_t)(row0 + c) * p.ldx : nullptr, k4 * 4, p.w.K, p.vec);
             const int b = k4 >> 4, j = (k4 >> 2) & 3, tt = k4 & 3;
-            sts8(xs + ((b * NT + (c >> 3)) * 2 + (j >> 1)) * 512 + ((c & 7) * 4 + tt) * 16 + (j & 1) * 8, row4(row, k4 * 4, p.w.K, p.vec));
+#pragma unroll
+            for (int c = 0; c < 8 * NT; c++) sts8(xs + ((b * NT + (c >> 3)) * 2 + (j >> 1)) * 512 + ((c & 7) * 4 + tt) * 16 + (j & 1) * 8, y[c]);
         }
         team_sync<TEAMS * TEAM_W * 32>(TEAMS + 1);
         const int end = run_end(first);
@@ -517,8 +526,9 @@ gemm_q4_stream_kernel(const __grid_constant__ Args p, const int stages) {
 // Four strips of the output go through ALL picked experts and the shared one, w_te on the sums of each block of 64 k: nothing is left to
 // combine.  Tokens that did not pick an expert meet it with the zeros that the first kernel left.  A block of 64 k of the rows is 2 KB: for each 16 k a
 // B fragment of 32 lanes x (four k rounded to bfloat16, what that left rounded likewise).  Grid: (fours of strips, 1, S); the S blocks of a unit are
-// a cluster and share its blocks of 64 k, sixteen a stage and one a warp; the first block adds their sums up in order.
-constexpr int DOWN_W = 16, DOWN_MT = 4, DOWN_STAGES = 3, DOWN_THREADS = DOWN_W * 32 + 32;
+// a cluster and share its blocks of 64 k; the first of them adds their sums up in order.  A warp takes every sixteenth block and copies for itself
+// into a ring of its own (cp.async: its pieces of 512 bytes and less are too small for bulk copies, of which an SM issued one in ten to twenty cycles).
+constexpr int DOWN_W = 16, DOWN_MT = 4, DOWN_DEPTH = 3, DOWN_THREADS = DOWN_W * 32;
 struct DownArgs {
     Weight down, shared;           // shared.codes null: none
     const uint8_t *frag, *sfrag;
@@ -529,184 +539,136 @@ struct DownArgs {
     void* out;
     int out_bf16, ldo;
     q4::Bits bits;
-    q4::Waits waits;
 };
 template <int GROUP>
-struct DownStage {
-    static constexpr int SCALE_BLOCK = GROUP == 32 ? 64 : 32;      // (128: each block has its own copy)
-    static constexpr int CODES = DOWN_W * 512, SCALES = DOWN_W * SCALE_BLOCK, X = DOWN_W * 2048;
-    static constexpr int STAGE = DOWN_MT * (CODES + SCALES) + X, BYTES = DOWN_STAGES * STAGE;
-    static constexpr int RED_FLOATS = DOWN_W * DOWN_MT * 8 * 17;   // lies over the stages, and the other blocks' sums behind it
+struct DownRing {
+    static constexpr int SCALES = GROUP == 32 ? 64 : 32, X = DOWN_MT * (512 + SCALES), SLOT = X + 2048, BYTES = DOWN_W * DOWN_DEPTH * SLOT;
+    static constexpr int RED_FLOATS = DOWN_W * DOWN_MT * 8 * 17;   // lies over the rings, and the other blocks' sums behind it
     static_assert(RED_FLOATS * 4 + 8 * DOWN_MT * 128 * 4 <= BYTES, "sums");
 };
 
 template <int GROUP>
 __global__ void __launch_bounds__(DOWN_THREADS, 1)
 experts_down_kernel(const __grid_constant__ DownArgs p) {
-    using D = DownStage<GROUP>;
+    using D = DownRing<GROUP>;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ Picked picked;
     __shared__ float wk[PAIRS_MAX];
     __shared__ __align__(16) float wt[PAIRS_MAX + 1][FEW];      // a slot's weight of each token; the last one's: the shared expert's gate
-    __shared__ __align__(8) unsigned long long s_bars[2][DOWN_STAGES];
-    __shared__ volatile int s_abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3, strip0 = blockIdx.x * DOWN_MT, rank = blockIdx.z;
-    if (threadIdx.x == 0) {
-        s_abort = 0;
-        for (int s = 0; s < DOWN_STAGES; s++) q4::mbar_init(smem_u32(&s_bars[0][s]), 1), q4::mbar_init(smem_u32(&s_bars[1][s]), DOWN_W);
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    }
     // The picks were written at least two kernels ago (this one's predecessor let it in behind its own wait): they, and the weights, are
     // read before the wait.
-    find_picked(p.idx, p.T, p.top_k, p.E, nullptr, picked);
-    const int slots = picked.before[32];
-    for (int i = threadIdx.x; i < slots * FEW; i += DOWN_THREADS) wt[i >> 3][i & 7] = 0.f;
     const int pairs = p.T * p.top_k;
-    if (threadIdx.x < pairs) wk[threadIdx.x] = p.wk[threadIdx.x];
+    if (warp == 0)
+        find_picked(p.idx, p.T, p.top_k, p.E, nullptr, picked, lane);
+    else if (threadIdx.x - 32 < pairs)
+        wk[threadIdx.x - 32] = p.wk[threadIdx.x - 32];
+    const float gate = threadIdx.x < p.T && p.gate ? p.gate[threadIdx.x] : 1.f;
     __syncthreads();
-    if (threadIdx.x < pairs && picked.pick[threadIdx.x] >= 0) {
-        const int e = picked.pick[threadIdx.x], c = threadIdx.x / p.top_k;
-        float v = 0.f;
-        bool first = true;                                      // an expert may be picked twice: the first of the picks adds them up
-        for (int j = c * p.top_k; j < (c + 1) * p.top_k; j++)
-            if (picked.pick[j] == e) first = first && j >= (int)threadIdx.x, v += wk[j];
-        if (first) wt[picked.slot_of(e)][c] = v;
-    }
-    if (threadIdx.x < FEW) wt[slots][threadIdx.x] = (int)threadIdx.x < p.T && p.shared.codes ? (p.gate ? p.gate[threadIdx.x] : 1.f) : 0.f;
-    __syncthreads();
-    const int nb = p.down.blocks, total = slots * nb + (p.shared.codes ? p.shared.blocks : 0);
-    const int lo = (int)((long long)total * rank / p.S), hi = (int)((long long)total * (rank + 1) / p.S), count = (hi - lo + DOWN_W - 1) / DOWN_W;
-    bool ok = true;
+    const int slots = picked.before[32], nb = p.down.blocks, total = slots * nb + (p.shared.codes ? p.shared.blocks : 0);
+    const int lo = (int)((long long)total * rank / p.S), hi = (int)((long long)total * (rank + 1) / p.S);
+    const int count = hi - lo > warp ? (hi - lo - warp - 1) / DOWN_W + 1 : 0;      // this warp's blocks
 
-    if (warp == DOWN_W) {
-        // ---- copies.  The pieces of a stage that lie in one expert are neighbours in memory: a lane for each of its strips' codes and scales, one for
-        // the rows' fragments.
-        ok = p.waits.test_fault != 1;
-        int done = 0;
-        struct Place {
-            int slot, b;
-        };
-        const int strip = min(strip0 + (lane & 3), p.down.strips - 1);
-        // one stage from `at` on; where it ends
-        auto copy_stage = [&](int st, Place at, bool codes, bool rows) {
-            const uint32_t base = smem_u32(smem) + st % DOWN_STAGES * D::STAGE, bar = smem_u32(&s_bars[0][st % DOWN_STAGES]);
-            const int all = min(DOWN_W, hi - lo - st * DOWN_W);
-            for (int i = 0; i < all;) {
-                const bool own = at.slot < slots;
-                const Weight& w = own ? p.down : p.shared;
-                const int n = min(all - i, w.blocks - at.b);
-                if (codes && lane < DOWN_MT) {
-                    const size_t row = (size_t)(own ? picked.expert[at.slot] : 0) * w.strips + strip;
-                    q4::bulk_copy(base + lane * D::CODES + i * 512, w.codes + (row * w.blocks + at.b) * 32, n * 512, bar);
-                    const uint32_t sc = base + DOWN_MT * D::CODES + lane * D::SCALES + i * D::SCALE_BLOCK;
-                    const uint32_t* from = w.scales + row * w.qgroups * 8;
-                    if (GROUP == 128)
-                        for (int j = 0; j < n; j++) q4::bulk_copy(sc + j * 32, from + (size_t)((at.b + j) >> 1) * 8, 32, bar);
-                    else if (GROUP == 64)
-                        q4::bulk_copy(sc, from + (size_t)at.b * 8, n * 32, bar);
-                    else
-                        q4::bulk_copy(sc, from + (size_t)at.b * 16, min(2 * n, w.qgroups - 2 * at.b) * 32, bar);
-                }
-                if (rows && lane == DOWN_MT)
-                    q4::bulk_copy(base + DOWN_MT * (D::CODES + D::SCALES) + i * 2048, (own ? p.frag + (size_t)at.slot * nb * 2048 : p.sfrag) + (size_t)at.b * 2048, n * 2048, bar);
-                i += n, at.b += n;
-                if (own && at.b == nb) at.b = 0, at.slot++;
-            }
-            return at;
-        };
-        auto expect = [&](int st, Place at) {
-            const int all = min(DOWN_W, hi - lo - st * DOWN_W);
-            int bytes = all * (DOWN_MT * (512 + (GROUP == 32 ? 64 : 32)) + 2048);
-            if (GROUP == 32)                             // (a last block of no more than 32 k has one group)
-                for (int i = 0; i < all; i++) {
-                    if (2 * at.b + 1 >= (at.slot < slots ? p.down.qgroups : p.shared.qgroups)) bytes -= DOWN_MT * 32;
-                    if (++at.b == nb && at.slot < slots) at.b = 0, at.slot++;
-                }
-            if (lane == 0) q4::mbar_expect_tx(smem_u32(&s_bars[0][st % DOWN_STAGES]), bytes);
-            __syncwarp();
-        };
-        Place codes_at, rows_at;
-        codes_at.slot = min(lo / nb, slots), codes_at.b = lo - codes_at.slot * nb;
-        rows_at = codes_at;
-        for (int st = 0; st < min(count, DOWN_STAGES) && ok; st++) {
-            expect(st, codes_at);
-            codes_at = copy_stage(st, codes_at, true, false);
-        }
-        pdl_sync();
-        for (; done < count && ok; done++) {
-            if (done < DOWN_STAGES)
-                rows_at = copy_stage(done, rows_at, false, true);
-            else {
-                ok = q4::mbar_wait(smem_u32(&s_bars[1][done % DOWN_STAGES]), ((done / DOWN_STAGES) & 1) ^ 1, &s_abort, p.waits.limit_us, p.waits.status, 0x71);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                expect(done, codes_at);
-                codes_at = copy_stage(done, codes_at, true, true);
-            }
-            __syncwarp();
-        }
-        if (!ok && p.waits.test_fault != 1) {
-            s_abort = 1;
-            for (int i = max(0, done - DOWN_STAGES); i < done; i++)      // copies in flight must land
-                q4::mbar_wait(smem_u32(&s_bars[0][i % DOWN_STAGES]), (i / DOWN_STAGES) & 1, nullptr, p.waits.limit_us, p.waits.status, 0x72);
-        }
-    }
-    float acc[DOWN_MT][4] = {};
-    if (warp < DOWN_W) {
-        int slot = min((lo + warp) / nb, slots), b = lo + warp - slot * nb;      // this warp's block of the stage
-        for (int st = 0; st < count && ok; st++) {
-            const int s = st % DOWN_STAGES;
-            ok = q4::mbar_wait(smem_u32(&s_bars[0][s]), (st / DOWN_STAGES) & 1, &s_abort, p.waits.limit_us, p.waits.status, 0x74);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
-            if (lo + st * DOWN_W + warp < hi) {
-                const uint32_t base = smem_u32(smem) + s * D::STAGE, xa = base + DOWN_MT * (D::CODES + D::SCALES) + warp * 2048 + lane * 16;
-                float c[DOWN_MT][4], sum[DOWN_MT][4];
-                uint4 code[DOWN_MT];
-#pragma unroll
-                for (int m = 0; m < DOWN_MT; m++) code[m] = lds16(base + m * D::CODES + warp * 512 + lane * 16);
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const uint4 x = lds16(xa + j * 512);
-                    const bool fresh = GROUP == 32 ? j % 2 == 0 : j == 0, last = GROUP == 32 ? j % 2 == 1 : j == 3;
-#pragma unroll
-                    for (int m = 0; m < DOWN_MT; m++) {
-                        uint32_t a[4];
-                        q4::unpack(q4::word(code[m], j), p.bits, a);
-                        if (fresh)
-                            q4::mma(c[m], a, x.x, x.y, 0.f, 0.f, 0.f, 0.f);
-                        else
-                            q4::mma(c[m], a, x.x, x.y, c[m][0], c[m][1], c[m][2], c[m][3]);
-                        q4::mma(c[m], a, x.z, x.w, c[m][0], c[m][1], c[m][2], c[m][3]);
-                    }
-                    if (last)
-#pragma unroll
-                        for (int m = 0; m < DOWN_MT; m++) {
-                            uint32_t sc = lds4(base + DOWN_MT * D::CODES + m * D::SCALES + warp * D::SCALE_BLOCK + (GROUP == 32 ? j / 2 * 32 : 0) + r * 4);
-                            if (GROUP == 32 && j == 3 && 2 * b + 1 >= (slot < slots ? p.down.qgroups : p.shared.qgroups)) sc = 0u;      // (not copied; its q are 0)
-                            const float l = q4::scale_lo(sc), h = q4::scale_hi(sc);
-                            const bool one = GROUP != 32 || j == 1;
-                            sum[m][0] = one ? l * c[m][0] : fmaf(l, c[m][0], sum[m][0]), sum[m][1] = one ? l * c[m][1] : fmaf(l, c[m][1], sum[m][1]);
-                            sum[m][2] = one ? h * c[m][2] : fmaf(h, c[m][2], sum[m][2]), sum[m][3] = one ? h * c[m][3] : fmaf(h, c[m][3], sum[m][3]);
-                        }
-                }
-                const float2 w2 = *reinterpret_cast<const float2*>(&wt[slot][2 * t]);
-#pragma unroll
-                for (int m = 0; m < DOWN_MT; m++) {
-                    acc[m][0] = fmaf(w2.x, sum[m][0], acc[m][0]), acc[m][1] = fmaf(w2.y, sum[m][1], acc[m][1]);
-                    acc[m][2] = fmaf(w2.x, sum[m][2], acc[m][2]), acc[m][3] = fmaf(w2.y, sum[m][3], acc[m][3]);
-                }
-            }
-            __syncwarp();
-            if (lane == 0) q4::mbar_arrive(smem_u32(&s_bars[1][s]));
+    struct Place {
+        int slot, b;
+        __device__ __forceinline__ void next(int slots, int nb) {
             b += DOWN_W;
             while (slot < slots && b >= nb) b -= nb, slot++;
         }
-        if (!ok) s_abort = 1;
+    };
+    const uint32_t ring = smem_u32(smem) + warp * DOWN_DEPTH * D::SLOT;
+    // a lane's piece of the scales: strip lane / (2 NS)
+    constexpr int NS = q4::Scales<GROUP>::N;
+    int strips[DOWN_MT];
+#pragma unroll
+    for (int m = 0; m < DOWN_MT; m++) strips[m] = min(strip0 + m, p.down.strips - 1);
+    const int scale_strip = min(strip0 + lane / (2 * NS), p.down.strips - 1);
+    auto copy_codes = [&](uint32_t to, Place at) {
+        const bool own = at.slot < slots;
+        const Weight& w = own ? p.down : p.shared;
+        const size_t first = (size_t)(own ? picked.expert[at.slot] : 0) * w.strips;
+#pragma unroll
+        for (int m = 0; m < DOWN_MT; m++) copy16(to + m * 512 + lane * 16, w.codes + ((first + strips[m]) * w.blocks + at.b) * 32 + lane);
+        if (lane < DOWN_MT * 2 * NS) {
+            const int q = GROUP == 32 ? min(2 * at.b + (lane >> 1) % 2, w.qgroups - 1) : GROUP == 64 ? at.b : at.b >> 1;      // (a group beyond the last: its q are 0)
+            copy16(to + DOWN_MT * 512 + lane * 16, reinterpret_cast<const uint4*>(w.scales) + ((first + scale_strip) * w.qgroups + q) * 2 + (lane & 1));
+        }
+    };
+    auto copy_rows = [&](uint32_t to, Place at) {
+        const uint8_t* from = (at.slot < slots ? p.frag + (size_t)at.slot * nb * 2048 : p.sfrag) + (size_t)at.b * 2048 + lane * 16;
+#pragma unroll
+        for (int j = 0; j < 4; j++) copy16(to + D::X + j * 512 + lane * 16, from + j * 512);
+    };
+    Place now;
+    now.slot = min((lo + warp) / nb, slots), now.b = lo + warp - now.slot * nb;
+    Place ahead = now;
+    for (int i = 0; i < min(count, DOWN_DEPTH - 1); i++, ahead.next(slots, nb)) copy_codes(ring + i * D::SLOT, ahead);
+    // the slots' weights (an expert may be picked twice), under the first copies
+    for (int i = threadIdx.x; i < slots * FEW; i += DOWN_THREADS) {
+        const int e = picked.expert[i >> 3], c = i & 7;
+        float v = 0.f;
+        if ((picked.takes[i >> 3] >> c) & 1)
+            for (int j = c * p.top_k; j < (c + 1) * p.top_k; j++)
+                if (picked.pick[j] == e) v += wk[j];
+        wt[i >> 3][c] = v;
     }
-    __syncthreads();                                            // every stage has been copied and read: the sums lie over them
+    if (threadIdx.x < FEW) wt[slots][threadIdx.x] = (int)threadIdx.x < p.T && p.shared.codes ? gate : 0.f;
+    pdl_sync();
+    ahead = now;
+#pragma unroll 1
+    for (int i = 0; i < DOWN_DEPTH - 1; i++) {
+        if (i < count) copy_rows(ring + i * D::SLOT, ahead), ahead.next(slots, nb);
+        copy_commit();                                          // (the codes are part of the first group)
+    }
+    __syncthreads();
+
+    float acc[DOWN_MT][4] = {};
+    uint32_t at = ring, spare = ring + (DOWN_DEPTH - 1) * D::SLOT;
+    for (int i = 0; i < count; i++) {
+        if (i + DOWN_DEPTH - 1 < count) copy_codes(spare, ahead), copy_rows(spare, ahead), ahead.next(slots, nb);
+        copy_commit();
+        copy_wait<DOWN_DEPTH - 1>();
+        __syncwarp();                                           // (the scales were copied by other lanes)
+        float c[DOWN_MT][4], sum[DOWN_MT][4];
+        uint4 code[DOWN_MT];
+#pragma unroll
+        for (int m = 0; m < DOWN_MT; m++) code[m] = lds16(at + m * 512 + lane * 16);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const uint4 x = lds16(at + D::X + j * 512 + lane * 16);
+            const bool fresh = GROUP == 32 ? j % 2 == 0 : j == 0, last = GROUP == 32 ? j % 2 == 1 : j == 3;
+#pragma unroll
+            for (int m = 0; m < DOWN_MT; m++) {
+                uint32_t a[4];
+                q4::unpack(q4::word(code[m], j), p.bits, a);
+                if (fresh)
+                    q4::mma(c[m], a, x.x, x.y, 0.f, 0.f, 0.f, 0.f);
+                else
+                    q4::mma(c[m], a, x.x, x.y, c[m][0], c[m][1], c[m][2], c[m][3]);
+                q4::mma(c[m], a, x.z, x.w, c[m][0], c[m][1], c[m][2], c[m][3]);
+            }
+            if (last)
+#pragma unroll
+                for (int m = 0; m < DOWN_MT; m++) {
+                    const uint32_t sc = lds4(at + DOWN_MT * 512 + m * D::SCALES + (GROUP == 32 ? j / 2 * 32 : 0) + r * 4);
+                    const float l = q4::scale_lo(sc), h = q4::scale_hi(sc);
+                    const bool one = GROUP != 32 || j == 1;
+                    sum[m][0] = one ? l * c[m][0] : fmaf(l, c[m][0], sum[m][0]), sum[m][1] = one ? l * c[m][1] : fmaf(l, c[m][1], sum[m][1]);
+                    sum[m][2] = one ? h * c[m][2] : fmaf(h, c[m][2], sum[m][2]), sum[m][3] = one ? h * c[m][3] : fmaf(h, c[m][3], sum[m][3]);
+                }
+        }
+        const float2 w2 = *reinterpret_cast<const float2*>(&wt[now.slot][2 * t]);
+#pragma unroll
+        for (int m = 0; m < DOWN_MT; m++) {
+            acc[m][0] = fmaf(w2.x, sum[m][0], acc[m][0]), acc[m][1] = fmaf(w2.y, sum[m][1], acc[m][1]);
+            acc[m][2] = fmaf(w2.x, sum[m][2], acc[m][2]), acc[m][3] = fmaf(w2.y, sum[m][3], acc[m][3]);
+        }
+        __syncwarp();                                           // (all lanes have read the place)
+        now.next(slots, nb);
+        spare = at, at = at + D::SLOT == ring + DOWN_DEPTH * D::SLOT ? ring : at + D::SLOT;
+    }
+    __syncthreads();                                            // every ring has been copied and read: the sums lie over them
     float* red = reinterpret_cast<float*>(smem);
-    if (warp < DOWN_W)
 #pragma unroll
         for (int m = 0; m < DOWN_MT; m++) leave_sums<DOWN_MT>(red, warp, lane, m, acc[m]);
     __syncthreads();
@@ -715,7 +677,7 @@ experts_down_kernel(const __grid_constant__ DownArgs p) {
     float y = live ? sum_of<DOWN_W, DOWN_MT>(red, m, col, f) : 0.f;
     if (p.S > 1) {
         const uint32_t part = smem_u32(smem) + D::RED_FLOATS * 4;
-        cluster_sync_all();                                     // (the first block's stages are free)
+        cluster_sync_all();                                     // (the first block's rings are free)
         if (rank && live) st_cluster_f32(mapa_cluster(part + (rank * DOWN_MT * 128 + i) * 4, 0), y);
         cluster_sync_all();
         if (rank) return;
@@ -790,10 +752,10 @@ int run_experts(const Args& up, const DownArgs& down, cudaStream_t stream) {
     const long long units = slots * (up.w.strips / 2) + (up.shared.codes ? up.shared.strips / 2 : 0);
     int e = launch_stream<EXPERTS, 1, GROUP, true>(up, units, stream);
     if (e) return e;
-    e = (int)cudaFuncSetAttribute(experts_down_kernel<GROUP>, cudaFuncAttributeMaxDynamicSharedMemorySize, DownStage<GROUP>::BYTES);
+    e = (int)cudaFuncSetAttribute(experts_down_kernel<GROUP>, cudaFuncAttributeMaxDynamicSharedMemorySize, DownRing<GROUP>::BYTES);
     if (e) return e;
     return launch_pdl_cluster(experts_down_kernel<GROUP>, dim3((down.down.strips + DOWN_MT - 1) / DOWN_MT, 1, down.S), dim3(DOWN_THREADS),
-                              (size_t)DownStage<GROUP>::BYTES, stream, down.S, down);
+                              (size_t)DownRing<GROUP>::BYTES, stream, down.S, down);
 }
 
 uint32_t g_wait_limit = WAIT_LIMIT_US;
@@ -852,7 +814,7 @@ MOE_API int moe_experts_q4(const void* x, int ldx, int T, int H, const int* idx,
     if (shared > 0) up.shared = weight(sgu_codes, sgu_scales, 2 * shared, H, group, 1), d.shared = weight(sdown_codes, sdown_scales, H, shared, group, 0);
     const long long slots = (long long)T * top_k < E ? (long long)T * top_k : E;
     up.frag = (uint8_t*)scratch, up.frag_blocks = d.down.blocks, up.sfrag = up.frag + slots * d.down.blocks * 2048;
-    d.frag = up.frag, d.sfrag = up.sfrag, d.bits = up.bits, d.waits = up.waits;
+    d.frag = up.frag, d.sfrag = up.sfrag, d.bits = up.bits;
     d.T = T, d.H = H, d.E = E, d.top_k = top_k, d.idx = idx, d.wk = wk, d.gate = gate, d.out = out, d.out_bf16 = out_bf16, d.ldo = ldo;
     d.S = max(1, min(8, sm_count() / ((d.down.strips + DOWN_MT - 1) / DOWN_MT)));      // one block an SM
 #define GO(GR) run_experts<GR>(up, d, stream)

@@ -194,7 +194,6 @@ WAIT_SITES = {
     0x10: "tensor-core product, one CTA a tile", 0x20: "tensor-core product, persistent",
     0x30: "tensor-core product, pairs of CTAs", 0x40: "tensor-core prompt attention",
     0x50: "tensor-core product over 4-bit weights", 0x60: "product of few rows over 4-bit weights",
-    0x70: "experts' down product over 4-bit weights",
 }
 WAIT_ROLES = {
     0x1: "producer: a free stage", 0x2: "producer: its own copies in flight", 0x3: "MMA issuer: a free accumulator",
