@@ -1,20 +1,23 @@
 // Products of many rows over weights held in 4 bits (the format: quant4.cuh), on the 5th-generation tensor cores.
 //
-// The weight is the MMA's A operand and is read from TENSOR MEMORY: a warp takes the codes of a strip (16 features x 64 k) as they lie in
-// global memory, forms the bfloat16 values q s (exact) in registers and hands them over with tcgen05.st.16x256b, whose register layout is that
-// of the codes.  Nothing of a weight passes through shared memory, which carries the activations alone (TMA, 128-byte swizzle): with A
-// in shared memory too it is what bounds a tile of one SM.  128 features x up to 192 rows a tile; two accumulators (2 x 192 columns) and
-// four stages of A (4 x 32 columns) fill the 512 columns, so the epilogue of a tile runs under the next one's products.
+// The weight is the MMA's A operand: a warp takes the codes of a strip (16 features x 64 k) as they lie in global memory, forms the bfloat16
+// values q s (exact) in registers and writes them to the stage's A tile in shared memory (128 rows of 128 bytes, the swizzle that TMA would have
+// given them; odd rows write their 16-byte pieces in another order, so that no two lanes meet in a bank).  The rows of x come by TMA.  128 features x up to
+// 256 rows a tile, two accumulators (all 512 columns of tensor memory), so the epilogue of a tile runs under the next one's products.
 //
-//   warps 0-7    two groups of four: the codes of every other block of 64 k to values in tensor memory, PREFETCH blocks ahead in registers
-//   warps 8-15   epilogue: accumulator -> registers -> global memory (warp w: lanes 32 (w % 4).., half of the tile's rows)
-//   warp 16      TMA producer of the rows of x, STAGES tiles of [rows x 64]
-//   warp 17      allocates tensor memory and issues the products
+//   teams of four warps   the codes of every TEAMS-th block of 64 k to values, PREFETCH blocks ahead in registers
+//   8 warps               epilogue: accumulator -> registers -> global memory (warp w: lanes 32 (w % 4).., half of the tile's rows)
+//   1 warp                TMA producer of the rows of x
+//   1 warp                allocates tensor memory and issues the products
 //
-// One CTA an SM walks over the tiles.  A gated pair's tile holds 64 features: gate strips in lanes 32 i.., up strips in lanes 32 i + 16.. .
+// What bounds a tile is shared memory's 128 bytes a cycle: 16 k of A are written and read (64 cycles), of N rows too (N / 2), against N / 2 cycles of the
+// tensor core.  (With the values in tensor memory instead, tcgen05.st in the codes' own layout, a product took 128 cycles whatever N, to load A, and
+// 190 beside the stores: 2,048 rows of a pair 11,264 x 2,048 113 us, 8,192 rows of 2,048 x 5,632 240 us.)
+//
+// One CTA an SM walks over the tiles.  A gated pair's tile holds 64 features: gate strips in rows 32 i.., up strips in rows 32 i + 16.. .
 // Groups (routed experts): rows [offsets[g], offsets[g + 1]) meet the weights of g.  Where a dense product has too few tiles for the
-// SMs, up to 8 CTAs of a cluster share a tile's k; each leaves its rows of the partial sums in their owners' shared memory and the owner
-// adds them up in the order of the splits.
+// SMs, up to 8 CTAs of a cluster share a tile's k; each leaves its partial sums in its shared memory, and each adds up an equal share of the rows in
+// the order of the splits.
 //
 // Every wait on a barrier is bounded; one that runs out sets ST_WAIT_TIMEOUT, the roles drain and the CTA frees its tensor memory.
 #include <cuda.h>
@@ -27,11 +30,11 @@ namespace {
 
 using q4::Weight;
 
-constexpr int FEATURES = 128, BK = 64, BN = 192, STAGES = 8, A_STAGES = 4, A_COLS = 32, NBUF = 2, PREFETCH = 3;
-constexpr int STAGE_BYTES = BN * BK * 2, SMEM = STAGES * STAGE_BYTES + 1024 + 256;
-constexpr int A_COL0 = NBUF * BN, TMEM_COLS = 512, MAX_GROUPS = 1024, MAX_CLUSTER = 8;
-constexpr int DEQUANT_WARPS = 8, EPI_WARPS = 8, WARPS = DEQUANT_WARPS + EPI_WARPS + 2, THREADS = WARPS * 32;
-static_assert(A_COL0 + A_STAGES * A_COLS <= TMEM_COLS, "tensor memory");
+constexpr int FEATURES = 128, BK = 64, BN = 256, NBUF = 2, PREFETCH = 2, STAGES_MAX = 8;
+constexpr int A_BYTES = FEATURES * BK * 2, BOX = 64, BOX_BYTES = BOX * BK * 2, ROOM = 200 * 1024;      // ROOM: bytes for stages
+constexpr int TMEM_COLS = 512, MAX_GROUPS = 1024, MAX_CLUSTER = 8;
+constexpr int TEAMS = 2, DEQUANT_WARPS = 4 * TEAMS, EPI_WARPS = 8, WARPS = DEQUANT_WARPS + EPI_WARPS + 2, THREADS = WARPS * 32;
+static_assert(NBUF * BN <= TMEM_COLS, "tensor memory");
 
 struct Args {
     Weight w;
@@ -41,6 +44,7 @@ struct Args {
     const int* offsets;
     int G, M, N;                   // N: output features
     int bn;                        // rows of a tile, a multiple of 16
+    int stages, stage_bytes;       // A tile and boxes of 64 rows
     int n_tiles;                   // tiles of features
     int splits, kb_per_split;
     int act;
@@ -64,11 +68,16 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map
                  "r"(bar)
                  : "memory");
 }
+__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    return v;
+}
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-// D[128, N] (+)= A[128, 16] B[N, 16]^T, A in tensor memory (a lane a row, two k a column), B in shared memory
-__device__ __forceinline__ void umma(uint32_t d, uint32_t a, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b_desc), "r"(idesc),
+// D[128, N] (+)= A[128, 16] B[N, 16]^T, both in shared memory
+__device__ __forceinline__ void umma(uint32_t d, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a_desc), "l"(b_desc), "r"(idesc),
                  "r"(accumulate)
                  : "memory");
 }
@@ -85,13 +94,6 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[16]) {
 #pragma unroll
     for (int i = 0; i < 16; i++) v[i] = __uint_as_float(r[i]);
 }
-// 16 rows x 64 k of bfloat16: of each 16 k, registers 0 and 1 hold row lane / 4 at k 4 (lane % 4)..., registers 2 and 3 row lane / 4 + 8
-__device__ __forceinline__ void tmem_st_strip(uint32_t taddr, const uint32_t (&r)[16]) {
-    asm volatile("tcgen05.st.sync.aligned.16x256b.x4.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
-                 "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-                 : "memory");
-}
-__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // K-major tile with 128-byte swizzle: rows of 128 bytes, groups of 8 rows 1024 bytes apart
 __device__ __forceinline__ uint64_t smem_desc(uint32_t addr) {
     return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
@@ -126,6 +128,52 @@ __device__ __forceinline__ void put(const Args& p, int row, int n, float v) {
         ((float*)p.out)[(size_t)row * p.ldo + n] = v;
 }
 
+// silu(g) u by the quick exponential and quotient (2 ulp each, on 32-bit sums): the exact ones made the epilogue as long as a tile's products
+__device__ __forceinline__ float gated(const Args& p, float g, float u) {
+    if (p.act == ACT_SILU) return __fdividef(g, 1.f + __expf(-g)) * u;
+    return glu_mul(p.act, p.act_param, g, u);
+}
+
+// Rows [lo, hi) of a finished tile by one warp: lanes 32 q.. of the accumulator at taddr
+template <bool PAIR, typename T>
+__device__ __forceinline__ void store_part(const Args& p, T* out, const Tile& t, uint32_t taddr, int q, int lane, int lo, int hi) {
+    const bool upper = PAIR && (lane & 16);
+    const int n = PAIR ? t.ft * 64 + q * 16 + (lane & 15) : t.ft * FEATURES + q * 32 + lane;
+    const float bias = !PAIR && p.bias && n < p.N ? p.bias[n] : 0.f;
+    const bool live = n < p.N;
+    T* o = out + (size_t)(t.row0 + lo) * p.ldo + n;
+    for (int c0 = lo; c0 < hi; c0 += 16) {
+        float a[16];
+        __syncwarp();
+        tmem_ld16(taddr + c0, a);
+        if constexpr (PAIR) {
+            // lanes 0-15 hold gate, 16-31 up: of each two rows, the lower half takes the first and the upper half the second
+            float y[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const float recv = __shfl_xor_sync(0xffffffffu, upper ? a[2 * j] : a[2 * j + 1], 16);
+                y[j] = gated(p, upper ? recv : a[2 * j], upper ? a[2 * j + 1] : recv);
+            }
+            T* r = upper ? o + p.ldo : o;
+            const int left = hi - c0 - (upper ? 1 : 0);
+            if (live)
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+                    if (2 * j < left) st_f(r + (size_t)(2 * j) * p.ldo, y[j]);
+        } else if (live) {
+            if (p.act == ACT_SILU) {                     // (no activation)
+#pragma unroll
+                for (int j = 0; j < 16; j++)
+                    if (c0 + j < hi) st_f(o + (size_t)j * p.ldo, a[j] + bias);
+            } else
+#pragma unroll
+                for (int j = 0; j < 16; j++)
+                    if (c0 + j < hi) st_f(o + (size_t)j * p.ldo, plain_act(p.act, a[j] + bias));
+        }
+        o += (size_t)16 * p.ldo;
+    }
+}
+
 template <int GROUP, bool PAIR>
 __global__ void __launch_bounds__(THREADS, 1)
 gemm_q4_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ Args p) {
@@ -134,18 +182,16 @@ gemm_q4_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant
     __shared__ uint32_t s_tmem;
     __shared__ int s_offs[MAX_GROUPS + 1], s_prefix[MAX_GROUPS + 1];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u, bars = base + STAGES * STAGE_BYTES;
-    auto b_full = [&](int s) { return bars + 8u * s; };
-    auto b_empty = [&](int s) { return bars + 8u * (STAGES + s); };
-    auto a_full = [&](int s) { return bars + 8u * (2 * STAGES + s); };
-    auto a_empty = [&](int s) { return bars + 8u * (2 * STAGES + A_STAGES + s); };
-    auto acc_full = [&](int b) { return bars + 8u * (2 * STAGES + 2 * A_STAGES + b); };
-    auto acc_empty = [&](int b) { return bars + 8u * (2 * STAGES + 2 * A_STAGES + NBUF + b); };
-    const uint32_t drained = bars + 8u * (2 * STAGES + 2 * A_STAGES + 2 * NBUF);
+    __shared__ __align__(8) unsigned long long s_bars[2 * STAGES_MAX + 2 * NBUF + 1];
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u, bars = smem_u32(s_bars);
+    auto full = [&](int s) { return bars + 8u * s; };
+    auto empty = [&](int s) { return bars + 8u * (STAGES_MAX + s); };
+    auto acc_full = [&](int b) { return bars + 8u * (2 * STAGES_MAX + b); };
+    auto acc_empty = [&](int b) { return bars + 8u * (2 * STAGES_MAX + NBUF + b); };
+    const uint32_t drained = bars + 8u * (2 * STAGES_MAX + 2 * NBUF);
     if (threadIdx.x == 0) {
         s_abort = 0;
-        for (int s = 0; s < STAGES; s++) mbar_init(b_full(s), 1), mbar_init(b_empty(s), 1);
-        for (int s = 0; s < A_STAGES; s++) mbar_init(a_full(s), 4), mbar_init(a_empty(s), 1);
+        for (int s = 0; s < p.stages; s++) mbar_init(full(s), 1 + 4), mbar_init(empty(s), 1);      // the copies of x, and four warps of values
         for (int b = 0; b < NBUF; b++) mbar_init(acc_full(b), 1), mbar_init(acc_empty(b), EPI_WARPS);
         mbar_init(drained, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -186,69 +232,80 @@ gemm_q4_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant
     const int total = mine * kbs;
 
     if (warp < DEQUANT_WARPS) {
-        // ---- codes to values: block `it` of the CTA's sequence by the warps of group it % 2 --------------------------------------------
-        const int q = warp & 3, r = lane >> 2;
+        // ---- codes to values: block `it` of the CTA's sequence by the warps of team it % TEAMS -----------------------------------------
+        const int q = warp & 3, r = lane >> 2, half = PAIR ? p.w.strips / 2 : p.w.strips;
         uint4 code[PREFETCH][2];
         q4::Scales<GROUP> sc[PREFETCH][2];
-        int next = warp >> 2, next_item = -1;
-        Tile t;
-        auto load = [&](int d) {                         // the block `next` into place d
-            if (next < total) {
-                const int li = next / kbs, kb = kb0 + next - li * kbs;
-                if (li != next_item) t = tile_of(blockIdx.x + li * gridDim.x, m_tiles, p, s_prefix, s_offs), next_item = li;
-                const int half = PAIR ? p.w.strips / 2 : p.w.strips;
+        int li = 0, kb = warp >> 2;                      // the next block to ask for: tile of this CTA, block of its k
+        const uint4* nc[2];
+        const uint32_t* ns[2];
+        auto aim = [&]() {
+            while (kb >= kbs && li < mine) kb -= kbs, li++;
+            if (li >= mine) return;
+            const Tile t = tile_of(blockIdx.x + li * gridDim.x, m_tiles, p, s_prefix, s_offs);
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const int strip = PAIR ? t.ft * 4 + q : t.ft * 8 + 2 * q + i;
+                // (strips beyond the last: any values will do, their features are not stored)
+                const size_t s = (size_t)t.g * p.w.strips + min(strip, half - 1) + (PAIR && i ? half : 0);
+                nc[i] = p.w.codes + (s * p.w.blocks + kb0 + kb) * 32 + lane;
+                ns[i] = p.w.scales + s * p.w.qgroups * 8;
+            }
+        };
+        aim();
+        auto load = [&](int d) {                         // that block into place d
+            if (li < mine) {
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
-                    const int strip = PAIR ? t.ft * 4 + q : t.ft * 8 + 2 * q + i;
-                    if (strip < half) {
-                        const size_t s = (size_t)t.g * p.w.strips + strip + (PAIR && i ? half : 0);
-                        code[d][i] = __ldg(p.w.codes + (s * p.w.blocks + kb) * 32 + lane);
-                        sc[d][i].load(p.w.scales + s * p.w.qgroups * 8, kb, p.w.qgroups, r);
-                    } else {
-                        code[d][i] = make_uint4(0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u);
-                        sc[d][i] = q4::Scales<GROUP>{};
-                    }
+                    code[d][i] = __ldg(nc[i]);
+                    sc[d][i].load(ns[i], kb0 + kb, p.w.qgroups, r);
+                    nc[i] += TEAMS * 32;
                 }
+                kb += TEAMS;
+                if (kb >= kbs) aim();
             }
-            next += 2;
         };
 #pragma unroll
         for (int d = 0; d < PREFETCH; d++) load(d);
         bool ok = p.test_fault != 3;
-        for (int it0 = warp >> 2; it0 < total && ok; it0 += 2 * PREFETCH) {
+        // this lane's place in the A tile: rows 32 q + r (and 8, 16, 24 further on), the piece of four k at 4 t of the first 16 k (odd rows: the third)
+        const bool odd = r & 1;
+        const uint32_t place = (uint32_t)((32 * q + r) * 128 + ((((lane & 3) >> 1) ^ r ^ (odd ? 4 : 0)) << 4) + (lane & 1) * 8);
+        int s = (warp >> 2) % p.stages;
+        uint32_t parity = 1;
+        for (int it0 = warp >> 2; it0 < total && ok; it0 += TEAMS * PREFETCH) {
 #pragma unroll
             for (int d = 0; d < PREFETCH; d++) {
-                const int it = it0 + 2 * d;
+                const int it = it0 + TEAMS * d;
                 if (it >= total || !ok) break;
-                const int s = it % A_STAGES;
-                uint32_t v[2][16];
+                ok = __all_sync(0xffffffffu, mbar_wait(empty(s), parity, &s_abort, p, 0x56));
+                if (!ok) break;
+                const uint32_t to = base + s * p.stage_bytes + place;
 #pragma unroll
-                for (int i = 0; i < 2; i++)
+                for (int i = 0; i < 2; i++) {
 #pragma unroll
-                    for (int j = 0; j < 4; j++) {
+                    for (int j = 0; j < 4; j++) {        // odd rows take the 16 k in the order 2, 3, 0, 1
                         uint32_t a[4];
-                        q4::unpack(q4::word(code[d][i], j), p.bits, a);
-                        const uint32_t s2 = sc[d][i].s[GROUP == 32 ? j / 2 : 0];
+                        q4::unpack(odd ? q4::word(code[d][i], j ^ 2) : q4::word(code[d][i], j), p.bits, a);
+                        const uint32_t s2 = GROUP == 32 ? (odd != (j >= 2) ? sc[d][i].s[q4::Scales<GROUP>::N - 1] : sc[d][i].s[0]) : sc[d][i].s[0];
                         const uint32_t lo2 = __byte_perm(s2, 0, 0x1010), hi2 = __byte_perm(s2, 0, 0x3232);
+                        uint32_t v[4];
 #pragma unroll
-                        for (int e = 0; e < 4; e++) {      // registers of the fragment: rows r, r + 8, r, r + 8; of the store: r, r, r + 8, r + 8
+                        for (int e = 0; e < 4; e++) {      // rows r, r + 8, r, r + 8
                             const uint32_t m = (e & 1) ? hi2 : lo2;
                             const __nv_bfloat162 y = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&a[e]), *reinterpret_cast<const __nv_bfloat162*>(&m));
-                            v[i][4 * j + 2 * (e & 1) + (e >> 1)] = *reinterpret_cast<const uint32_t*>(&y);
+                            v[e] = *reinterpret_cast<const uint32_t*>(&y);
                         }
+                        q4::sts8((to ^ (j << 5)) + i * 2048, make_uint2(v[0], v[2]));
+                        q4::sts8((to ^ (j << 5)) + i * 2048 + 1024, make_uint2(v[1], v[3]));
                     }
-                ok = mbar_wait(a_empty(s), ((it / A_STAGES) & 1) ^ 1, &s_abort, p, 0x56);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                tc_fence_after();
-                const uint32_t at = tmem + A_COL0 + s * A_COLS + ((uint32_t)(q * 32) << 16);
-                tmem_st_strip(at, v[0]);
-                tmem_st_strip(at + (16u << 16), v[1]);
+                }
                 load(d);
-                tmem_st_wait();
-                tc_fence_before();
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // the tensor core reads what was written
                 __syncwarp();
-                if (lane == 0) mbar_arrive(a_full(s));
+                if (lane == 0) mbar_arrive(full(s));
+                s += TEAMS;
+                if (s >= p.stages) s -= p.stages, parity ^= 1;
             }
         }
         if (!ok && p.test_fault != 3) s_abort = 1;
@@ -265,28 +322,11 @@ gemm_q4_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant
                 if (!ok) break;
                 tc_fence_after();
                 const uint32_t taddr = tmem + b * BN + ((uint32_t)(q * 32) << 16);
-                const bool upper = PAIR && (lane & 16);
-                const int n = PAIR ? t.ft * 64 + q * 16 + (lane & 15) : t.ft * FEATURES + q * 32 + lane;
-                const float bias = !PAIR && p.bias && n < p.N ? p.bias[n] : 0.f;
-                const int part = ((t.rows + 31) / 32) * 16, lo = h * part, hi = min(t.rows, lo + part);
-                for (int c0 = lo; c0 < hi; c0 += 16) {
-                    float a[16];
-                    __syncwarp();
-                    tmem_ld16(taddr + c0, a);
-                    if (PAIR) {
-#pragma unroll
-                        for (int j = 0; j < 16; j += 2) {
-                            const float recv = __shfl_xor_sync(0xffffffffu, upper ? a[j] : a[j + 1], 16);
-                            const float g = upper ? recv : a[j], u = upper ? a[j + 1] : recv;
-                            const int c = c0 + j + (upper ? 1 : 0);
-                            if (c < hi && n < p.N) put(p, t.row0 + c, n, glu_mul(p.act, p.act_param, g, u));
-                        }
-                    } else if (n < p.N) {
-#pragma unroll
-                        for (int j = 0; j < 16; j++)
-                            if (c0 + j < hi) put(p, t.row0 + c0 + j, n, plain_act(p.act, a[j] + bias));
-                    }
-                }
+                const int part = ((t.rows + 31) / 32) * 16, lo = min(t.rows, h * part), hi = min(t.rows, lo + part);
+                if (p.out_bf16)
+                    store_part<PAIR>(p, (__nv_bfloat16*)p.out, t, taddr, q, lane, lo, hi);
+                else
+                    store_part<PAIR>(p, (float*)p.out, t, taddr, q, lane, lo, hi);
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(acc_empty(b));
@@ -297,28 +337,33 @@ gemm_q4_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant
         // ---- rows of x -------------------------------------------------------------------------------------------------------------------
         if (lane == 0) {
             if (!p.offsets) pdl_sync();
-            int it = 0;
+            int it = 0, s = 0;
+            uint32_t parity = 1;
             bool ok = p.test_fault != 1;
             for (int li = 0; li < mine && ok; li++) {
                 const Tile t = tile_of(blockIdx.x + li * gridDim.x, m_tiles, p, s_prefix, s_offs);
-                const int boxes = (t.rows + 63) / 64;
+                const int boxes = (t.rows + BOX - 1) / BOX;
                 for (int kb = 0; kb < kbs; kb++, it++) {
-                    const int s = it % STAGES;
-                    ok = mbar_wait(b_empty(s), ((it / STAGES) & 1) ^ 1, &s_abort, p, 0x51);
+                    ok = mbar_wait(empty(s), parity, &s_abort, p, 0x51);
                     if (!ok) break;
-                    mbar_expect_tx(b_full(s), boxes * 64 * BK * 2);
-                    for (int c = 0; c < boxes; c++) tma_load_2d(base + s * STAGE_BYTES + c * 64 * BK * 2, &tmX, (kb0 + kb) * BK, t.row0 + c * 64, b_full(s));
+                    mbar_expect_tx(full(s), boxes * BOX_BYTES);
+                    for (int c = 0; c < boxes; c++) tma_load_2d(base + s * p.stage_bytes + A_BYTES + c * BOX_BYTES, &tmX, (kb0 + kb) * BK, t.row0 + c * BOX, full(s));
+                    if (++s == p.stages) s = 0, parity ^= 1;
                 }
             }
             if (!ok && p.test_fault != 1) {
                 s_abort = 1;
-                for (int i = max(0, it - STAGES); i < it; i++) mbar_wait(b_full(i % STAGES), (i / STAGES) & 1, nullptr, p, 0x52);      // copies in flight must land
+                // copies in flight must land: with the values never coming, the stages' barriers would not say so
+                for (int i = max(0, it - p.stages); i < it; i++)
+                    for (int w = 0; w < 4; w++) mbar_arrive(full(i % p.stages));
+                for (int i = max(0, it - p.stages); i < it; i++) mbar_wait(full(i % p.stages), (i / p.stages) & 1, nullptr, p, 0x52);
             }
         }
     } else {
         // ---- products --------------------------------------------------------------------------------------------------------------------
         if (lane == 0) {
-            int it = 0;
+            int s = 0;
+            uint32_t parity = 0;
             bool ok = p.test_fault != 2;
             for (int li = 0; li < mine && ok; li++) {
                 const Tile t = tile_of(blockIdx.x + li * gridDim.x, m_tiles, p, s_prefix, s_offs);
@@ -326,16 +371,16 @@ gemm_q4_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant
                 const int b = li % NBUF;
                 ok = mbar_wait(acc_empty(b), ((li / NBUF) & 1) ^ 1, &s_abort, p, 0x53);
                 if (!ok) break;
-                for (int kb = 0; kb < kbs; kb++, it++) {
-                    const int s = it % STAGES, a = it % A_STAGES;
-                    ok = mbar_wait(b_full(s), (it / STAGES) & 1, &s_abort, p, 0x54) && mbar_wait(a_full(a), (it / A_STAGES) & 1, &s_abort, p, 0x57);
+                for (int kb = 0; kb < kbs; kb++) {
+                    ok = mbar_wait(full(s), parity, &s_abort, p, 0x54);
                     if (!ok) break;
                     tc_fence_after();
+                    const uint32_t st = base + s * p.stage_bytes;
 #pragma unroll
                     for (int k4 = 0; k4 < BK / 16; k4++)
-                        umma(tmem + b * BN, tmem + A_COL0 + a * A_COLS + k4 * 8, smem_desc(base + s * STAGE_BYTES + k4 * 32), idesc, kb > 0 || k4 > 0);
-                    umma_commit(b_empty(s));
-                    umma_commit(a_empty(a));
+                        umma(tmem + b * BN, smem_desc(st + k4 * 32), smem_desc(st + A_BYTES + k4 * 32), idesc, kb > 0 || k4 > 0);
+                    umma_commit(empty(s));
+                    if (++s == p.stages) s = 0, parity ^= 1;
                 }
                 if (ok) umma_commit(acc_full(b));
             }
@@ -350,41 +395,49 @@ gemm_q4_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant
         tc_fence_before();
         __syncthreads();
         tc_fence_after();
-        cluster_sync_all();                              // every CTA's products are done: the stages are free to receive
         const Tile t = tile_of(blockIdx.x, m_tiles, p, s_prefix, s_offs);
         const int S = p.splits, cpo = (t.rows + S - 1) / S;
-        const bool fine = !s_abort;
-        if (warp >= DEQUANT_WARPS && warp < DEQUANT_WARPS + EPI_WARPS && fine) {
+        if (warp >= DEQUANT_WARPS && warp < DEQUANT_WARPS + EPI_WARPS) {      // the stages are free: the partial tile, [row][128 features]
             const int q = warp & 3, h = (warp - DEQUANT_WARPS) >> 2;
             const uint32_t taddr = tmem + ((uint32_t)(q * 32) << 16);
-            const int part = ((t.rows + 31) / 32) * 16, lo = h * part, hi = min(t.rows, lo + part);
+            const int part = ((t.rows + 31) / 32) * 16, lo = min(t.rows, h * part), hi = min(t.rows, lo + part);
             for (int c0 = lo; c0 < hi; c0 += 16) {
                 float a[16];
                 __syncwarp();
                 tmem_ld16(taddr + c0, a);
+                const uint32_t to = base + (uint32_t)(c0 * FEATURES + q * 32 + lane) * 4u;
 #pragma unroll
-                for (int j = 0; j < 16; j++) {
-                    const int c = c0 + j, owner = c / cpo;
-                    if (c < hi) st_cluster_f32(mapa_cluster(base + (uint32_t)((rank * cpo + c - owner * cpo) * FEATURES + q * 32 + lane) * 4u, owner), a[j]);
-                }
+                for (int j = 0; j < 16; j++) asm volatile("st.shared.f32 [%0], %1;" ::"r"(to + j * FEATURES * 4), "f"(a[j]) : "memory");
             }
         }
         __syncwarp();
         cluster_sync_all();
-        const float* recv = reinterpret_cast<const float*>(smem_raw + (base - smem_u32(smem_raw)));
-        const int first = rank * cpo, cols = min(cpo, t.rows - first), per = PAIR ? 64 : FEATURES;
-        for (int i = threadIdx.x; i < cols * per && fine; i += THREADS) {
-            const int c = i / per, f = i - c * per, n = t.ft * per + f;
-            if (n >= p.N) continue;
-            const int l = PAIR ? (f >> 4) * 32 + (f & 15) : f;
-            float a = 0.f, b = 0.f;
-            for (int s = 0; s < S; s++) {
-                a += recv[(s * cpo + c) * FEATURES + l];
-                if (PAIR) b += recv[(s * cpo + c) * FEATURES + l + 16];
-            }
-            const float v = PAIR ? glu_mul(p.act, p.act_param, a, b) : plain_act(p.act, p.bias ? a + p.bias[n] : a);
-            put(p, t.row0 + first + c, n, v);
+        // four features a thread: one 16-byte read of every peer's memory
+        const int first = rank * cpo, cols = min(cpo, t.rows - first), per = PAIR ? 16 : FEATURES / 4;
+        for (int i = threadIdx.x; i < cols * per; i += THREADS) {
+            const int c = i / per, f = (i - c * per) * 4, n = t.ft * per * 4 + f;
+            const uint32_t at = base + (uint32_t)((first + c) * FEATURES + (PAIR ? (f >> 4) * 32 + (f & 15) : f)) * 4u;
+            float4 v[MAX_CLUSTER], w[PAIR ? MAX_CLUSTER : 1];
+#pragma unroll
+            for (int s = 0; s < MAX_CLUSTER; s++)
+                if (s < S) {
+                    const uint32_t peer = mapa_cluster(at, s);
+                    v[s] = ld_cluster_f32x4(peer);
+                    if constexpr (PAIR) w[s] = ld_cluster_f32x4(peer + 64);
+                }
+            float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
+#pragma unroll
+            for (int s = 0; s < MAX_CLUSTER; s++)
+                if (s < S) {
+                    x.x += v[s].x, x.y += v[s].y, x.z += v[s].z, x.w += v[s].w;
+                    if constexpr (PAIR) y.x += w[s].x, y.y += w[s].y, y.z += w[s].z, y.w += w[s].w;
+                }
+            const float xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (n + e < p.N) put(p, t.row0 + first + c, n + e, PAIR ? gated(p, xs[e], ys[e]) : plain_act(p.act, p.bias ? xs[e] + p.bias[n + e] : xs[e]));
         }
+        cluster_sync_all();                              // nobody leaves while its memory is read
     }
     tc_fence_before();
     __syncthreads();
@@ -412,9 +465,9 @@ int g_test_fault = 0;
 template <int GROUP, bool PAIR>
 int launch(const CUtensorMap& map, const Args& p, unsigned ctas, cudaStream_t stream) {
     // (the attribute belongs to a device's copy of the kernel: set per launch it costs a fraction of a microsecond and is right on every device)
-    const cudaError_t e = cudaFuncSetAttribute(gemm_q4_tc_kernel<GROUP, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+    const cudaError_t e = cudaFuncSetAttribute(gemm_q4_tc_kernel<GROUP, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, p.stages * p.stage_bytes + 1024);
     if (e != cudaSuccess) return (int)e;
-    return launch_pdl_cluster(gemm_q4_tc_kernel<GROUP, PAIR>, dim3(ctas, 1, p.splits), dim3(THREADS), (size_t)SMEM, stream, p.splits, map, p);
+    return launch_pdl_cluster(gemm_q4_tc_kernel<GROUP, PAIR>, dim3(ctas, 1, p.splits), dim3(THREADS), (size_t)(p.stages * p.stage_bytes + 1024), stream, p.splits, map, p);
 }
 
 }  // namespace
@@ -439,14 +492,18 @@ MOE_API int moe_gemm_q4_tc(const void* x, int ldx, int M, const void* codes, con
     p.out = out, p.out_bf16 = out_bf16, p.ldo = ldo, p.bias = bias, p.offsets = offsets, p.G = G, p.M = M;
     p.act = act, p.act_param = act_param, p.status = status, p.wait_limit = g_wait_limit, p.test_fault = g_test_fault, p.bits = q4::bits();
     p.n_tiles = pair ? (p.N + 63) / 64 : (p.N + FEATURES - 1) / FEATURES;
-    // rows of a tile: as few tiles as 192 rows allow, of equal height
+    // Rows of a tile: as few tiles as 256 rows allow, of equal height.  Groups: what holds a group of half as many rows again as the mean (a smaller tile
+    // leaves room for more stages, and the copies' latency counts).
+    const int mean = (M + G - 1) / G;
     const int mt = (M + BN - 1) / BN;
-    p.bn = offsets ? BN : ((M + mt - 1) / mt + 15) / 16 * 16;
+    p.bn = offsets ? min(BN, (mean * 3 / 2 + BOX - 1) / BOX * BOX) : ((M + mt - 1) / mt + 15) / 16 * 16;
+    p.stage_bytes = A_BYTES + (p.bn + BOX - 1) / BOX * BOX_BYTES;
+    p.stages = min(STAGES_MAX, ROOM / p.stage_bytes);
     int dev = 0, sms = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
     if (e != cudaSuccess) return (int)e;
-    const long long tiles = (offsets ? (long long)(M < G ? M : G) + M / BN : (long long)((M + p.bn - 1) / p.bn)) * p.n_tiles;
+    const long long tiles = (offsets ? (long long)(M < G ? M : G) + M / p.bn : (long long)((M + p.bn - 1) / p.bn)) * p.n_tiles;
     if (tiles > 0x3fffffff) return -1;
     if (offsets || splits < 1) splits = 1;
     if (splits > MAX_CLUSTER) splits = MAX_CLUSTER;

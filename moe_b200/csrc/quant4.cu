@@ -1,13 +1,14 @@
 // Weights to 4 bits and back (the format: quant4.cuh).
 //
 //   s = max |w| over the group / 7, rounded to five significant bits (nearest, ties to even); q = w / s rounded (ties to even).
-// s may be rounded down by 1 / 33 of itself at most, so |w| / s <= 7 (1 + 1 / 32) < 7.5 and q needs no clamp.  Decisions at a border are
-// exact: the quotient max / 7 is formed in 64 bits (of a 24-bit number: never nearer to a border of five bits than 2^-27 of itself unless on
-// it), and w - q s, which 32 bits hold exactly, says which side of half a step w lies on.  A group whose maximum is below 7 * 2^-126 is
+// s may be rounded down by 1 / 33 of itself at most, so |w| / s <= 7 (1 + 1 / 32) < 7.5 and q needs no clamp.  Decisions at a border are exact.  For
+// bfloat16: max / 7 and w / s as correctly rounded 32-bit quotients, which are a border (five bits; half a step) only where the exact quotient
+// is, its operands having eight and five bits.  For float32: max / 7 in 64 bits (of a 24-bit number: never nearer to a border of five bits than 2^-27 of itself
+// unless on it), and w - q s, which 32 bits hold exactly, says which side of half a step w lies on.  A group whose maximum is below 7 * 2^-126 is
 // held as zeros; one that holds an infinity or a NaN gets the scale NaN, so that products of it are NaN, and sets ST_NOT_FINITE.
 //
-// Both directions are bound by DRAM: a warp takes one strip (16 rows) x 64 k (128 where a group is 128), 8 bytes a load of bfloat16, four
-// lanes a 32-byte sector.
+// A warp takes one strip (16 rows) x 64 k (128 where a group is 128), 8 bytes a load of bfloat16, four
+// lanes a 32-byte sector.  DRAM should bound both directions; what does is the issue of about a dozen instructions an element.
 #include "quant4.cuh"
 
 namespace {
@@ -30,9 +31,15 @@ __device__ __forceinline__ void load4(const T* row, int k, int K, bool vec, floa
 }
 
 // max / 7 to five significant bits; 0 for what is held as zeros, NaN for what is no number
+template <typename T>
 __device__ __forceinline__ float scale_of(float amax) {
     if (!(amax <= 3.402823466e38f)) return __uint_as_float(0x7fc00000u);
     if (amax < 0x1.cp-124f) return 0.f;                                   // 7 * 2^-126
+    if constexpr (sizeof(T) == 2) {
+        uint32_t u = __float_as_uint(__fdiv_rn(amax, 7.f));
+        u += (1u << 18) - 1 + ((u >> 19) & 1);                            // 23 - 4 bits go
+        return __uint_as_float(u & ~((1u << 19) - 1));
+    }
     const double d = (double)amax / 7.0;
     unsigned long long u = (unsigned long long)__double_as_longlong(d);
     u += (1ull << 47) - 1 + ((u >> 48) & 1);                              // 52 - 4 bits go
@@ -40,12 +47,17 @@ __device__ __forceinline__ float scale_of(float amax) {
     return (float)__longlong_as_double((long long)u);
 }
 
-// w / s to the nearest whole number, ties to even
-__device__ __forceinline__ int code_of(float w, float s, float rs) {
+// w / s to the nearest whole number, ties to even, plus 8, in the low four bits
+template <typename T>
+__device__ __forceinline__ uint32_t code_of(float w, float s, float rs) {
+    if constexpr (sizeof(T) == 2) {
+        const float v = w * rs;
+        return __float_as_uint(fmaf(fmaf(-v, s, w), rs, v) + 12582920.f);      // the correctly rounded quotient; 1.5 * 2^23 + 8
+    }
     float q = rintf(w * rs);
     const float r = fmaf(-q, s, w), h = 0.5f * s, a = fabsf(r);           // exact: q s has eight bits and lies within a step of w
     if (a > h || (a == h && ((int)q & 1))) q += r > 0.f ? 1.f : -1.f;
-    return (int)q;
+    return (uint32_t)((int)q + 8);
 }
 
 __device__ __forceinline__ bool row_of(int strip, int r, int strips, int N, int pair, int* row) {
@@ -91,20 +103,14 @@ quantize_kernel(const T* __restrict__ w, int N, int K, int pair, int strips, int
     for (int half = 0; half < 2; half++)
 #pragma unroll
         for (int g = 0; g < SETS; g++) {
-            float m = 0.f;
-            bool fine = true;
+            uint32_t m = 0;                                               // (magnitudes are ordered as their bits, infinity and NaN above all)
 #pragma unroll
-            for (int i = 0; i < PER; i++) {
-                const float a = fabsf(v[half][(g * PER + i) / 16][(g * PER + i) % 16]);
-                fine = fine && a <= 3.402823466e38f;
-                m = fmaxf(m, a);
-            }
-            if (!fine) m = INFINITY;
-            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-            s[half][g] = scale_of(m);
+            for (int i = 0; i < PER; i++) m = max(m, __float_as_uint(v[half][(g * PER + i) / 16][(g * PER + i) % 16]) & 0x7fffffffu);
+            m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+            m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+            s[half][g] = scale_of<T>(__uint_as_float(m));
             bad = bad || s[half][g] != s[half][g];
-            rs[half][g] = s[half][g] > 0.f ? 1.f / s[half][g] : 0.f;      // (0 too for NaN: q = 0)
+            rs[half][g] = s[half][g] > 0.f ? 1.f / s[half][g] : 0.f;
         }
     if (bad && status) atomicOr(status, ST_NOT_FINITE);
     if (t == 0) {
@@ -124,12 +130,17 @@ quantize_kernel(const T* __restrict__ w, int N, int K, int pair, int strips, int
             const int g = GROUP == 32 ? j / 2 : 0;
             uint32_t o = 0;
 #pragma unroll
-            for (int i = 0; i < 4; i++)                                   // k 4 t + i: pair i / 2, place i % 2
-#pragma unroll
-                for (int half = 0; half < 2; half++) {
-                    const int q = rs[half][g] > 0.f ? code_of(v[half][b][4 * j + i], s[half][g], rs[half][g]) : 0;
-                    o |= (uint32_t)(q + 8) << (16 * (i & 1) + 8 * (i >> 1) + 4 * half);
+            for (int half = 0; half < 2; half++) {
+                if (!(rs[half][g] > 0.f)) {                               // zeros, or no numbers: q = 0
+                    o |= 0x88888888u & (0x0f0f0f0fu << (4 * half));
+                    continue;
                 }
+#pragma unroll
+                for (int i = 0; i < 4; i++) {                             // k 4 t + i: pair i / 2, place i % 2
+                    const int at = 16 * (i & 1) + 8 * (i >> 1) + 4 * half;
+                    o |= (code_of<T>(v[half][b][4 * j + i], s[half][g], rs[half][g]) << at) & (15u << at);
+                }
+            }
             out[j] = o;
         }
         codes[((size_t)gs * blocks + u * SPAN + b) * 32 + lane] = make_uint4(out[0], out[1], out[2], out[3]);

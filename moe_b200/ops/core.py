@@ -198,7 +198,7 @@ WAIT_SITES = {
 WAIT_ROLES = {
     0x1: "producer: a free stage", 0x2: "producer: its own copies in flight", 0x3: "MMA issuer: a free accumulator",
     0x4: "MMA issuer: a loaded stage", 0x5: "epilogue: a finished accumulator",
-    0x6: "converter: a free stage of values", 0x7: "MMA issuer: a stage of values", 0x8: "MMA issuer: its last product",
+    0x6: "converter: a free stage", 0x8: "MMA issuer: its last product",
 }
 WAIT_ROLES_ATTENTION = {
     0x1: "producer: a free key stage", 0x2: "producer: a free value stage", 0x3: "producer: its own copies in flight",

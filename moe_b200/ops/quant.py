@@ -193,12 +193,17 @@ def gemm4(x: torch.Tensor, w: Weight4, out: torch.Tensor, *, swiglu: bool = Fals
 
 
 def _splits(M: int, N: int, w: Weight4, device) -> int:
-    """K splits of a tensor-core product: as many as find SMs for all tiles of 128 features (64 of a pair) and up to 192 rows, 4 blocks of 64 k
-    and more each."""
+    """K splits of a tensor-core product whose tiles (128 features, 64 of a pair, and up to 256 rows) leave SMs without work: four or two where a cluster
+    of that size finds room for every tile at once, 4 blocks of 64 k and more each.  (us, none / 2 / 3 / 4 / 8: 113 rows of 2,048 x 5,632, 16 tiles, 34.8 /
+    20.8 / - / 13.0 / 20.5; 32 rows of 6,144 x 2,048, 48 tiles, 13.4 / 10.4 / 16.6 / 14.8 / 26.2: clusters of three or eight leave SMs of a GPC unused,
+    and what does not fit at once takes a second round.)"""
     from . import tc
 
-    tiles = -(-M // 192) * -(-N // (64 if w.pair else 128))
-    return max(1, min(8, tc.num_sms(device) // tiles, -(-w.K // 64) // 4))
+    tiles, sms, blocks = -(-M // 256) * -(-N // (64 if w.pair else 128)), tc.num_sms(device), -(-w.K // 64)
+    for splits in (4, 2):
+        if tiles * splits <= sms * 9 // 10 and blocks >= 4 * splits:
+            return splits
+    return 1
 
 
 def experts4(x: torch.Tensor, topk_idx: torch.Tensor, topk_w: torch.Tensor, gate_up: Weight4, down: Weight4, out: torch.Tensor, *,
