@@ -30,25 +30,39 @@ def _dtype(dtype) -> torch.dtype:
     return _DTYPES[dtype]
 
 
-def load_model(model_dir: str, dtype="bfloat16", device="cuda"):
+def _weight_group(weights, group: int) -> int:
+    if weights in (None, ""):
+        return 0
+    if weights != "int4":
+        raise ValueError(f"weights: 'int4' or nothing, not {weights!r}")
+    if group not in (32, 64, 128):
+        raise ValueError(f"weight_group: 32, 64 or 128, not {group!r}")
+    return group
+
+
+def load_model(model_dir: str, dtype="bfloat16", device="cuda", weights=None, weight_group: int = 64):
     """Load a model folder (config.json + *.safetensors); the class of model is chosen
-    by config.json through the architecture registry."""
+    by config.json through the architecture registry.
+
+    ``weights="int4"`` (with dtype bfloat16): the matrices of attention, recurrent mixers and feed-forwards, routed experts among them, are held in
+    4 bits, ``weight_group`` (32, 64 or 128) neighbouring elements of a row to a scale (``ops.quant``); embedding, output projection, routers, norms and
+    what the checkpoint stores in 32 bits stay as they are."""
     from .models import DecoderModel
 
     arch, typed = parse_config(read_config_json(model_dir))
     spec = arch.model_spec(typed)
-    model = DecoderModel(spec, SafetensorsStore(model_dir), Runtime(device, _dtype(dtype)))
+    model = DecoderModel(spec, SafetensorsStore(model_dir), Runtime(device, _dtype(dtype), _weight_group(weights, weight_group)))
     model.config = typed
     return model
 
 
 def random_model(config: Union[Dict[str, Any], Any], seed: int = 0, dtype="bfloat16", device="cuda",
-                 std: float = 0.02, stored_dtype=None):
+                 std: float = 0.02, stored_dtype=None, weights=None, weight_group: int = 64):
     """A model with random weights drawn on ``device`` (no files written), part by part: at no
     time is more held than the model itself and the tensors of the part being bound.
     ``stored_dtype``: the dtype the weights are drawn in, as if a checkpoint of that dtype were read
     (default: ``dtype``); a float32 model of bfloat16 weights has exactly the weights of the
-    bfloat16 model of the same seed."""
+    bfloat16 model of the same seed.  ``weights``, ``weight_group``: as in ``load_model``."""
     from .models import DecoderModel
 
     if isinstance(config, dict):
@@ -60,7 +74,7 @@ def random_model(config: Union[Dict[str, Any], Any], seed: int = 0, dtype="bfloa
     spec = arch.model_spec(typed)
     dt = _dtype(dtype)
     model = DecoderModel(spec, RandomStore(spec, seed, std, _dtype(stored_dtype) if stored_dtype else dt, device),
-                         Runtime(device, dt), check=False)
+                         Runtime(device, dt, _weight_group(weights, weight_group)), check=False)
     model.config = typed
     return model
 

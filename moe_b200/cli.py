@@ -10,7 +10,7 @@ Options keep the reference's names, meanings and defaults where it has them
 (``--ids``, ``-n/--tokens`` [128], ``--ctx``, ``--temp`` [0], ``--top-p`` [0.95],
 ``--top-k`` [0], ``--repeat-penalty`` [1.0], ``--seed`` [0], ``--prompts``,
 ``--no-stream``, ``--stats``, ``--prompt-len`` [32], bench ``--tokens`` [16]).
-Added here: ``--dtype bfloat16|float32`` [bfloat16], ``--batch N``,
+Added here: ``--dtype bfloat16|float32`` [bfloat16], ``--weights int4`` with ``--weight-group N`` [64], ``--batch N``,
 ``--max-tokens N`` (cache size), ``--random CONFIG.json`` (with ``--seed``),
 ``--peak-gbs F`` (bench: the bandwidth its roofline line is a percentage of).  Prompts are token ids; there is no tokenizer.
 Arguments are parsed as the reference does: ``--k v``, ``--k=v``, short aliases
@@ -63,6 +63,9 @@ GLOBAL
       --random CONFIG.json  instead of <model>: random weights of this configuration, drawn on
                             the GPU from --seed (the sampler's seed and the weights' are one option)
       --dtype NAME          bfloat16 | float32            [bfloat16]
+      --weights int4        hold the layers' matrices in 4 bits (with bfloat16), a scale for every
+                            group of elements
+      --weight-group N      elements a scale: 32, 64 or 128   [64]
       --max-tokens N        tokens the cache can hold     [what the run needs]
   -h, --help                this message
   -V, --version             version
@@ -138,12 +141,14 @@ def _load(path: str, opt, device="cuda"):
     import moe_b200
 
     dtype = opt.get("dtype", "bfloat16")
+    # (``info`` says what a folder holds, and loads on the CPU, which has no 4-bit weights)
+    held = {} if device == "cpu" else dict(weights=opt.get("weights"), weight_group=_num(opt, "weight-group", 64, int))
     try:
         if "random" in opt:
             with open(opt["random"], encoding="utf-8") as f:
                 cfg = json.load(f)
-            return moe_b200.random_model(cfg, seed=_num(opt, "seed", 0, int), dtype=dtype, device=device)
-        return moe_b200.load_model(path, dtype=dtype, device=device)
+            return moe_b200.random_model(cfg, seed=_num(opt, "seed", 0, int), dtype=dtype, device=device, **held)
+        return moe_b200.load_model(path, dtype=dtype, device=device, **held)
     except (moe_b200.ConfigError, moe_b200.WeightError, ValueError, OSError) as e:
         fail(e)
 
@@ -186,20 +191,20 @@ def step_bytes(model, live_lengths: List[int]) -> Tuple[float, float]:
     """Bytes that a step of one token for each of the live sequences has to read: every weight it
     uses once (``Part.step_elements``; a layer that the schedule runs twice is read twice), and
     the keys and values of the live sequences (a window bounds them).  -> (weights, cache)"""
-    esize = 2 if model.rt.is_bf16 else 4
-    B = len(live_lengths)
-    weights = model.embedding.step_elements(B) + model.final_norm.step_elements(B) + model.head.step_elements(B)
+    rt, B = model.rt, len(live_lengths)
+    esize = 2 if rt.is_bf16 else 4
+    weights = model.embedding.step_bytes(B, rt) + model.final_norm.step_bytes(B, rt) + model.head.step_bytes(B, rt)
     cache = 0.0
     for e in model.spec.schedule:
         blk = model.blocks[e.layer]
-        weights += sum(p.step_elements(B) for p in blk.parts())
+        weights += sum(p.step_bytes(B, rt) for p in blk.parts())
         if e.join is not None:
-            weights += model.joins[e.join].step_elements(B)
+            weights += model.joins[e.join].step_bytes(B, rt)
         req = blk.mixer.kv_request()
         if req is not None:
             per_pos = 2 * req.num_kv_heads * req.head_dim * esize
             cache += per_pos * sum(min(n, req.window) if req.window else n for n in live_lengths)
-    return weights * esize, cache
+    return weights, cache
 
 
 def cmd_info(path: str, opt) -> None:

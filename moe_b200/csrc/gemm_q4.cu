@@ -789,19 +789,14 @@ MOE_API int moe_gemm_q4(const void* x, int ldx, int M, const void* codes, const 
 #undef GO
 }
 
-// Bytes of scratch that moe_experts_q4 wants, 16-byte aligned
-MOE_API long long moe_experts_q4_scratch(int T, int top_k, int E, int size, int shared) {
-    const long long slots = (long long)T * top_k < E ? (long long)T * top_k : E;
-    return (slots * ((size + 63) / 64) + (shared + 63) / 64) * 2048;
-}
-
 // x: [T, H] bfloat16, row pitch ldx; idx, wk: [T, top_k]; gate: [T] or null; gu [E, 2 size, H] and sgu [2 shared, H] pairs, down [E, H, size], sdown
-// [H, shared]; shared 0: no shared expert.  Returns -1 for what it does not take: more than 8 tokens, 1,024 experts or 128 picks, rows that shared
+// [H, shared]; shared 0: no shared expert; scratch: 2 KB for each 64 features of the experts that may be picked
+// (min(T top_k, E)) and of the shared one.  Returns -1 for what it does not take: more than 8 tokens, 1,024 experts or 128 picks, rows that shared
 // memory does not hold (H beyond 7,000 or so).
 MOE_API int moe_experts_q4(const void* x, int ldx, int T, int H, const int* idx, const float* wk, int top_k, int E, int size, const void* gu_codes,
                            const void* gu_scales, const void* down_codes, const void* down_scales, int shared, const void* sgu_codes,
                            const void* sgu_scales, const void* sdown_codes, const void* sdown_scales, const float* gate, int group, void* scratch,
-                           void* out, int out_bf16, int ldo, int* status, cudaStream_t stream) {
+                           long long scratch_bytes, void* out, int out_bf16, int ldo, int* status, cudaStream_t stream) {
     if (T <= 0 || H <= 0) return 0;
     if (T > FEW || E > EXPERTS_MAX || (long long)T * top_k > PAIRS_MAX) return -1;
     if (!x || !idx || !wk || !scratch || !out || E <= 0 || top_k <= 0 || size <= 0 || ((uintptr_t)scratch & 15) || (shared > 0 && (!sgu_codes || !sdown_codes)))
@@ -814,6 +809,7 @@ MOE_API int moe_experts_q4(const void* x, int ldx, int T, int H, const int* idx,
     if (shared > 0) up.shared = weight(sgu_codes, sgu_scales, 2 * shared, H, group, 1), d.shared = weight(sdown_codes, sdown_scales, H, shared, group, 0);
     const long long slots = (long long)T * top_k < E ? (long long)T * top_k : E;
     up.frag = (uint8_t*)scratch, up.frag_blocks = d.down.blocks, up.sfrag = up.frag + slots * d.down.blocks * 2048;
+    if (scratch_bytes < (slots * d.down.blocks + (shared + 63) / 64) * 2048) return (int)cudaErrorInvalidValue;
     d.frag = up.frag, d.sfrag = up.sfrag, d.bits = up.bits;
     d.T = T, d.H = H, d.E = E, d.top_k = top_k, d.idx = idx, d.wk = wk, d.gate = gate, d.out = out, d.out_bf16 = out_bf16, d.ldo = ldo;
     d.S = max(1, min(8, sm_count() / ((d.down.strips + DOWN_MT - 1) / DOWN_MT)));      // one block an SM

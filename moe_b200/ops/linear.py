@@ -3,7 +3,8 @@
 The bfloat16 path uses the tcgen05 kernel (``tc.gemm_tc``) wherever activations and
 weight are both bfloat16 and the shape qualifies, and the plain kernel otherwise (a
 weight stored in 32-bit, a width that is no multiple of 8).  The float32 path always
-uses the plain kernel, which is true 32-bit arithmetic.
+uses the plain kernel, which is true 32-bit arithmetic.  A weight may be a ``quant.Weight4`` (held in 4
+bits), with bfloat16 activations: ``quant.gemm4`` takes every such product.
 """
 from __future__ import annotations
 
@@ -12,6 +13,7 @@ from typing import Optional
 import torch
 
 from . import core
+from .quant import Weight4, gemm4
 
 
 def _use_tc(rt, a: torch.Tensor, w: torch.Tensor) -> bool:
@@ -23,6 +25,8 @@ def linear(rt, a: torch.Tensor, w: torch.Tensor, *, bias: Optional[torch.Tensor]
     """a: [M, K]; w: [N, K]; returns [M, N] in ``out_dtype``.  ``beside``: see ``tc.gemm_tc``; so, from 257 rows on, on the runtime
     of a branch (``Runtime.beside``): the other branch wants the SMs that the splits would fill"""
     out = torch.empty((a.shape[0], w.shape[0]), dtype=out_dtype, device=a.device)
+    if isinstance(w, Weight4):
+        return gemm4(a, w, out, bias=bias, status=rt.status)
     if _use_tc(rt, a, w):
         from . import tc
 
@@ -39,6 +43,8 @@ def swiglu_linear(rt, a: torch.Tensor, w_gate_up: torch.Tensor, act: str = "silu
     constant, if it has one)."""
     M, inter = a.shape[0], w_gate_up.shape[0] // 2
     out = torch.empty((M, inter), dtype=rt.compute_dtype, device=a.device)
+    if isinstance(w_gate_up, Weight4):
+        return gemm4(a, w_gate_up, out, swiglu=True, status=rt.status, act=act, act_param=act_param)
     if _use_tc(rt, a, w_gate_up):
         from . import tc
 
@@ -50,6 +56,14 @@ def swiglu_linear(rt, a: torch.Tensor, w_gate_up: torch.Tensor, act: str = "silu
     return out
 
 
+def _gather(rt, a: torch.Tensor, rows: torch.Tensor, n: int) -> torch.Tensor:
+    if a.shape[1] % 8 == 0 and a.stride(0) % 8 == 0:
+        from . import tc
+
+        return tc.gather_rows(a, rows, n, rt.status)
+    return a.index_select(0, rows[:n])
+
+
 def grouped_swiglu_linear(rt, a: torch.Tensor, w_gate_up: torch.Tensor, group_offsets: torch.Tensor,
                           rows: Optional[torch.Tensor], num_rows: int,
                           gathered: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -58,6 +72,9 @@ def grouped_swiglu_linear(rt, a: torch.Tensor, w_gate_up: torch.Tensor, group_of
     a[rows] already gathered; with ``rows`` None, a itself holds them in order."""
     inter = w_gate_up.shape[1] // 2
     act = torch.empty((num_rows, inter), dtype=rt.compute_dtype, device=a.device)
+    if isinstance(w_gate_up, Weight4):
+        xs = a if rows is None else gathered if gathered is not None else _gather(rt, a, rows, num_rows)
+        return gemm4(xs, w_gate_up, act, swiglu=True, group_offsets=group_offsets, status=rt.status)
     if _use_tc(rt, a, w_gate_up) and a.shape[1] % 8 == 0:
         from . import tc
 
@@ -75,6 +92,8 @@ def grouped_linear(rt, a: torch.Tensor, w: torch.Tensor, group_offsets: torch.Te
     """Rows [offsets[g], offsets[g+1]) of a use w[g] ([G, N, K]); returns float32 [num_rows, N].
     ``early_offsets``: see ``tc.gemm_tc``."""
     out = torch.empty((num_rows, w.shape[1]), dtype=torch.float32, device=a.device)
+    if isinstance(w, Weight4):
+        return gemm4(a, w, out, group_offsets=group_offsets, status=rt.status)
     if _use_tc(rt, a, w):
         from . import tc
 

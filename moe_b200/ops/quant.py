@@ -26,7 +26,7 @@ from . import build, core
 
 GROUPS = (32, 64, 128)
 EXPERTS_TOKENS = 8            # tokens that ``experts4`` takes
-FEW_ROWS = 16                 # rows up to which a product streams its weights through registers
+FEW_ROWS = 16                 # rows (of a group: on average) up to which a product streams its weights through registers
 
 _lib = None
 
@@ -35,15 +35,14 @@ def lib():
     global _lib
     if _lib is None:
         L = build.load("q4")
-        P, I, F = c_void_p, c_int, c_float
+        P, I, F, LL = c_void_p, c_int, c_float, c_longlong
         for name, args in (("moe_q4_quantize", [P, I, I, I, I, I, I, P, P, P, P]),
                            ("moe_q4_dequantize", [P, P, I, I, I, I, I, P, P]),
                            ("moe_gemm_q4", [P, I, I, P, P, I, I, I, I, I, P, I, I, P, P, I, F, P, P]),
                            ("moe_gemm_q4_tc", [P, I, I, P, P, I, I, I, I, I, P, I, I, P, P, I, F, I, P, P]),
-                           ("moe_experts_q4", [P, I, I, I, P, P, I, I, I, P, P, P, P, I, P, P, P, P, P, I, P, P, I, I, P, P])):
+                           ("moe_experts_q4", [P, I, I, I, P, P, I, I, I, P, P, P, P, I, P, P, P, P, P, I, P, LL, P, I, I, P, P])):
             fn = getattr(L, name)
             fn.argtypes, fn.restype = args, c_int
-        L.moe_experts_q4_scratch.argtypes, L.moe_experts_q4_scratch.restype = [I] * 5, c_longlong
         L.moe_q4_set_wait_test.argtypes, L.moe_q4_set_wait_test.restype = [I, c_uint], None
         L.moe_q4_set_pdl.argtypes, L.moe_q4_set_pdl.restype = [I], None
         if os.environ.get("MOE_B200_PDL", "1") == "0":      # programmatic dependent launch off
@@ -61,27 +60,39 @@ class Weight4:
     significant bits.  Rows beyond N have scale 0, elements beyond K q = 0.  With ``pair`` the rows are a gated feed-forward's, N / 2 of
     the gate and N / 2 of up, and either half fills whole strips; a pair is what products with ``swiglu`` take."""
 
-    __slots__ = ("codes", "scales", "shape", "group", "pair", "G", "N", "K")
+    __slots__ = ("codes", "scales", "shape", "group", "pair", "G", "N", "K", "place", "pointers")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, shape: Tuple[int, ...], group: int = 64, pair: bool = False):
-        if len(shape) not in (2, 3) or min(shape) < 1:
+        if len(shape) == 2:
+            G, (N, K) = 1, shape
+        elif len(shape) == 3:
+            G, N, K = shape
+        else:
             raise core.KernelError(f"Weight4: the shape is (N, K) or (G, N, K), not {tuple(shape)}")
+        if G < 1 or N < 1 or K < 1:
+            raise core.KernelError(f"Weight4: a shape without elements, {tuple(shape)}")
         if group not in GROUPS:
             raise core.KernelError(f"Weight4: the group is one of {GROUPS}, not {group}")
-        self.G, self.N, self.K = (1, *shape) if len(shape) == 2 else shape
-        if pair and self.N % 2:
+        if pair and N % 2:
             raise core.KernelError("Weight4: a pair has as many gate rows as up rows")
-        strips = self.G * _strips(self.N, pair)
-        if (codes.dtype != torch.uint8 or scales.dtype != torch.bfloat16 or not codes.is_contiguous() or not scales.is_contiguous()
-                or codes.numel() != strips * -(-self.K // 64) * 512 or scales.numel() != strips * -(-self.K // group) * 16
-                or codes.data_ptr() % 16 or scales.data_ptr() % 16 or codes.device != scales.device):
+        strips = G * _strips(N, pair)
+        pc, ps, place = codes.data_ptr(), scales.data_ptr(), codes.get_device()
+        if (codes.dtype is not torch.uint8 or scales.dtype is not torch.bfloat16 or codes.numel() != strips * -(-K // 64) * 512
+                or scales.numel() != strips * -(-K // group) * 16 or not codes.is_contiguous() or not scales.is_contiguous()
+                or pc % 16 or ps % 16 or scales.get_device() != place):
             raise core.KernelError(f"Weight4: codes and scales of {tuple(shape)} in groups of {group} are contiguous uint8 and bfloat16 tensors "
-                                   f"of {strips * -(-self.K // 64) * 512} and {strips * -(-self.K // group) * 16} elements on one device")
-        self.codes, self.scales, self.shape, self.group, self.pair = codes, scales, tuple(shape), int(group), bool(pair)
+                                   f"of {strips * -(-K // 64) * 512} and {strips * -(-K // group) * 16} elements on one device")
+        self.codes, self.scales, self.shape, self.group, self.pair = codes, scales, tuple(shape), group, bool(pair)
+        self.G, self.N, self.K, self.place, self.pointers = G, N, K, place, (pc, ps)
 
     @property
     def device(self) -> torch.device:
         return self.codes.device
+
+    @property
+    def dtype(self) -> str:
+        """(No ``torch.dtype``: whoever asks whether a weight is bfloat16 is told no.)"""
+        return "int4"
 
     @property
     def nbytes(self) -> int:
@@ -95,27 +106,32 @@ def _strips(N: int, pair: bool) -> int:
     return 2 * -(-(N // 2) // 16) if pair else -(-N // 16)
 
 
-def _here(device: torch.device, what: str):
+def _here(place: int, what: str):
     """A kernel launches on the current device's current stream: its tensors have to lie there."""
-    if device.type != "cuda":
+    if place < 0:
         raise core.KernelError(f"{what}: expected CUDA tensors; there is no CPU path")
-    if core._raw_device is not None and device.index != core._raw_device():
-        raise core.KernelError(f"{what}: tensors on {device}, but the current device is cuda:{core._raw_device()}")
+    if core._raw_device is not None and place != core._raw_device():
+        raise core.KernelError(f"{what}: tensors on cuda:{place}, but the current device is cuda:{core._raw_device()}")
 
 
-def _on(t: Optional[torch.Tensor], device, name: str, dtype, numel: Optional[int] = None):
+def _on(t: Optional[torch.Tensor], place: int, name: str, dtype, numel: Optional[int] = None):
     if t is None:
         return None
-    if t.dtype != dtype or t.device != device or not t.is_contiguous() or (numel is not None and t.numel() != numel):
-        raise core.KernelError(f"{name}: expected a contiguous {dtype} tensor{'' if numel is None else f' of {numel} elements'} on {device}, got "
+    if t.dtype is not dtype or t.get_device() != place or not t.is_contiguous() or (numel is not None and t.numel() != numel):
+        raise core.KernelError(f"{name}: expected a contiguous {dtype} tensor{'' if numel is None else f' of {numel} elements'} on cuda:{place}, got "
                                f"{t.dtype} {tuple(t.shape)} on {t.device}")
     return t.data_ptr()
 
 
-def _matrix(t: torch.Tensor, device, name: str, dtypes):
-    if t.dtype not in dtypes or t.device != device or t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
-        raise core.KernelError(f"{name}: expected a matrix of {' or '.join(map(str, dtypes))} with dense rows on {device}, got {t.dtype} "
-                               f"{tuple(t.shape)} with strides {t.stride()} on {t.device}")
+def _matrix(t: torch.Tensor, place: int, name: str, wide: bool):
+    """(rows, columns, row pitch) of a matrix with dense rows, bfloat16 or (``wide``) float32."""
+    if (t.dtype is not torch.bfloat16 and not (wide and t.dtype is torch.float32)) or t.get_device() != place or t.dim() != 2:
+        raise core.KernelError(f"{name}: expected a matrix of bfloat16{' or float32' if wide else ''} on cuda:{place}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    rows, columns = t.shape
+    pitch, step = t.stride()
+    if (step != 1 and columns > 1) or (rows > 1 and pitch < columns):
+        raise core.KernelError(f"{name}: expected dense rows that do not overlap, got strides {t.stride()} of {tuple(t.shape)}")
+    return rows, columns, pitch
 
 
 def quantize(w: torch.Tensor, group: int = 64, *, pair: bool = False, status=None) -> Weight4:
@@ -123,7 +139,7 @@ def quantize(w: torch.Tensor, group: int = 64, *, pair: bool = False, status=Non
     products over it are NaN, and reported through ``status``."""
     core._chk(w, "w")
     core._dt(w)
-    _here(w.device, "quantize")
+    _here(w.get_device(), "quantize")
     if w.dim() not in (2, 3) or not w.numel():
         raise core.KernelError(f"quantize: a matrix or a stack of matrices, not {tuple(w.shape)}")
     if group not in GROUPS:
@@ -135,19 +151,19 @@ def quantize(w: torch.Tensor, group: int = 64, *, pair: bool = False, status=Non
     codes = torch.empty((G, strips, -(-K // 64), 8, 4, 4, 2, 2), dtype=torch.uint8, device=w.device)
     scales = torch.empty((G, strips, -(-K // group), 8, 2), dtype=torch.bfloat16, device=w.device)
     core._ok(lib().moe_q4_quantize(w.data_ptr(), core._dt(w), G, N, K, group, 1 if pair else 0, codes.data_ptr(), scales.data_ptr(),
-                                   _on(status, w.device, "status", torch.int32), core._stream()), "quantize")
+                                   _on(status, w.get_device(), "status", torch.int32), core._stream()), "quantize")
     return Weight4(codes, scales, tuple(w.shape), group, pair)
 
 
 def dequantize(w: Weight4, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The values that ``w`` stands for, exactly, as bfloat16 of ``w.shape``."""
-    _here(w.device, "dequantize")
+    _here(w.place, "dequantize")
     if out is None:
         out = torch.empty(w.shape, dtype=torch.bfloat16, device=w.device)
     elif tuple(out.shape) != w.shape:
         raise core.KernelError(f"dequantize: out is {tuple(out.shape)}, the weight {w.shape}")
-    core._ok(lib().moe_q4_dequantize(w.codes.data_ptr(), w.scales.data_ptr(), w.G, w.N, w.K, w.group, 1 if w.pair else 0,
-                                     _on(out, w.device, "out", torch.bfloat16), core._stream()), "dequantize")
+    core._ok(lib().moe_q4_dequantize(*w.pointers, w.G, w.N, w.K, w.group, 1 if w.pair else 0,
+                                     _on(out, w.place, "out", torch.bfloat16), core._stream()), "dequantize")
     return out
 
 
@@ -158,48 +174,56 @@ def gemm4(x: torch.Tensor, w: Weight4, out: torch.Tensor, *, swiglu: bool = Fals
     x: bfloat16 [M, K], dense rows of any pitch; out: float32 or bfloat16 [M, N] (a pair: [M, N / 2]), dense rows of any pitch.
     A stack needs ``group_offsets`` (int32 [G + 1], ascending): rows [offsets[g], offsets[g + 1]) of x meet w[g]; rows that no group
     has are left as they were."""
-    dev = x.device
-    _here(dev, "gemm4")
-    _matrix(x, dev, "x", (torch.bfloat16,))
-    _matrix(out, dev, "out", (torch.float32, torch.bfloat16))
-    M, N = x.shape[0], w.N // 2 if swiglu else w.N
-    if w.device != dev or x.shape[1] != w.K or out.shape[0] != M or out.shape[1] != N:
-        raise core.KernelError(f"gemm4: shapes x{tuple(x.shape)} w{w.shape} out{tuple(out.shape)}, on {dev} and {w.device}")
+    place = x.get_device()
+    _here(place, "gemm4")
+    M, K, ldx = _matrix(x, place, "x", False)
+    rows, N, ldo = _matrix(out, place, "out", True)
+    if w.place != place or K != w.K or rows != M or N != (w.N // 2 if swiglu else w.N):
+        raise core.KernelError(f"gemm4: shapes x{tuple(x.shape)} w{w.shape} out{tuple(out.shape)}, on {x.device} and {w.device}")
     if swiglu != w.pair:
         raise core.KernelError("gemm4: a pair is multiplied with swiglu, another weight without")
-    if swiglu and (bias is not None or act not in core.GLU_ACTS):
-        raise core.KernelError("gemm4: a gated product takes no bias and an activation of core.GLU_ACTS")
-    if not swiglu and act != "silu" and act not in core.PLAIN_ACTS:
-        raise core.KernelError("gemm4: the activation of an ungated product is one of core.PLAIN_ACTS")
+    if swiglu:
+        if bias is not None or act not in core.GLU_ACTS:
+            raise core.KernelError("gemm4: a gated product takes no bias and an activation of core.GLU_ACTS")
+        code = core.GLU_ACTS[act]
+    else:
+        if act != "silu" and act not in core.PLAIN_ACTS:
+            raise core.KernelError("gemm4: the activation of an ungated product is one of core.PLAIN_ACTS")
+        code = core.PLAIN_ACTS.get(act, 0)
     if group_offsets is None and w.G != 1:
         raise core.KernelError("gemm4: a stack needs group_offsets")
-    code = core.GLU_ACTS[act] if swiglu else core.PLAIN_ACTS.get(act, 0)
+    pb = _on(bias, place, "bias", torch.float32, N)
+    po = _on(group_offsets, place, "group_offsets", torch.int32, w.G + 1)
+    st = _on(status, place, "status", torch.int32)
     if not M:
         return out
-    args = (x.data_ptr(), x.stride(0), M, w.codes.data_ptr(), w.scales.data_ptr(), w.G, w.N, w.K, w.group, 1 if w.pair else 0, out.data_ptr(),
-            1 if out.dtype == torch.bfloat16 else 0, out.stride(0), _on(bias, dev, "bias", torch.float32, N),
-            _on(group_offsets, dev, "group_offsets", torch.int32, w.G + 1), code, float(act_param))
-    st = _on(status, dev, "status", torch.int32)
-    if st is not None and (M > FEW_ROWS if group_offsets is None else M > 16 * w.G):
-        done = lib().moe_gemm_q4_tc(*args, 1 if group_offsets is not None else _splits(M, N, w, dev), st, core._stream())
+    pc, ps = w.pointers
+    L = _lib or lib()
+    # Few rows (of a group: on average) stream the weights through registers, more go to the tensor core, whose tiles of 128 features cost the same
+    # for 16 rows as for 200.  (us, this way / the other: 16 rows of 6,144 x 2,048 9.2 / 10, 32 rows 17 / 10.4; 60 experts of a pair 2,816 x 2,048 at 17
+    # rows an expert 50 / 95, at 34 120 / 121.)
+    if st is not None and (M > FEW_ROWS if po is None else M > FEW_ROWS * w.G):
+        done = L.moe_gemm_q4_tc(x.data_ptr(), ldx, M, pc, ps, w.G, w.N, K, w.group, w.pair, out.data_ptr(), out.dtype is torch.bfloat16, ldo, pb, po,
+                                code, act_param, 1 if po is not None else _splits(M, N, w, place), st, core._stream())
         if done != -1:
             core._ok(done, "gemm4")
             return out
-    done = lib().moe_gemm_q4(*args, st, core._stream())
+    done = L.moe_gemm_q4(x.data_ptr(), ldx, M, pc, ps, w.G, w.N, K, w.group, w.pair, out.data_ptr(), out.dtype is torch.bfloat16, ldo, pb, po, code,
+                         act_param, st, core._stream())
     if done == -1:
         raise core.KernelError("gemm4: more than 1,024 weights in a stack, or K too large for one")
     core._ok(done, "gemm4")
     return out
 
 
-def _splits(M: int, N: int, w: Weight4, device) -> int:
+def _splits(M: int, N: int, w: Weight4, place: int) -> int:
     """K splits of a tensor-core product whose tiles (128 features, 64 of a pair, and up to 256 rows) leave SMs without work: four or two where a cluster
     of that size finds room for every tile at once, 4 blocks of 64 k and more each.  (us, none / 2 / 3 / 4 / 8: 113 rows of 2,048 x 5,632, 16 tiles, 34.8 /
     20.8 / - / 13.0 / 20.5; 32 rows of 6,144 x 2,048, 48 tiles, 13.4 / 10.4 / 16.6 / 14.8 / 26.2: clusters of three or eight leave SMs of a GPC unused,
     and what does not fit at once takes a second round.)"""
     from . import tc
 
-    tiles, sms, blocks = -(-M // 256) * -(-N // (64 if w.pair else 128)), tc.num_sms(device), -(-w.K // 64)
+    tiles, sms, blocks = -(-M // 256) * -(-N // (64 if w.pair else 128)), tc.num_sms(place), -(-w.K // 64)
     for splits in (4, 2):
         if tiles * splits <= sms * 9 // 10 and blocks >= 4 * splits:
             return splits
@@ -216,40 +240,41 @@ def experts4(x: torch.Tensor, topk_idx: torch.Tensor, topk_w: torch.Tensor, gate
     x: bfloat16 [T, H]; topk_idx int32 and topk_w float32 [T, k]; gate_up: a pair's stack [E, 2 I, H], down: [E, H, I]; the shared expert's two
     likewise without the stack, shared_gate float32 [T] (None: 1); out: float32 or bfloat16 [T, H].  An index of -1 is no pick
     (all of a row's: zeros but for the shared expert), any other outside [0, E) is reported through ``status`` and taken for none.  False, with
-    nothing launched, for more tokens, 1,024 experts or 128 picks than that."""
-    dev = x.device
-    _here(dev, "experts4")
-    _matrix(x, dev, "x", (torch.bfloat16,))
-    _matrix(out, dev, "out", (torch.float32, torch.bfloat16))
-    T, H = x.shape
+    nothing launched, for more tokens, more than 1,024 experts or 128 picks, or rows that shared memory does not hold (H beyond 7,000 or so)."""
+    place = x.get_device()
+    _here(place, "experts4")
+    T, H, ldx = _matrix(x, place, "x", False)
+    rows, columns, ldo = _matrix(out, place, "out", True)
     E, size, k = gate_up.G, gate_up.N // 2, topk_idx.shape[-1] if topk_idx.dim() == 2 else 0
-    if (not gate_up.pair or down.pair or gate_up.K != H or down.G != E or down.N != H or down.K != size or tuple(out.shape) != (T, H)
-            or tuple(topk_idx.shape) != (T, k) or topk_w.shape != topk_idx.shape or gate_up.device != dev or down.device != dev):
+    if (not gate_up.pair or down.pair or gate_up.K != H or down.G != E or down.N != H or down.K != size or rows != T or columns != H
+            or topk_idx.shape != (T, k) or topk_w.shape != (T, k) or gate_up.place != place or down.place != place or not k):
         raise core.KernelError(f"experts4: shapes x{tuple(x.shape)} gate_up{gate_up.shape} down{down.shape} picks{tuple(topk_idx.shape)} "
                                f"weights{tuple(topk_w.shape)} out{tuple(out.shape)}")
-    shared = 0
+    group, shared, s = gate_up.group, 0, (None, None, None, None)
     if (shared_gate_up is None) != (shared_down is None) or (shared_gate is not None and shared_down is None):
         raise core.KernelError("experts4: the shared expert is a pair and its down projection, its gate goes with them")
     if shared_gate_up is not None:
-        shared = shared_gate_up.N // 2
+        shared, s = shared_gate_up.N // 2, shared_gate_up.pointers + shared_down.pointers
         if (not shared_gate_up.pair or shared_down.pair or shared_gate_up.shape != (2 * shared, H) or shared_down.shape != (H, shared)
-                or shared_gate_up.device != dev or shared_down.device != dev):
-            raise core.KernelError(f"experts4: shapes of the shared expert {shared_gate_up.shape} {shared_down.shape}, on {dev}")
-    if any(w is not None and w.group != gate_up.group for w in (down, shared_gate_up, shared_down)):
+                or shared_gate_up.place != place or shared_down.place != place):
+            raise core.KernelError(f"experts4: shapes of the shared expert {shared_gate_up.shape} {shared_down.shape}, on {x.device}")
+        if shared_gate_up.group != group or shared_down.group != group:
+            group = -1
+    if down.group != group:
         raise core.KernelError("experts4: the weights of a layer have one group size")
-    pi, pw = _on(topk_idx, dev, "topk_idx", torch.int32), _on(topk_w, dev, "topk_w", torch.float32)
-    pg, ps = _on(shared_gate, dev, "shared_gate", torch.float32, T), _on(status, dev, "status", torch.int32)
+    pi, pw = _on(topk_idx, place, "topk_idx", torch.int32), _on(topk_w, place, "topk_w", torch.float32)
+    pg, ps = _on(shared_gate, place, "shared_gate", torch.float32, T), _on(status, place, "status", torch.int32)
     if T > EXPERTS_TOKENS or E > 1024 or T * k > 128:
         return False
     if not T:
         return True
-    L = lib()
-    scratch = torch.empty(L.moe_experts_q4_scratch(T, k, E, size, shared), dtype=torch.uint8, device=dev)
-    s = (None, None, None, None) if not shared else (shared_gate_up.codes.data_ptr(), shared_gate_up.scales.data_ptr(),
-                                                     shared_down.codes.data_ptr(), shared_down.scales.data_ptr())
-    code = L.moe_experts_q4(x.data_ptr(), x.stride(0), T, H, pi, pw, k, E, size, gate_up.codes.data_ptr(), gate_up.scales.data_ptr(),
-                            down.codes.data_ptr(), down.scales.data_ptr(), shared, *s, pg, gate_up.group, scratch.data_ptr(), out.data_ptr(),
-                            1 if out.dtype == torch.bfloat16 else 0, out.stride(0), ps, core._stream())
+    L = _lib or lib()
+    slots = min(T * k, E)
+    scratch = torch.empty((slots * -(-size // 64) + -(-shared // 64)) * 2048, dtype=torch.uint8, device=x.device)
+    code = L.moe_experts_q4(x.data_ptr(), ldx, T, H, pi, pw, k, E, size, *gate_up.pointers, *down.pointers, shared, *s, pg, group, scratch.data_ptr(),
+                            scratch.numel(), out.data_ptr(), out.dtype is torch.bfloat16, ldo, ps, core._stream())
+    if code == -1:
+        return False
     core._ok(code, "experts4")
     core.launches += 1            # (two kernels)
     return True

@@ -258,14 +258,14 @@ class GQAttention(Part):
         if self.out_gate:
             ws.append(tensors[n["gate"]])        # the gate's rows ride in the same product
         dt = ws[0].dtype if all(w.dtype == ws[0].dtype for w in ws) else torch.float32
-        self.wqkv = torch.cat([w.to(dt) for w in ws], dim=0).contiguous()
+        self.wqkv = self.hold(rt, torch.cat([w.to(dt) for w in ws], dim=0).contiguous())
         self.bqkv = None
         if self.bias:
             bs = [tensors[n[r + "_bias"]].to(torch.float32) for r in roles]
             if self.out_gate:
                 bs.append(torch.zeros(self.nh * self.vd, dtype=torch.float32, device=bs[0].device))
             self.bqkv = torch.cat(bs).contiguous()
-        self.wo = tensors[n["o"]].contiguous()
+        self.wo = self.hold(rt, tensors[n["o"]].contiguous())
         self.bo = tensors[n["o_bias"]].to(torch.float32).contiguous() if self.o_bias else None
         self.taps_w = None
         if self.taps:

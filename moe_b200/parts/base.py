@@ -109,9 +109,15 @@ class TensorSpec:
 class Runtime:
     """Device, compute dtype and the device status word shared by all parts of a model."""
 
-    def __init__(self, device, compute_dtype: torch.dtype):
+    def __init__(self, device, compute_dtype: torch.dtype, weight_group: int = 0):
+        """``weight_group``: 0, or the group size of matrices held in 4 bits (``ops.quant``)."""
         if compute_dtype not in (torch.float32, torch.bfloat16):
             raise ValueError("compute dtype must be float32 or bfloat16")
+        if weight_group and compute_dtype != torch.bfloat16:
+            raise ValueError("weights in 4 bits go with the compute dtype bfloat16")
+        if weight_group not in (0, 32, 64, 128):
+            raise ValueError(f"weights in 4 bits have groups of 32, 64 or 128, not {weight_group}")
+        self.weight_group = int(weight_group)
         self.device = torch.device(device)
         self.compute_dtype = compute_dtype
         self.forked = False            # see ``beside``
@@ -212,6 +218,24 @@ class Part:
                 k *= d
             n += k
         return float(n)
+
+    # whether the part holds its matrices in 4 bits (``hold``)
+    in_4_bits = False
+
+    def hold(self, rt: Runtime, w: torch.Tensor, pair: bool = False):
+        """What the part keeps of a matrix (or a stack of them) that only products read: the tensor, or where the model holds its weights in 4
+        bits, and this one came in bfloat16, its ``Weight4``.  ``pair``: gate rows and up rows of a gated feed-forward."""
+        if not rt.weight_group or w.dtype != torch.bfloat16:
+            return w
+        from ..ops import quant
+
+        self.in_4_bits = True
+        return quant.quantize(w.contiguous(), rt.weight_group, pair=pair, status=rt.status)
+
+    def step_bytes(self, num_tokens: int, rt: Runtime) -> float:
+        """Bytes of ``step_elements``: a part that holds its matrices in 4 bits counts all its elements so."""
+        each = 0.5 + 2.0 / rt.weight_group if self.in_4_bits else 2 if rt.is_bf16 else 4
+        return self.step_elements(num_tokens) * each
 
     def bind(self, tensors: Dict[str, torch.Tensor], rt: Runtime) -> None:
         """Take ownership of the loaded tensors (re-laying them out is allowed)."""

@@ -119,7 +119,7 @@ class DifferentialAttention(Part):
         if self.out_gate:
             ws.append(tensors[n["gate"]])          # the gate's rows ride in the same product
         dt = ws[0].dtype if all(w.dtype == ws[0].dtype for w in ws) else torch.float32
-        self.wqkv = torch.cat([w.to(dt) for w in ws], dim=0).contiguous()
+        self.wqkv = self.hold(rt, torch.cat([w.to(dt) for w in ws], dim=0).contiguous())
         self.bqkv = None
         if self.bias:
             bv = tensors[n["v_bias"]].to(torch.float32)
@@ -128,7 +128,7 @@ class DifferentialAttention(Part):
             if self.out_gate:
                 bs.append(torch.zeros(H, dtype=torch.float32, device=bv.device))
             self.bqkv = torch.cat(bs).contiguous()
-        self.wo = tensors[n["o"]].contiguous()
+        self.wo = self.hold(rt, tensors[n["o"]].contiguous())
         l = {r: tensors[n[r]].to(torch.float32) for r in ("lq1", "lk1", "lq2", "lk2")}
         # one number a layer, formed once in 32-bit
         self.lam = float((torch.exp((l["lq1"] * l["lk1"]).sum()) - torch.exp((l["lq2"] * l["lk2"]).sum())

@@ -15,6 +15,7 @@ import torch
 
 from ..ops import core
 from ..ops.linear import grouped_linear, grouped_swiglu_linear, linear, swiglu_linear
+from ..ops.quant import EXPERTS_TOKENS, Weight4, experts4, gemm4
 from .base import Activations, LazyDelta, Part, TensorSpec, register_part
 
 
@@ -59,8 +60,8 @@ class DenseSwiGLU(Part):
     def bind(self, tensors, rt):
         super().bind(tensors, rt)
         n = self.names
-        self.w_gu = _fuse_rows([tensors[n["gate"]], tensors[n["up"]]])
-        self.w_down = tensors[n["down"]].contiguous()
+        self.w_gu = self.hold(rt, _fuse_rows([tensors[n["gate"]], tensors[n["up"]]]), pair=True)
+        self.w_down = self.hold(rt, tensors[n["down"]].contiguous())
 
     def forward(self, rt, h, batch):
         return linear(rt, swiglu_linear(rt, h.act, self.w_gu, self.activation, self.limit), self.w_down)
@@ -72,6 +73,8 @@ def act_linear(rt, a, w_up, act, out=None):
     output and then the activation."""
     if out is None:
         out = torch.empty((a.shape[0], w_up.shape[0]), dtype=rt.compute_dtype, device=a.device)
+    if isinstance(w_up, Weight4):
+        return gemm4(a, w_up, out, status=rt.status, act=act)
     if rt.is_bf16 and a.dtype == torch.bfloat16 and w_up.dtype == torch.bfloat16:
         from ..ops import tc
 
@@ -111,8 +114,8 @@ class DenseMLP(Part):
 
     def bind(self, tensors, rt):
         super().bind(tensors, rt)
-        self.w_up = tensors[self.names["up"]].contiguous()
-        self.w_down = tensors[self.names["down"]].contiguous()
+        self.w_up = self.hold(rt, tensors[self.names["up"]].contiguous())
+        self.w_down = self.hold(rt, tensors[self.names["down"]].contiguous())
 
     def forward(self, rt, h, batch):
         return linear(rt, act_linear(rt, h.act, self.w_up, self.activation), self.w_down)
@@ -320,10 +323,14 @@ class RoutedExperts(Part):
                     dst = {"expert_gate": self.w_gu[e, : self.size], "expert_up": self.w_gu[e, self.size:],
                            "expert_down": self.w_down[e]}[role]
                     dst.copy_(t)
+        self.w_gu, self.w_down = self.hold(rt, self.w_gu, pair=True), self.hold(rt, self.w_down)
         self.ws_gu = self.ws_down = self.w_sgate = None
         if self.shared_size:
-            self.ws_gu = _fuse_rows([tensors[n["shared_gate_proj"]], tensors[n["shared_up"]]])
-            self.ws_down = tensors[n["shared_down"]].contiguous()
+            self.ws_gu = self.hold(rt, _fuse_rows([tensors[n["shared_gate_proj"]], tensors[n["shared_up"]]]), pair=True)
+            self.ws_down = self.hold(rt, tensors[n["shared_down"]].contiguous())
+        # all of the layer's experts in 4 bits: up to 8 tokens go through them in two launches, combine included
+        self.whole_in_4_bits = all(isinstance(w, Weight4) for w in (self.w_gu, self.w_down)) and (
+            not self.shared_size or all(isinstance(w, Weight4) for w in (self.ws_gu, self.ws_down)))
         if self.shared_gate:
             self.w_sgate = tensors[n["shared_gate"]].reshape(-1).to(self.w_router.dtype).contiguous()
         # For prompts the router's logits come from the tensor cores: the 32-bit activations as three
@@ -335,7 +342,7 @@ class RoutedExperts(Part):
             self.w_router3 = torch.cat([one, one, one], dim=1).contiguous()
         # every product that reads the normed rows takes them on the tensor cores, from rows of any pitch
         self.split_router = self.w_router3 is not None and all(
-            w is None or (w.dtype == torch.bfloat16 and w.data_ptr() % 16 == 0) for w in (self.w_gu, self.ws_gu, self.w_router3))
+            w is None or isinstance(w, Weight4) or (w.dtype == torch.bfloat16 and w.data_ptr() % 16 == 0) for w in (self.w_gu, self.ws_gu, self.w_router3))
 
     def route(self, rt, h, batch, after_logits=None):
         """-> (topk_idx [T, k] int32, topk_w [T, k] float32, shared_gate [T] float32 or None)
@@ -380,10 +387,11 @@ class RoutedExperts(Part):
         return linear(rt, swiglu_linear(rt, h.act, self.ws_gu), self.ws_down, beside=beside and h.act.shape[0] <= 256)
 
     def forward(self, rt, h, batch):
-        return self._run(rt, h, batch, None).materialize(rt)
+        out = self._run(rt, h, batch, None)
+        return out.materialize(rt) if isinstance(out, LazyDelta) else out
 
     def forward_lazy(self, rt, h, batch):
-        """The same, the combine left to whoever adds the delta (see ``CombineDelta``)."""
+        """The same, the combine left to whoever adds the delta (see ``CombineDelta``); a tensor where nothing is left to combine."""
         return self._run(rt, h, batch, None)
 
     def forward_prenorm(self, rt, x, delta, norm, batch):
@@ -423,8 +431,24 @@ class RoutedExperts(Part):
         h = Activations(act=out16 if rt.is_bf16 else out32, f32=out32)
         return self._run(rt, h, batch, routed[2:])
 
+    def _whole_in_4_bits(self, rt, h, batch, routed):
+        """Router (where ``routed`` does not bring its picks), then all experts, the shared one and the combine; None where they do not fit."""
+        T = h.act.shape[0]
+        if not self.whole_in_4_bits or T > EXPERTS_TOKENS or self.weight_input or h.act.dtype != torch.bfloat16:
+            return None
+        topk_idx, topk_w, sg = routed[:3] if routed is not None else self.route(rt, h, batch)
+        out = rt.empty((T, self.hidden), torch.float32)
+        if not experts4(h.act, topk_idx, topk_w, self.w_gu, self.w_down, out, shared_gate_up=self.ws_gu, shared_down=self.ws_down, shared_gate=sg,
+                        status=rt.status):
+            return None
+        self._record(topk_idx, topk_w)
+        return out
+
     def _run(self, rt, h, batch, routed):
         T = h.act.shape[0]
+        whole = self._whole_in_4_bits(rt, h, batch, routed)
+        if whole is not None:
+            return whole
         if self.ws_gu is None:
             return self._routed(rt, h, batch, routed, self._record)
         if not (T <= 64 and self.E <= 256) and not (self.shared_beside and rt.is_bf16 and T <= self.shared_first_tokens):

@@ -188,8 +188,8 @@ class LatentAttention(Part):
         if rot or self.q_rank or self.head_gate:
             total = sum(w.shape[0] for w in rows)
             rows.append(torch.zeros((-total % 8, self.hidden), dtype=dt, device=wdown.device))
-        self.w_in = torch.cat(rows, dim=0).contiguous()
-        self.w_q_up = wq.to(dt).contiguous() if self.q_rank else None
+        self.w_in = self.hold(rt, torch.cat(rows, dim=0).contiguous())
+        self.w_q_up = self.hold(rt, wq.to(dt).contiguous()) if self.q_rank else None
         self.cq_norm = tensors[n["q_down_norm"]].to(torch.float32).contiguous() if self.q_rank else None
         # with a gate the attended latents are gated and packed to r columns a head; without one the output
         # projection reads whole records (its columns beyond r are zeros)
@@ -199,11 +199,11 @@ class LatentAttention(Part):
             ov = torch.bmm(wo.double().reshape(self.hidden, H, dv).transpose(0, 1), uv.double())     # [H, hidden, r]
             full = torch.zeros((self.hidden, H, r if self.packs else D), dtype=torch.float64, device=ov.device)
             full[:, :, :r] = ov.transpose(0, 1)
-            self.wo = full.reshape(self.hidden, -1).to(wo.dtype).contiguous()
+            self.wo = self.hold(rt, full.reshape(self.hidden, -1).to(wo.dtype).contiguous())
             self.w_cv = None
         else:
             self.w_cv = uv.contiguous()                                    # grouped [head, dv, r]
-            self.wo = wo.contiguous()
+            self.wo = self.hold(rt, wo.contiguous())
         self.w_norm = tensors[n["down_norm"]].to(torch.float32).contiguous()
         self.sinks = tensors[n["sink"]].to(torch.float32).contiguous() if self.sink else False
         self._offsets = {}

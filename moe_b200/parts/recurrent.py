@@ -107,7 +107,7 @@ class WKVMixer(Part):
         self.w0 = tensors[n["w0"]].to(torch.float32).contiguous()
         self.u = tensors[n["u"]].to(torch.float32).contiguous()
         self.norm_w = tensors[n["norm"]].to(torch.float32).contiguous()
-        self.wo = tensors[n["o"]].contiguous()
+        self.wo = self.hold(rt, tensors[n["o"]].contiguous())
         self._offsets = {}
 
     def _group_offsets(self, T, device):
@@ -223,14 +223,14 @@ class SSDMixer(Part):
     def bind(self, tensors, rt):
         super().bind(tensors, rt)
         n = self.names
-        self.w_in = tensors[n["in"]].contiguous()
+        self.w_in = self.hold(rt, tensors[n["in"]].contiguous())
         self.taps_w = tensors[n["conv"]].to(torch.float32).t().contiguous()          # [taps, channels]
         self.conv_b = tensors[n["conv_bias"]].to(torch.float32).contiguous()
         self.dt_bias = tensors[n["dt_bias"]].to(torch.float32).contiguous()
         self.a_log = tensors[n["a_log"]].to(torch.float32).contiguous()
         self.d_skip = tensors[n["d"]].to(torch.float32).contiguous()
         self.norm_w = tensors[n["norm"]].to(torch.float32).contiguous()
-        self.wo = tensors[n["o"]].contiguous()
+        self.wo = self.hold(rt, tensors[n["o"]].contiguous())
 
     def forward(self, rt, h, batch, cache_view, state):
         T, I, C = batch.num_tokens, self.inner, self.channels
@@ -324,14 +324,14 @@ class DeltaMixer(Part):
         rows = sum(w.shape[0] for w in ws)
         # (rows of zeros up to a multiple of eight: rows of the output stay 16-byte units)
         ws.append(torch.zeros((-rows % 8, self.hidden), dtype=dt, device=ws[0].device))
-        self.w_in = torch.cat([w.to(dt) for w in ws], dim=0).contiguous()
+        self.w_in = self.hold(rt, torch.cat([w.to(dt) for w in ws], dim=0).contiguous())
         self.gate_at = self.channels
         self.b_at, self.a_at = self.channels + self.inner, self.channels + self.inner + self.nh
         self.taps_w = torch.cat([tensors[n[r + "_conv"]].to(torch.float32) for r in ("q", "k", "v")], dim=0).t().contiguous()
         self.a_log = tensors[n["a_log"]].to(torch.float32).contiguous()
         self.dt_bias = tensors[n["dt_bias"]].to(torch.float32).contiguous()
         self.norm_w = tensors[n["norm"]].to(torch.float32).repeat(self.nh).contiguous()
-        self.wo = tensors[n["o"]].contiguous()
+        self.wo = self.hold(rt, tensors[n["o"]].contiguous())
 
     gate_fn = "silu"
 
@@ -413,7 +413,7 @@ class ChannelDeltaMixer(DeltaMixer):
         dt = ws[0].dtype if all(w.dtype == ws[0].dtype for w in ws) else torch.float32
         dev = ws[0].device
         ws.append(torch.zeros((-sum(w.shape[0] for w in ws) % 8, self.hidden), dtype=dt, device=dev))
-        self.w_in = torch.cat([w.to(dt) for w in ws], dim=0).contiguous()
+        self.w_in = self.hold(rt, torch.cat([w.to(dt) for w in ws], dim=0).contiguous())
         self.gate_at = self.a_at = 0                   # (the gate and the decays have a product of their own)
         self.b_at = self.channels
         a1, a2, g1, g2 = (tensors[n[r]] for r in ("a1", "a2", "g1", "g2"))
@@ -432,7 +432,7 @@ class ChannelDeltaMixer(DeltaMixer):
         self.a_log = tensors[n["a_log"]].to(torch.float32).contiguous()
         self.dt_bias = tensors[n["dt_bias"]].to(torch.float32).contiguous()
         self.norm_w = tensors[n["norm"]].to(torch.float32).repeat(self.nh).contiguous()
-        self.wo = tensors[n["o"]].contiguous()
+        self.wo = self.hold(rt, tensors[n["o"]].contiguous())
 
     def _low(self, rt, h):
         low = linear(rt, h.act, self.w_low1, out_dtype=rt.compute_dtype)
@@ -518,11 +518,11 @@ class MLSTMMixer(Part):
             self.at[r] = rows
             rows += w.shape[0]
         ws.append(torch.zeros((-rows % 8, self.hidden), dtype=dt, device=ws[0].device))
-        self.w_in = torch.cat([w.to(dt) for w in ws], dim=0).contiguous()
+        self.w_in = self.hold(rt, torch.cat([w.to(dt) for w in ws], dim=0).contiguous())
         self.i_bias = tensors[n["i_bias"]].to(torch.float32).contiguous()
         self.f_bias = tensors[n["f_bias"]].to(torch.float32).contiguous()
         self.norm_w = tensors[n["norm"]].to(torch.float32).contiguous()
-        self.wo = tensors[n["o"]].contiguous()
+        self.wo = self.hold(rt, tensors[n["o"]].contiguous())
 
     def forward(self, rt, h, batch, cache_view, state):
         T, I = batch.num_tokens, self.inner
@@ -620,6 +620,9 @@ class SideBySideMixer(Part):
 
     def step_elements(self, num_tokens):
         return float(sum(m.step_elements(num_tokens) for _, m in self.subs) + (2 * self.hidden if self.scales is None else 0))
+
+    def step_bytes(self, num_tokens, rt):
+        return sum(m.step_bytes(num_tokens, rt) for _, m in self.subs) + (2 * self.hidden * (2 if rt.is_bf16 else 4) if self.scales is None else 0)
 
     def kv_request(self):
         for _, m in self.subs:
