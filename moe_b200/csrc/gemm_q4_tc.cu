@@ -477,7 +477,7 @@ int launch(const CUtensorMap& map, const Args& p, unsigned ctas, cudaStream_t st
 MOE_API int moe_gemm_q4_tc(const void* x, int ldx, int M, const void* codes, const void* scales, int G, int N, int K, int group, int pair, void* out,
                            int out_bf16, int ldo, const float* bias, const int* offsets, int act, float act_param, int splits, int* status, cudaStream_t stream) {
     if (M <= 0 || N <= 0) return 0;
-    if (!x || !codes || !scales || !out || !status || K <= 0 || G <= 0 || (G > 1 && !offsets) || (pair && N % 2)) return (int)cudaErrorInvalidValue;
+    if (!x || !codes || !scales || !out || K <= 0 || G <= 0 || (G > 1 && !offsets) || (pair && N % 2)) return (int)cudaErrorInvalidValue;
     if (K % 8 || ldx % 8 || ((uintptr_t)x & 15) || G > MAX_GROUPS || !encode_fn()) return -1;
     CUtensorMap map;
     const cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)M}, strides[1] = {(cuuint64_t)ldx * 2};

@@ -202,18 +202,19 @@ def gemm4(x: torch.Tensor, w: Weight4, out: torch.Tensor, *, swiglu: bool = Fals
     # Few rows (of a group: on average) stream the weights through registers, more go to the tensor core, whose tiles of 128 features cost the same
     # for 16 rows as for 200.  (us, this way / the other: 16 rows of 6,144 x 2,048 9.2 / 10, 32 rows 17 / 10.4; 60 experts of a pair 2,816 x 2,048 at 17
     # rows an expert 50 / 95, at 34 120 / 121.)
-    if st is not None and (M > FEW_ROWS if po is None else M > FEW_ROWS * w.G):
-        done = L.moe_gemm_q4_tc(x.data_ptr(), ldx, M, pc, ps, w.G, w.N, K, w.group, w.pair, out.data_ptr(), out.dtype is torch.bfloat16, ldo, pb, po,
-                                code, act_param, 1 if po is not None else _splits(M, N, w, place), st, core._stream())
+    few = M <= (FEW_ROWS if po is None else FEW_ROWS * w.G)
+    done = -1
+    for form in (few, not few):            # (what one does not take, -1, the other may)
+        if form:
+            done = L.moe_gemm_q4(x.data_ptr(), ldx, M, pc, ps, w.G, w.N, K, w.group, w.pair, out.data_ptr(), out.dtype is torch.bfloat16, ldo, pb, po,
+                                 code, act_param, st, core._stream())
+        else:
+            done = L.moe_gemm_q4_tc(x.data_ptr(), ldx, M, pc, ps, w.G, w.N, K, w.group, w.pair, out.data_ptr(), out.dtype is torch.bfloat16, ldo, pb,
+                                    po, code, act_param, 1 if po is not None else _splits(M, N, w, place), st, core._stream())
         if done != -1:
             core._ok(done, "gemm4")
             return out
-    done = L.moe_gemm_q4(x.data_ptr(), ldx, M, pc, ps, w.G, w.N, K, w.group, w.pair, out.data_ptr(), out.dtype is torch.bfloat16, ldo, pb, po, code,
-                         act_param, st, core._stream())
-    if done == -1:
-        raise core.KernelError("gemm4: more than 1,024 weights in a stack, or K too large for one")
-    core._ok(done, "gemm4")
-    return out
+    raise core.KernelError("gemm4: a stack of more than 1,024 weights, or one of K beyond 7,000 or so with rows that are no whole 16-byte units")
 
 
 def _splits(M: int, N: int, w: Weight4, place: int) -> int:
