@@ -178,11 +178,12 @@ __device__ __forceinline__ void put(const Args& p, int row, int n, float y) {
 
 // ---- few strips -----------------------------------------------------------------------------------------------------------------------------
 // Grid: strips of the output (of a pair: of one half).  Warp w takes blocks w, w + 8, ... of 64 k, DEPTH of them in flight; the codes are asked for
-// before the wait on the predecessor, the rows behind it.
+// before the wait on the predecessor, the rows behind it and one block ahead.  (All four ahead cost registers: two blocks an SM instead of three,
+// us, 8 rows of 6,144 x 2,048 6.3 / 3.6, of a pair 11,264 x 2,048 6.7 / 4.8, of 2,048 x 5,632 4.8 / 5.6.)
 template <int MT, int NT, int GROUP>
-__global__ void __launch_bounds__(256, NT == 1 ? 2 : 1)
+__global__ void __launch_bounds__(256, NT == 1 ? 3 : 2)
 gemm_q4_direct_kernel(const __grid_constant__ Args p) {
-    constexpr int W = 8, DEPTH = NT == 1 ? 4 : 2, NS = q4::Scales<GROUP>::N;
+    constexpr int W = 8, DEPTH = 4, NS = q4::Scales<GROUP>::N;
     __shared__ float red[W * MT * 8 * 17];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3, strip = blockIdx.x, blocks = p.w.blocks;
     const uint4* codes[MT];
@@ -197,7 +198,7 @@ gemm_q4_direct_kernel(const __grid_constant__ Args p) {
     for (int row0 = 0; row0 < p.M; row0 += 8 * NT) {
         uint4 code[DEPTH][MT];
         uint32_t sc[DEPTH][MT][NS];
-        uint2 x[DEPTH][NT][4];
+        uint2 x[NT][4];                                  // one block ahead
         const __nv_bfloat16* xr[NT];
 #pragma unroll
         for (int n = 0; n < NT; n++) xr[n] = row0 + 8 * n + r < p.M ? p.x + (size_t)(row0 + 8 * n + r) * p.ldx : nullptr;
@@ -213,11 +214,11 @@ gemm_q4_direct_kernel(const __grid_constant__ Args p) {
                 for (int i = 0; i < NS; i++) sc[d][m][i] = s.s[i];
             }
         };
-        auto ask_rows = [&](int d, int b) {
+        auto ask_rows = [&](int b) {
 #pragma unroll
             for (int n = 0; n < NT; n++)
 #pragma unroll
-                for (int j = 0; j < 4; j++) x[d][n][j] = row4(xr[n], b * 64 + 16 * j + 4 * t, p.w.K, p.vec);
+                for (int j = 0; j < 4; j++) x[n][j] = row4(xr[n], b * 64 + 16 * j + 4 * t, p.w.K, p.vec);
         };
         float acc[MT][NT][4];
 #pragma unroll
@@ -229,16 +230,15 @@ gemm_q4_direct_kernel(const __grid_constant__ Args p) {
             if (warp + d * W < blocks) ask(d, warp + d * W);
         if (!waited) pdl_sync();
         waited = true;
-#pragma unroll
-        for (int d = 0; d < DEPTH; d++)
-            if (warp + d * W < blocks) ask_rows(d, warp + d * W);
+        if (warp < blocks) ask_rows(warp);
         for (int b0 = warp; b0 < blocks; b0 += DEPTH * W) {
 #pragma unroll
             for (int d = 0; d < DEPTH; d++) {
                 const int b = b0 + d * W;
                 if (b >= blocks) break;
-                block_product<MT, NT, GROUP>(code[d], sc[d], x[d], p.bits, acc);
-                if (b + DEPTH * W < blocks) ask(d, b + DEPTH * W), ask_rows(d, b + DEPTH * W);
+                block_product<MT, NT, GROUP>(code[d], sc[d], x, p.bits, acc);
+                if (b + W < blocks) ask_rows(b + W);
+                if (b + DEPTH * W < blocks) ask(d, b + DEPTH * W);
             }
         }
 #pragma unroll
@@ -264,12 +264,12 @@ gemm_q4_direct_kernel(const __grid_constant__ Args p) {
 //         that nothing is gathered; the shared expert's strips come first.  What comes out lies as the B fragments of the next
 //         product, as two bfloat16 terms (rounded to one, the layer's output would be as far off again as its own rounding).
 //
-// A unit is two strips (a pair's gate and up strip, or neighbours) and up to 8 NT rows.  A block takes a run of neighbouring units; its four teams of
+// A unit is two strips (a pair's gate and up strip, or neighbours) and up to 8 NT rows.  A block takes a run of neighbouring units; its five teams of
 // four warps take them in turn, and the warps of a team every fourth block of 64 k.  One more warp a team has its codes copied (cp.async.bulk) into
 // stages of KC blocks, across the borders of units.  The fragments of the rows lie in shared memory for all teams; where the
 // rows change (GROUPED), all teams meet.
 enum { DENSE = 0, GROUPED = 1, EXPERTS = 2 };
-constexpr int GROUPS_MAX = 1024, TEAM_W = 4, TEAMS = 4, KC = 8, STREAM_THREADS = TEAMS * (TEAM_W + 1) * 32, STAGES_MAX = 8;
+constexpr int GROUPS_MAX = 1024, TEAM_W = 4, TEAMS = 5, KC = 8, STREAM_THREADS = TEAMS * (TEAM_W + 1) * 32, STAGES_MAX = 8;
 
 template <int NT, int GROUP>
 struct Stream {
@@ -701,11 +701,6 @@ Weight weight(const void* codes, const void* scales, int N, int K, int group, in
     return w;
 }
 
-int sm_count() {
-    int dev = 0, n = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
-    return n;
-}
 
 // Stages of a team beside the fragments of the rows: 0 where there is no room for two.
 template <int MODE, int NT, int GROUP>
@@ -720,9 +715,9 @@ template <int MODE, int NT, int GROUP, bool PAIR>
 int launch_stream(const Args& p, long long max_units, cudaStream_t stream) {
     const int stages = stream_stages<MODE, NT, GROUP>(p.w.blocks), bytes = Stream<NT, GROUP>::bytes(p.w.blocks, stages);
     auto kernel = gemm_q4_stream_kernel<MODE, NT, GROUP, PAIR>;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e != cudaSuccess) return (int)e;
-    const int sms = sm_count();
+    static q4::SmemLimit limit;
+    if (const int e = limit.lift((const void*)kernel)) return e;
+    const int sms = q4::sm_count();
     return launch_pdl(kernel, dim3((unsigned)(max_units < sms ? max_units : sms)), dim3(STREAM_THREADS), (size_t)bytes, stream, p, stages);
 }
 
@@ -737,7 +732,7 @@ int run_gemm(const Args& p, bool pair, cudaStream_t stream) {
     }
     const bool two = p.M > 8;
     const long long units = pair ? half : (half + 1) / 2;
-    if (p.M <= (two ? 16 : 8) && units >= 4 * sm_count() && (two ? stream_stages<DENSE, 2, GROUP>(p.w.blocks) : stream_stages<DENSE, 1, GROUP>(p.w.blocks)))
+    if (p.M <= (two ? 16 : 8) && units >= 4 * q4::sm_count() && (two ? stream_stages<DENSE, 2, GROUP>(p.w.blocks) : stream_stages<DENSE, 1, GROUP>(p.w.blocks)))
         return pair ? (two ? launch_stream<DENSE, 2, GROUP, true>(p, units, stream) : launch_stream<DENSE, 1, GROUP, true>(p, units, stream))
                     : (two ? launch_stream<DENSE, 2, GROUP, false>(p, units, stream) : launch_stream<DENSE, 1, GROUP, false>(p, units, stream));
     const dim3 grid(half);
@@ -752,8 +747,8 @@ int run_experts(const Args& up, const DownArgs& down, cudaStream_t stream) {
     const long long units = slots * (up.w.strips / 2) + (up.shared.codes ? up.shared.strips / 2 : 0);
     int e = launch_stream<EXPERTS, 1, GROUP, true>(up, units, stream);
     if (e) return e;
-    e = (int)cudaFuncSetAttribute(experts_down_kernel<GROUP>, cudaFuncAttributeMaxDynamicSharedMemorySize, DownRing<GROUP>::BYTES);
-    if (e) return e;
+    static q4::SmemLimit limit;
+    if ((e = limit.lift((const void*)experts_down_kernel<GROUP>))) return e;
     return launch_pdl_cluster(experts_down_kernel<GROUP>, dim3((down.down.strips + DOWN_MT - 1) / DOWN_MT, 1, down.S), dim3(DOWN_THREADS),
                               (size_t)DownRing<GROUP>::BYTES, stream, down.S, down);
 }
@@ -812,7 +807,7 @@ MOE_API int moe_experts_q4(const void* x, int ldx, int T, int H, const int* idx,
     if (scratch_bytes < (slots * d.down.blocks + (shared + 63) / 64) * 2048) return (int)cudaErrorInvalidValue;
     d.frag = up.frag, d.sfrag = up.sfrag, d.bits = up.bits;
     d.T = T, d.H = H, d.E = E, d.top_k = top_k, d.idx = idx, d.wk = wk, d.gate = gate, d.out = out, d.out_bf16 = out_bf16, d.ldo = ldo;
-    d.S = max(1, min(8, sm_count() / ((d.down.strips + DOWN_MT - 1) / DOWN_MT)));      // one block an SM
+    d.S = max(1, min(8, q4::sm_count() / ((d.down.strips + DOWN_MT - 1) / DOWN_MT)));      // one block an SM
 #define GO(GR) run_experts<GR>(up, d, stream)
     BY_GROUP(GO);
 #undef GO

@@ -464,9 +464,8 @@ int g_test_fault = 0;
 
 template <int GROUP, bool PAIR>
 int launch(const CUtensorMap& map, const Args& p, unsigned ctas, cudaStream_t stream) {
-    // (the attribute belongs to a device's copy of the kernel: set per launch it costs a fraction of a microsecond and is right on every device)
-    const cudaError_t e = cudaFuncSetAttribute(gemm_q4_tc_kernel<GROUP, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, p.stages * p.stage_bytes + 1024);
-    if (e != cudaSuccess) return (int)e;
+    static q4::SmemLimit limit;
+    if (const int e = limit.lift((const void*)gemm_q4_tc_kernel<GROUP, PAIR>)) return e;
     return launch_pdl_cluster(gemm_q4_tc_kernel<GROUP, PAIR>, dim3(ctas, 1, p.splits), dim3(THREADS), (size_t)(p.stages * p.stage_bytes + 1024), stream, p.splits, map, p);
 }
 
@@ -499,10 +498,7 @@ MOE_API int moe_gemm_q4_tc(const void* x, int ldx, int M, const void* codes, con
     p.bn = offsets ? min(BN, (mean * 3 / 2 + BOX - 1) / BOX * BOX) : ((M + mt - 1) / mt + 15) / 16 * 16;
     p.stage_bytes = A_BYTES + (p.bn + BOX - 1) / BOX * BOX_BYTES;
     p.stages = min(STAGES_MAX, ROOM / p.stage_bytes);
-    int dev = 0, sms = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    if (e != cudaSuccess) return (int)e;
+    const int sms = q4::sm_count();
     const long long tiles = (offsets ? (long long)(M < G ? M : G) + M / p.bn : (long long)((M + p.bn - 1) / p.bn)) * p.n_tiles;
     if (tiles > 0x3fffffff) return -1;
     if (offsets || splits < 1) splits = 1;

@@ -124,6 +124,39 @@ struct Waits {
     int test_fault;
 };
 
+// ---- host -------------------------------------------------------------------------------------------------------------------------------
+constexpr int DEVICES = 64;
+inline int device() {
+    int d = 0;
+    return cudaGetDevice(&d) == cudaSuccess && d >= 0 && d < DEVICES ? d : DEVICES;
+}
+// SMs of the current device
+inline int sm_count() {
+    static int known[DEVICES + 1];
+    const int d = device();
+    if (!known[d]) {
+        int n = 0;
+        known[d] = d < DEVICES && cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, d) == cudaSuccess ? n : 148;
+    }
+    return known[d];
+}
+// Lets a kernel have all the dynamic shared memory that a block may have, once a device (each has its own copy of the kernel; two threads that come first
+// set the same).
+struct SmemLimit {
+    bool done[DEVICES + 1] = {};
+    int lift(const void* kernel) {
+        const int d = device();
+        if (d < DEVICES && done[d]) return 0;
+        int most = 0;
+        cudaFuncAttributes a;
+        cudaError_t e = cudaDeviceGetAttribute(&most, cudaDevAttrMaxSharedMemoryPerBlockOptin, d);
+        if (e == cudaSuccess) e = cudaFuncGetAttributes(&a, kernel);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most - (int)a.sharedSizeBytes);
+        if (e == cudaSuccess) done[d] = true;
+        return (int)e;
+    }
+};
+
 void few_rows_wait_test(int fault, uint32_t wait_limit);      // gemm_q4.cu
 
 }  // namespace q4
