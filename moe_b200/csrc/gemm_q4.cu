@@ -495,8 +495,8 @@ gemm_q4_stream_kernel(const __grid_constant__ Args p, const int stages) {
                     team_sync<TEAM_W * 32>(team + 1);
                 if (!ok) s_abort = 1;
 #pragma unroll
-                for (int m = 0; m < UM; m++) {
-                    const int i = tw * 32 + lane, col = i >> 4, f = i & 15, n = (v.strip + m) * 16 + f;
+                for (int o = 0; o < UM * 128; o += TEAM_W * 32) {
+                    const int m = o >> 7, i = (o & 127) + tw * 32 + lane, col = i >> 4, f = i & 15, n = (v.strip + m) * 16 + f;
                     if (MODE == EXPERTS) {
                         const bool takes = col < p.M && (v.slot < 0 || ((picked.takes[v.slot] >> col) & 1));
                         float a = 0.f;

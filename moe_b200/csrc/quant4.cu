@@ -13,9 +13,9 @@
 
 namespace {
 
-template <typename T>
+template <typename T, bool FULL>
 __device__ __forceinline__ void load4(const T* row, int k, int K, bool vec, float (&v)[4]) {
-    if (vec && k + 4 <= K) {
+    if (FULL || (vec && k + 4 <= K)) {
         if constexpr (sizeof(T) == 2) {
             const uint2 u = __ldg(reinterpret_cast<const uint2*>(row + k));
             v[0] = __uint_as_float(u.x << 16), v[1] = __uint_as_float(u.x & 0xffff0000u);
@@ -26,8 +26,9 @@ __device__ __forceinline__ void load4(const T* row, int k, int K, bool vec, floa
         }
         return;
     }
+    if constexpr (!FULL)
 #pragma unroll
-    for (int i = 0; i < 4; i++) v[i] = k + i < K ? ld_f(row + k + i) : 0.f;
+        for (int i = 0; i < 4; i++) v[i] = k + i < K ? ld_f(row + k + i) : 0.f;
 }
 
 // max / 7 to five significant bits; 0 for what is held as zeros, NaN for what is no number
@@ -60,44 +61,55 @@ __device__ __forceinline__ uint32_t code_of(float w, float s, float rs) {
     return (uint32_t)((int)q + 8);
 }
 
-__device__ __forceinline__ bool row_of(int strip, int r, int strips, int N, int pair, int* row) {
-    const int half = pair ? N / 2 : N, per = pair ? strips / 2 : strips;
-    const int h = strip / per, in = (strip - h * per) * q4::STRIP + r;
+// One weight's sizes, and how a block's eight warps lie: 1 << kw of them beside one another in k (units of one strip), the others in further strips.
+// Grid: (units in k, strips, groups); the latter two in rounds where there are more than a grid has.
+struct Shape {
+    int G, N, K, pair, strips, blocks, qgroups, units, kw;
+};
+__device__ __forceinline__ bool row_of(const Shape& p, int strip, int r, int* row) {
+    const int half = p.pair ? p.N / 2 : p.N, per = p.pair ? p.strips / 2 : p.strips;
+    const int h = strip >= per ? 1 : 0, in = (strip - h * per) * q4::STRIP + r;
     *row = h * half + in;
     return in < half;
 }
+Shape shape_of(int G, int N, int K, int group, int pair, int span) {
+    Shape s = {G, N, K, pair};
+    s.strips = ((pair ? N / 2 : N) + 15) / 16 * (pair ? 2 : 1), s.blocks = (K + 63) / 64, s.qgroups = (K + group - 1) / group;
+    s.units = (s.blocks + span - 1) / span;
+    while (s.kw < 3 && (1 << s.kw) < s.units) s.kw++;
+    return s;
+}
+dim3 grid_of(const Shape& s) {
+    const int across = 8 >> s.kw, y = (s.strips + across - 1) / across;
+    return dim3((unsigned)((s.units + (1 << s.kw) - 1) >> s.kw), (unsigned)(y < 65535 ? y : 65535), (unsigned)(s.G < 65535 ? s.G : 65535));
+}
 
-template <typename T, int GROUP>
-__global__ void __launch_bounds__(256)
-quantize_kernel(const T* __restrict__ w, int N, int K, int pair, int strips, int blocks, int qgroups, int vec, long long units, uint4* __restrict__ codes,
-                uint32_t* __restrict__ scales, int* status) {
+// FULL: whole strips and units, rows of whole 16-byte units: no check at a load
+template <typename T, int GROUP, bool FULL>
+__device__ __forceinline__ void quantize_unit(const T* __restrict__ w, const Shape& p, int g0, int strip, int u, int vec, uint4* __restrict__ codes,
+                                              uint32_t* __restrict__ scales, int* status) {
     constexpr int SPAN = GROUP == 128 ? 2 : 1;                            // blocks of a unit
-    pdl_sync();
-    const int lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
-    const int per_strip = (blocks + SPAN - 1) / SPAN;
-    const long long unit = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-    if (unit >= units) return;
-    const long long gs = unit / per_strip;                                // group and strip
-    const int u = (int)(unit - gs * per_strip), strip = (int)(gs % strips);
-    const T* wg = w + (size_t)(gs / strips) * N * K;
+    const int lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3, K = p.K, blocks = p.blocks, qgroups = p.qgroups;
+    const size_t gs = (size_t)g0 * p.strips + strip;
+    const T* wg = w + (size_t)g0 * p.N * K;
     float v[2][SPAN][16];
 #pragma unroll
     for (int half = 0; half < 2; half++) {
         int row;
-        const bool live = row_of(strip, r + 8 * half, strips, N, pair, &row);
-        const T* p = wg + (size_t)(live ? row : 0) * K;
+        const bool live = row_of(p, strip, r + 8 * half, &row) || FULL;
+        const T* p_row = wg + (size_t)(live ? row : 0) * K;
 #pragma unroll
         for (int b = 0; b < SPAN; b++)
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 float x[4];
-                load4(p, live ? (u * SPAN + b) * 64 + 16 * j + 4 * t : K, K, vec, x);
+                load4<T, FULL>(p_row, live ? (u * SPAN + b) * 64 + 16 * j + 4 * t : K, K, vec, x);
 #pragma unroll
                 for (int i = 0; i < 4; i++) v[half][b][4 * j + i] = x[i];
             }
     }
     constexpr int SETS = GROUP == 32 ? 2 : 1, PER = 16 * SPAN / SETS;     // scales of a unit and row, elements of this lane under one
-    float s[2][SETS], rs[2][SETS];
+    float s[2][SETS], rs[2][SETS], sq[2][SETS];
     bool bad = false;
 #pragma unroll
     for (int half = 0; half < 2; half++)
@@ -110,7 +122,8 @@ quantize_kernel(const T* __restrict__ w, int N, int K, int pair, int strips, int
             m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
             s[half][g] = scale_of<T>(__uint_as_float(m));
             bad = bad || s[half][g] != s[half][g];
-            rs[half][g] = s[half][g] > 0.f ? 1.f / s[half][g] : 0.f;
+            // (a group of zeros, or of no numbers: w * 0 for q, and no step)
+            rs[half][g] = s[half][g] > 0.f ? 1.f / s[half][g] : 0.f, sq[half][g] = s[half][g] > 0.f ? s[half][g] : 0.f;
         }
     if (bad && status) atomicOr(status, ST_NOT_FINITE);
     if (t == 0) {
@@ -118,7 +131,7 @@ quantize_kernel(const T* __restrict__ w, int N, int K, int pair, int strips, int
         for (int g = 0; g < SETS; g++) {
             const int q = GROUP == 32 ? 2 * u + g : u;
             if (q < qgroups)
-                scales[((size_t)gs * qgroups + q) * 8 + r] = (__float_as_uint(s[0][g]) >> 16) | (__float_as_uint(s[1][g]) & 0xffff0000u);
+                scales[(gs * qgroups + q) * 8 + r] = (__float_as_uint(s[0][g]) >> 16) | (__float_as_uint(s[1][g]) & 0xffff0000u);
         }
     }
 #pragma unroll
@@ -131,38 +144,40 @@ quantize_kernel(const T* __restrict__ w, int N, int K, int pair, int strips, int
             uint32_t o = 0;
 #pragma unroll
             for (int half = 0; half < 2; half++) {
-                if (!(rs[half][g] > 0.f)) {                               // zeros, or no numbers: q = 0
-                    o |= 0x88888888u & (0x0f0f0f0fu << (4 * half));
-                    continue;
-                }
 #pragma unroll
                 for (int i = 0; i < 4; i++) {                             // k 4 t + i: pair i / 2, place i % 2
                     const int at = 16 * (i & 1) + 8 * (i >> 1) + 4 * half;
-                    o |= (code_of<T>(v[half][b][4 * j + i], s[half][g], rs[half][g]) << at) & (15u << at);
+                    o |= (code_of<T>(v[half][b][4 * j + i], sq[half][g], rs[half][g]) << at) & (15u << at);
                 }
             }
             out[j] = o;
         }
-        codes[((size_t)gs * blocks + u * SPAN + b) * 32 + lane] = make_uint4(out[0], out[1], out[2], out[3]);
+        codes[(gs * blocks + u * SPAN + b) * 32 + lane] = make_uint4(out[0], out[1], out[2], out[3]);
     }
 }
 
-template <int GROUP>
+template <typename T, int GROUP, bool FULL>
 __global__ void __launch_bounds__(256)
-dequantize_kernel(const uint4* __restrict__ codes, const uint32_t* __restrict__ scales, int N, int K, int pair, int strips, int blocks, int qgroups,
-                  int vec, long long units, const q4::Bits bits, __nv_bfloat16* __restrict__ out) {
+quantize_kernel(const T* __restrict__ w, const Shape p, int vec, uint4* __restrict__ codes, uint32_t* __restrict__ scales, int* status) {
     pdl_sync();
-    const int lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
-    const long long unit = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-    if (unit >= units) return;
-    const long long gs = unit / blocks;
-    const int b = (int)(unit - gs * blocks), strip = (int)(gs % strips);
-    const uint4 c = __ldg(codes + (size_t)unit * 32 + lane);
+    const int warp = threadIdx.x >> 5, u = ((int)blockIdx.x << p.kw) + (warp & ((1 << p.kw) - 1));
+    if (u >= p.units) return;
+    for (int g = blockIdx.z; g < p.G; g += gridDim.z)
+        for (int strip = blockIdx.y * (8 >> p.kw) + (warp >> p.kw); strip < p.strips; strip += gridDim.y * (8 >> p.kw))
+            quantize_unit<T, GROUP, FULL>(w, p, g, strip, u, vec, codes, scales, status);
+}
+
+template <int GROUP>
+__device__ __forceinline__ void dequantize_unit(const uint4* __restrict__ codes, const uint32_t* __restrict__ scales, const Shape& p, int g0, int strip, int b,
+                                                int vec, const q4::Bits& bits, __nv_bfloat16* __restrict__ out) {
+    const int lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3, K = p.K;
+    const size_t gs = (size_t)g0 * p.strips + strip;
+    const uint4 c = __ldg(codes + (gs * p.blocks + b) * 32 + lane);
     q4::Scales<GROUP> sc;
-    sc.load(scales + (size_t)gs * qgroups * 8, b, qgroups, r);
-    __nv_bfloat16* og = out + (size_t)(gs / strips) * N * K;
+    sc.load(scales + gs * p.qgroups * 8, b, p.qgroups, r);
+    __nv_bfloat16* og = out + (size_t)g0 * p.N * K;
     int row[2];
-    const bool live[2] = {row_of(strip, r, strips, N, pair, &row[0]), row_of(strip, r + 8, strips, N, pair, &row[1])};
+    const bool live[2] = {row_of(p, strip, r, &row[0]), row_of(p, strip, r + 8, &row[1])};
 #pragma unroll
     for (int j = 0; j < 4; j++) {
         uint32_t a[4];
@@ -186,6 +201,17 @@ dequantize_kernel(const uint4* __restrict__ codes, const uint32_t* __restrict__ 
     }
 }
 
+template <int GROUP>
+__global__ void __launch_bounds__(256)
+dequantize_kernel(const uint4* __restrict__ codes, const uint32_t* __restrict__ scales, const Shape p, int vec, const q4::Bits bits, __nv_bfloat16* __restrict__ out) {
+    pdl_sync();
+    const int warp = threadIdx.x >> 5, u = ((int)blockIdx.x << p.kw) + (warp & ((1 << p.kw) - 1));
+    if (u >= p.units) return;
+    for (int g = blockIdx.z; g < p.G; g += gridDim.z)
+        for (int strip = blockIdx.y * (8 >> p.kw) + (warp >> p.kw); strip < p.strips; strip += gridDim.y * (8 >> p.kw))
+            dequantize_unit<GROUP>(codes, scales, p, g, strip, u, vec, bits, out);
+}
+
 }  // namespace
 
 #define BY_GROUP(CALL)            \
@@ -201,16 +227,13 @@ dequantize_kernel(const uint4* __restrict__ codes, const uint32_t* __restrict__ 
 MOE_API int moe_q4_quantize(const void* w, int w_dt, int G, int N, int K, int group, int pair, void* codes, void* scales, int* status, cudaStream_t stream) {
     if (G <= 0 || N <= 0 || K <= 0) return 0;
     if (!w || !codes || !scales || (pair && N % 2)) return (int)cudaErrorInvalidValue;
-    const int half = pair ? N / 2 : N, strips = (half + 15) / 16 * (pair ? 2 : 1), blocks = (K + 63) / 64, qgroups = (K + group - 1) / group;
-    const int span = group == 128 ? 2 : 1;
-    const long long units = (long long)G * strips * ((blocks + span - 1) / span), grid = (units + 7) / 8;
-    if (grid > 0x7fffffffll) return (int)cudaErrorInvalidValue;
+    const Shape s = shape_of(G, N, K, group > 0 ? group : 1, pair, group == 128 ? 2 : 1);
     const int vec = K % 4 == 0 && ((uintptr_t)w & 15) == 0;
-#define GO(GR)                                                                                                                                    \
-    (w_dt == DT_BF16 ? launch_pdl(quantize_kernel<__nv_bfloat16, GR>, (unsigned)grid, 256, 0, stream, (const __nv_bfloat16*)w, N, K, pair, strips, blocks, \
-                                  qgroups, vec, units, (uint4*)codes, (uint32_t*)scales, status)                                                  \
-                     : launch_pdl(quantize_kernel<float, GR>, (unsigned)grid, 256, 0, stream, (const float*)w, N, K, pair, strips, blocks, qgroups, vec,  \
-                                  units, (uint4*)codes, (uint32_t*)scales, status))
+    const bool full = vec && K % 128 == 0 && (pair ? N / 2 : N) % 16 == 0;
+    auto go = [&](auto kernel, auto* from) { return launch_pdl(kernel, grid_of(s), 256, 0, stream, from, s, vec, (uint4*)codes, (uint32_t*)scales, status); };
+#define GO(GR)                                                                                                                              \
+    (w_dt == DT_BF16 ? go(full ? quantize_kernel<__nv_bfloat16, GR, true> : quantize_kernel<__nv_bfloat16, GR, false>, (const __nv_bfloat16*)w) \
+                     : go(full ? quantize_kernel<float, GR, true> : quantize_kernel<float, GR, false>, (const float*)w))
     BY_GROUP(GO);
 #undef GO
 }
@@ -219,13 +242,9 @@ MOE_API int moe_q4_quantize(const void* w, int w_dt, int G, int N, int K, int gr
 MOE_API int moe_q4_dequantize(const void* codes, const void* scales, int G, int N, int K, int group, int pair, void* out, cudaStream_t stream) {
     if (G <= 0 || N <= 0 || K <= 0) return 0;
     if (!out || !codes || !scales || (pair && N % 2)) return (int)cudaErrorInvalidValue;
-    const int half = pair ? N / 2 : N, strips = (half + 15) / 16 * (pair ? 2 : 1), blocks = (K + 63) / 64, qgroups = (K + group - 1) / group;
-    const long long units = (long long)G * strips * blocks, grid = (units + 7) / 8;
-    if (grid > 0x7fffffffll) return (int)cudaErrorInvalidValue;
+    const Shape s = shape_of(G, N, K, group > 0 ? group : 1, pair, 1);
     const int vec = K % 4 == 0 && ((uintptr_t)out & 7) == 0;
-#define GO(GR)                                                                                                                             \
-    launch_pdl(dequantize_kernel<GR>, (unsigned)grid, 256, 0, stream, (const uint4*)codes, (const uint32_t*)scales, N, K, pair, strips, blocks, qgroups, \
-               vec, units, q4::bits(), (__nv_bfloat16*)out)
+#define GO(GR) launch_pdl(dequantize_kernel<GR>, grid_of(s), 256, 0, stream, (const uint4*)codes, (const uint32_t*)scales, s, vec, q4::bits(), (__nv_bfloat16*)out)
     BY_GROUP(GO);
 #undef GO
 }

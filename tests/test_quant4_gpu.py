@@ -48,7 +48,8 @@ def weight(quant, shape, group=64, pair=False, std=None, seed=0):
 # ------------------------------------------------------------------------------------------------ quantiser
 @pytest.mark.parametrize("group", [32, 64, 128])
 @pytest.mark.parametrize("dtype", [BF, torch.float32])
-@pytest.mark.parametrize("shape,pair", [((1, 1), False), ((16, 64), False), ((33, 130), False), ((3, 50, 333), False), ((2, 34, 96), True), ((62, 1000), True)])
+@pytest.mark.parametrize("shape,pair", [((1, 1), False), ((16, 64), False), ((33, 130), False), ((3, 50, 333), False), ((2, 34, 96), True), ((62, 1000), True),
+                                        ((32, 128), False), ((3, 48, 384), False), ((2, 64, 1152), True)])
 def test_values_are_the_plain_ones(quant, shape, pair, dtype, group):
     torch.manual_seed(shape[-1] + group)
     kinds = {
