@@ -292,7 +292,7 @@ gemm_q4_stream_kernel(const __grid_constant__ Args p, const int stages) {
     extern __shared__ __align__(128) uint8_t smem[];     // the teams' stages, the teams' sums, the rows' fragments [blocks][NT][2][32] x 16 bytes
     __shared__ int s_first[MODE == GROUPED ? GROUPS_MAX + 1 : 1], s_off[MODE == GROUPED ? GROUPS_MAX + 1 : 1];
     __shared__ Picked picked;
-    __shared__ __align__(8) unsigned long long s_bars[TEAMS][2][STAGES_MAX];
+    __shared__ __align__(8) unsigned long long s_bars[TEAMS][2][STAGES_MAX], s_ready;
     __shared__ volatile int s_abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int blocks = p.w.blocks, half = PAIR ? p.w.strips / 2 : p.w.strips, per = (half + UM - 1) / UM;      // units of a weight and row chunk
@@ -302,19 +302,28 @@ gemm_q4_stream_kernel(const __grid_constant__ Args p, const int stages) {
     }
     if (threadIdx.x == 0) {
         s_abort = 0;
+        q4::mbar_init(smem_u32(&s_ready), 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    int units, shared_units = 0;
-    if (MODE == DENSE)
-        units = per;
-    else {
-        pdl_sync();
-        if (MODE == EXPERTS) {
-            if (warp == 0) find_picked(p.idx, p.M, p.top_k, p.E, blockIdx.x == 0 ? p.waits.status : nullptr, picked, lane);
-            __syncthreads();
-            shared_units = p.shared.codes ? p.shared.strips / 2 : 0;
-            units = shared_units + picked.before[32] * per;
-        } else {
+    // This block's units [u0, u1).  EXPERTS: its part of the shared expert's strips, which is known (and copied) before the picks are, [0, n1), and then its part
+    // of the picked experts' from number ea on, [n1, u1).
+    auto part = [&](int units, int i) { return (int)((long long)units * i / gridDim.x); };
+    const int shared_units = MODE == EXPERTS && p.shared.codes ? p.shared.strips / 2 : 0, sa = part(shared_units, blockIdx.x), n1 = part(shared_units, blockIdx.x + 1) - sa;
+    int u0 = 0, u1 = n1, ea = 0;
+    // (with a unit a block or more of the picked experts, both parts together are as even as one part would be: a block whose first part was rounded up takes
+    // less in the second)
+    auto know_picks = [&]() {
+        const int units = picked.before[32] * per;
+        auto first = [&](int i) {
+            const long long over = units >= (int)gridDim.x ? (long long)shared_units * i % gridDim.x : 0;
+            return (int)(((long long)units * i + over) / gridDim.x);
+        };
+        ea = first(blockIdx.x), u1 = n1 + first(blockIdx.x + 1) - ea;
+    };
+    if (MODE != EXPERTS) {
+        int units = per;
+        if (MODE == GROUPED) {
+            pdl_sync();
             for (int i = threadIdx.x; i <= p.G; i += STREAM_THREADS) s_off[i] = min(p.M, max(0, p.offsets[i]));
             __syncthreads();
             if (warp == 0) {                             // row chunks of the groups before each
@@ -335,17 +344,17 @@ gemm_q4_stream_kernel(const __grid_constant__ Args p, const int stages) {
             __syncthreads();
             units = s_first[p.G] * per;
         }
+        u0 = part(units, blockIdx.x), u1 = part(units, blockIdx.x + 1);
     }
     __syncthreads();
-    const int u0 = (int)((long long)units * blockIdx.x / gridDim.x), u1 = (int)((long long)units * (blockIdx.x + 1) / gridDim.x);      // this block's units
     auto locate = [&](int u) {
         Unit v;
         v.g = 0, v.slot = 0;
         if (MODE == EXPERTS) {
-            if (u < shared_units)
-                v.slot = -1, v.strip = u;
+            if (u < n1)
+                v.slot = -1, v.strip = sa + u;
             else
-                u -= shared_units, v.slot = u / per, v.strip = u - v.slot * per, v.g = picked.expert[v.slot];
+                u += ea - n1, v.slot = u / per, v.strip = u - v.slot * per, v.g = picked.expert[v.slot];
         } else {
             const int c = u / per;
             v.strip = (u - c * per) * UM;
@@ -363,7 +372,7 @@ gemm_q4_stream_kernel(const __grid_constant__ Args p, const int stages) {
     // the unit TEAMS further on, u
     auto step = [&](Unit& v, int u) {
         v.strip += TEAMS * UM;
-        if (v.strip >= (MODE == EXPERTS && v.slot < 0 ? shared_units : half)) v = locate(u);
+        if (v.strip >= half || (MODE == EXPERTS && v.slot < 0)) v = locate(u);
     };
     // A run: units of the same rows.  GROUPED: a chunk's; else all.
     auto run_end = [&](int u) { return MODE == GROUPED ? min(u1, (u / per + 1) * per) : u1; };
@@ -371,15 +380,24 @@ gemm_q4_stream_kernel(const __grid_constant__ Args p, const int stages) {
 
     if (warp >= TEAMS * TEAM_W) {
         // ---- copies of team q ---------------------------------------------------------------------------------------------------------------
-        if (lane || u0 >= u1 || p.waits.test_fault == 1) return;
+        if (lane || p.waits.test_fault == 1) return;
         const int q = warp - TEAMS * TEAM_W;
-        int u = u0 + q, end = run_end(u0), s = 0, it = 0;
+        int u = u0 + q, end = u0 < u1 ? run_end(u0) : u0, s = 0, it = 0;
+        bool waits = MODE == EXPERTS;                    // for the picks
         uint32_t parity = 1;
         const uint32_t base = smem_u32(smem) + q * stages * S::STAGE, bars = smem_u32(&s_bars[q][0][0]);
         bool ok = true;
         while (ok) {
-            while (u >= end && end < u1) u = end + q, end = run_end(end);      // past its run: the team's first unit of the next one
-            if (u >= end) break;
+            if (MODE == GROUPED)
+                while (u >= end && end < u1) u = end + q, end = run_end(end);      // past its run: the team's first unit of the next one
+            if (u >= end) {
+                if (!waits) break;
+                waits = false;
+                if (!(ok = q4::mbar_wait(smem_u32(&s_ready), 0, &s_abort, p.waits.limit_us, p.waits.status, 0x63))) break;
+                know_picks();
+                end = u1;
+                continue;
+            }
             for (Unit v = locate(u); ok && u < end;) {
                 const Weight& w = MODE == EXPERTS && v.slot < 0 ? p.shared : p.w;
                 const size_t s0 = (size_t)v.g * w.strips + v.strip, s1 = PAIR ? s0 + w.strips / 2 : v.strip + 1 < half ? s0 + 1 : s0;
@@ -403,11 +421,9 @@ gemm_q4_stream_kernel(const __grid_constant__ Args p, const int stages) {
                 if (u < end) step(v, u);
             }
         }
-        if (!ok) {
-            s_abort = 1;
-            for (int i = max(0, it - stages); i < it; i++)      // copies in flight must land
-                q4::mbar_wait(bars + 8 * (i % stages), (i / stages) & 1, nullptr, p.waits.limit_us, p.waits.status, 0x62);
-        }
+        if (!ok) s_abort = 1;
+        for (int i = max(0, it - stages); i < it; i++)      // copies in flight must land before the block leaves
+            q4::mbar_wait(bars + 8 * (i % stages), (i / stages) & 1, nullptr, p.waits.limit_us, p.waits.status, 0x62);
         return;
     }
 
@@ -415,7 +431,14 @@ gemm_q4_stream_kernel(const __grid_constant__ Args p, const int stages) {
     const int team = warp / TEAM_W, tw = warp % TEAM_W, r = lane >> 2;
     const uint32_t base = smem_u32(smem) + team * stages * S::STAGE, xs = smem_u32(smem) + TEAMS * stages * S::STAGE + S::RED;
     float* red = reinterpret_cast<float*>(smem + TEAMS * stages * S::STAGE) + team * S::RED_BUFFERS * S::RED_FLOATS;
-    if (MODE == DENSE) pdl_sync();
+    if (MODE != GROUPED) pdl_sync();
+    if (MODE == EXPERTS) {
+        if (warp == 0) {
+            find_picked(p.idx, p.M, p.top_k, p.E, blockIdx.x == 0 ? p.waits.status : nullptr, picked, lane);
+            if (lane == 0) q4::mbar_arrive(smem_u32(&s_ready));
+        }
+        u1 = n1 + 1;                                     // (one run, staged below; how long it is is known behind the barrier there)
+    }
     int s = 0, turn = 0;
     uint32_t parity = 0;
     bool ok = true;
@@ -437,6 +460,7 @@ gemm_q4_stream_kernel(const __grid_constant__ Args p, const int stages) {
             for (int c = 0; c < 8 * NT; c++) sts8(xs + ((b * NT + (c >> 3)) * 2 + (j >> 1)) * 512 + ((c & 7) * 4 + tt) * 16 + (j & 1) * 8, y[c]);
         }
         team_sync<TEAMS * TEAM_W * 32>(TEAMS + 1);
+        if (MODE == EXPERTS) know_picks();
         const int end = run_end(first);
         Unit v;
         if (first + team < end) v = locate(first + team);
@@ -807,7 +831,9 @@ MOE_API int moe_experts_q4(const void* x, int ldx, int T, int H, const int* idx,
     if (scratch_bytes < (slots * d.down.blocks + (shared + 63) / 64) * 2048) return (int)cudaErrorInvalidValue;
     d.frag = up.frag, d.sfrag = up.sfrag, d.bits = up.bits;
     d.T = T, d.H = H, d.E = E, d.top_k = top_k, d.idx = idx, d.wk = wk, d.gate = gate, d.out = out, d.out_bf16 = out_bf16, d.ldo = ldo;
-    d.S = max(1, min(8, q4::sm_count() / ((d.down.strips + DOWN_MT - 1) / DOWN_MT)));      // one block an SM
+    // blocks of a cluster: one block an SM, but five blocks of 64 k a warp are done sooner than two cluster barriers
+    const long long most = slots * d.down.blocks + (shared > 0 ? d.shared.blocks : 0);
+    d.S = most <= 5 * DOWN_W ? 1 : max(1, min(8, q4::sm_count() / ((d.down.strips + DOWN_MT - 1) / DOWN_MT)));
 #define GO(GR) run_experts<GR>(up, d, stream)
     BY_GROUP(GO);
 #undef GO

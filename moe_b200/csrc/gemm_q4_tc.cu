@@ -351,12 +351,13 @@ gemm_q4_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant
                     if (++s == p.stages) s = 0, parity ^= 1;
                 }
             }
-            if (!ok && p.test_fault != 1) {
-                s_abort = 1;
-                // copies in flight must land: with the values never coming, the stages' barriers would not say so
-                for (int i = max(0, it - p.stages); i < it; i++)
+            // Copies in flight must land before the block leaves.  Where the values will not come any more, their arrivals are made up for.
+            if (!ok && p.test_fault != 1) s_abort = 1;
+            for (int i = max(0, it - p.stages); i < it; i++) {
+                if (!mbar_wait(full(i % p.stages), (i / p.stages) & 1, &s_abort, p, 0x52)) {
                     for (int w = 0; w < 4; w++) mbar_arrive(full(i % p.stages));
-                for (int i = max(0, it - p.stages); i < it; i++) mbar_wait(full(i % p.stages), (i / p.stages) & 1, nullptr, p, 0x52);
+                    mbar_wait(full(i % p.stages), (i / p.stages) & 1, nullptr, p, 0x52);
+                }
             }
         }
     } else {
