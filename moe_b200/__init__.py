@@ -53,6 +53,8 @@ def load_model(model_dir: str, dtype="bfloat16", device="cuda", weights=None, we
     spec = arch.model_spec(typed)
     model = DecoderModel(spec, SafetensorsStore(model_dir), Runtime(device, _dtype(dtype), _weight_group(weights, weight_group)))
     model.config = typed
+    if model.rt.weight_group:
+        model.rt.check()                 # a weight that is no number
     return model
 
 

@@ -749,8 +749,8 @@ template <int GROUP>
 int run_gemm(const Args& p, bool pair, cudaStream_t stream) {
     const int half = pair ? p.w.strips / 2 : p.w.strips;
     if (p.offsets) {
-        if (!stream_stages<GROUPED, 1, GROUP>(p.w.blocks)) return -1;
         const long long chunks = (long long)min(p.M, p.G) + p.M / 8;
+        if (!stream_stages<GROUPED, 1, GROUP>(p.w.blocks) || chunks * half > 0x3fffffff) return -1;
         if (pair) return launch_stream<GROUPED, 1, GROUP, true>(p, chunks * half, stream);
         return launch_stream<GROUPED, 1, GROUP, false>(p, chunks * ((half + 1) / 2), stream);
     }
@@ -792,7 +792,7 @@ int g_test_fault = 0;
 
 // x: [M, K] bfloat16, row pitch ldx; codes, scales: a weight of G groups of N rows (a pair's: both halves) and K columns; out: [M, N] (a pair:
 // [M, N / 2] act(gate) * up) float32 or bfloat16, row pitch ldo; offsets: null (G must be 1) or [G + 1], rows [offsets[g], offsets[g + 1]) meet group g.
-// Returns -1, with nothing launched, for more than 1,024 groups, or groups of rows that shared memory does not hold (K beyond 7,000 or so).
+// Returns -1, with nothing launched, for more than 1,024 groups, or groups of rows that shared memory does not hold (K beyond 5,500 or so).
 MOE_API int moe_gemm_q4(const void* x, int ldx, int M, const void* codes, const void* scales, int G, int N, int K, int group, int pair, void* out,
                         int out_bf16, int ldo, const float* bias, const int* offsets, int act, float act_param, int* status, cudaStream_t stream) {
     if (M <= 0 || N <= 0) return 0;
@@ -811,7 +811,7 @@ MOE_API int moe_gemm_q4(const void* x, int ldx, int M, const void* codes, const 
 // x: [T, H] bfloat16, row pitch ldx; idx, wk: [T, top_k]; gate: [T] or null; gu [E, 2 size, H] and sgu [2 shared, H] pairs, down [E, H, size], sdown
 // [H, shared]; shared 0: no shared expert; scratch: 2 KB for each 64 features of the experts that may be picked
 // (min(T top_k, E)) and of the shared one.  Returns -1 for what it does not take: more than 8 tokens, 1,024 experts or 128 picks, rows that shared
-// memory does not hold (H beyond 7,000 or so).
+// memory does not hold (H beyond 6,000 or so).
 MOE_API int moe_experts_q4(const void* x, int ldx, int T, int H, const int* idx, const float* wk, int top_k, int E, int size, const void* gu_codes,
                            const void* gu_scales, const void* down_codes, const void* down_scales, int shared, const void* sgu_codes,
                            const void* sgu_scales, const void* sdown_codes, const void* sdown_scales, const float* gate, int group, void* scratch,

@@ -129,8 +129,8 @@ def _matrix(t: torch.Tensor, place: int, name: str, wide: bool):
         raise core.KernelError(f"{name}: expected a matrix of bfloat16{' or float32' if wide else ''} on cuda:{place}, got {t.dtype} {tuple(t.shape)} on {t.device}")
     rows, columns = t.shape
     pitch, step = t.stride()
-    if (step != 1 and columns > 1) or (rows > 1 and pitch < columns):
-        raise core.KernelError(f"{name}: expected dense rows that do not overlap, got strides {t.stride()} of {tuple(t.shape)}")
+    if (step != 1 and columns > 1) or (rows > 1 and pitch < columns) or pitch > 0x7fffffff or rows > 0x7fffffff:
+        raise core.KernelError(f"{name}: expected dense rows that do not overlap, less than 2^31 elements apart, got strides {t.stride()} of {tuple(t.shape)}")
     return rows, columns, pitch
 
 
@@ -214,7 +214,7 @@ def gemm4(x: torch.Tensor, w: Weight4, out: torch.Tensor, *, swiglu: bool = Fals
         if done != -1:
             core._ok(done, "gemm4")
             return out
-    raise core.KernelError("gemm4: a stack of more than 1,024 weights, or one of K beyond 7,000 or so with rows that are no whole 16-byte units")
+    raise core.KernelError("gemm4: a stack of more than 1,024 weights, or one of K beyond 5,500 or so with rows that are no whole 16-byte units")
 
 
 def _splits(M: int, N: int, w: Weight4, place: int) -> int:
@@ -241,7 +241,7 @@ def experts4(x: torch.Tensor, topk_idx: torch.Tensor, topk_w: torch.Tensor, gate
     x: bfloat16 [T, H]; topk_idx int32 and topk_w float32 [T, k]; gate_up: a pair's stack [E, 2 I, H], down: [E, H, I]; the shared expert's two
     likewise without the stack, shared_gate float32 [T] (None: 1); out: float32 or bfloat16 [T, H].  An index of -1 is no pick
     (all of a row's: zeros but for the shared expert), any other outside [0, E) is reported through ``status`` and taken for none.  False, with
-    nothing launched, for more tokens, more than 1,024 experts or 128 picks, or rows that shared memory does not hold (H beyond 7,000 or so)."""
+    nothing launched, for more tokens, more than 1,024 experts or 128 picks, or rows that shared memory does not hold (H beyond 6,000 or so)."""
     place = x.get_device()
     _here(place, "experts4")
     T, H, ldx = _matrix(x, place, "x", False)

@@ -178,6 +178,19 @@ def test_a_row_that_is_no_number_keeps_to_itself(quant):
         Q.check_product(out[rest], x[rest], W[0])
 
 
+def test_a_product_right_behind_the_quantiser_of_its_weight(quant):
+    """Products ask for their weights before they wait for what is in front of them: the quantiser lets them in when all is written."""
+    torch.manual_seed(2)
+    ws = [torch.randn(2048, 1024, device=DEV).to(BF) * 2.0 ** -5 for _ in range(4)]
+    for M in (1, 40):
+        x, outs = torch.randn(M, 1024, device=DEV).to(BF), [torch.empty(M, 2048, device=DEV) for _ in ws]
+        for _ in range(20):
+            for w, out in zip(ws, outs):
+                quant.gemm4(x, quant.quantize(w), out)
+        for w, out in zip(ws, outs):
+            Q.check_product(out, x, quant.dequantize(quant.quantize(w)))
+
+
 # ------------------------------------------------------------------------------------------------ grouped products
 @pytest.mark.parametrize("rows", [[0, 3, 0, 0, 8, 9, 1, 0], [0] * 8, [17, 0, 40, 16, 1, 0, 100, 33], [300, 0, 1, 0, 0, 257, 64, 5], [0, 0, 0, 0, 0, 0, 0, 1]])
 @pytest.mark.parametrize("pair", [False, True])
@@ -349,6 +362,24 @@ def test_what_a_layer_does_not_take(quant):
                 dict(status=torch.zeros(4, dtype=torch.int32)), dict(topk_idx=idx[:2, :0], topk_w=w[:2, :0])):
         with pytest.raises(core.KernelError):
             quant.experts4(x, **{**ok, **bad})
+
+
+def test_rows_that_shared_memory_does_not_hold(quant):
+    """A layer so wide is left to the products one by one; a stack so long goes to the tensor core, or is refused where its rows are no whole units."""
+    from moe_b200.ops import core
+
+    (gu, _), (d, _) = weight(quant, (2, 32, 8000), 128, pair=True), weight(quant, (2, 8000, 16), 128)
+    idx, w = torch.zeros(2, 1, dtype=torch.int32, device=DEV), torch.ones(2, 1, device=DEV)
+    x, out = torch.randn(2, 8000, device=DEV).to(BF), torch.full((2, 8000), 7.0, device=DEV)
+    assert not quant.experts4(x, idx, w, gu, d, out) and bool((out == 7).all())
+    off = torch.tensor([0, 1, 2], dtype=torch.int32, device=DEV)
+    stack, W = weight(quant, (2, 24, 8000))
+    out = quant.gemm4(x, stack, torch.empty(2, 24, device=DEV), group_offsets=off)
+    for g in range(2):
+        Q.check_product(out[g:g + 1], x[g:g + 1], W[g])
+    odd, _ = weight(quant, (2, 24, 7999))
+    with pytest.raises(core.KernelError):
+        quant.gemm4(x[:, :7999], odd, torch.empty(2, 24, device=DEV), group_offsets=off)
 
 
 def test_refusals(quant):
