@@ -109,7 +109,7 @@ struct Picked {
     int before[EXPERTS_MAX / 32 + 1];      // picked experts below each word
     short pick[PAIRS_MAX];                 // the expert of a pair, -1 for none
     short expert[PAIRS_MAX];               // of a slot: the picked experts in order of their numbers
-    uint32_t takes[PAIRS_MAX];             // of a slot: the tokens that picked it
+    uint32_t takes[PAIRS_MAX + 1];         // of a slot: the tokens that picked it; behind the last slot: all, for the shared expert
     __device__ __forceinline__ int slot_of(int e) const { return before[e >> 5] + __popc(bits[e >> 5] & ((1u << (e & 31)) - 1)); }
 };
 // By one warp; the block's other threads read it behind a barrier.
@@ -146,6 +146,7 @@ __device__ __forceinline__ void find_picked(const int* idx, int T, int top_k, in
         s.expert[slot] = (short)e;
         atomicOr(&s.takes[slot], 1u << (i / top_k));
     }
+    if (lane == 0) s.takes[s.before[32]] = (1u << T) - 1;
     __syncwarp();
 }
 
@@ -337,9 +338,10 @@ gemm_q4_stream_kernel(const __grid_constant__ Args p, const int stages) {
                         if (lane >= o) upto += v;
                     }
                     if (g < p.G) s_first[g] = run + upto - n;
-                    run += __shfl_sync(0xffffffffu, upto, 31);
+                    run = min(run + __shfl_sync(0xffffffffu, upto, 31), 1 << 29);
                 }
-                if (lane == 0) s_first[p.G] = run;
+                // (offsets that do not ascend may give more than the launch was sized for: nothing is done then)
+                if (lane == 0) s_first[p.G] = run <= min(p.M, p.G) + p.M / (8 * NT) ? run : 0;
             }
             __syncthreads();
             units = s_first[p.G] * per;
@@ -548,7 +550,7 @@ gemm_q4_stream_kernel(const __grid_constant__ Args p, const int stages) {
 // ---- the down products of a layer of routed experts ---------------------------------------------------------------------------------------
 //   out_t = sum_e w_te Wd_e a_te + gate_t Wd_s a_t,  w_te the sum of t's weights for expert e
 // Four strips of the output go through ALL picked experts and the shared one, w_te on the sums of each block of 64 k: nothing is left to
-// combine.  Tokens that did not pick an expert meet it with the zeros that the first kernel left.  A block of 64 k of the rows is 2 KB: for each 16 k a
+// combine.  Tokens that did not pick an expert meet it with the zeros that the first kernel left, and its sums stay out of theirs (a scale may be NaN).  A block of 64 k of the rows is 2 KB: for each 16 k a
 // B fragment of 32 lanes x (four k rounded to bfloat16, what that left rounded likewise).  Grid: (fours of strips, 1, S); the S blocks of a unit are
 // a cluster and share its blocks of 64 k; the first of them adds their sums up in order.  A warp takes every sixteenth block and copies for itself
 // into a ring of its own (cp.async: its pieces of 512 bytes and less are too small for bulk copies, of which an SM issued one in ten to twenty cycles).
@@ -682,10 +684,11 @@ experts_down_kernel(const __grid_constant__ DownArgs p) {
                 }
         }
         const float2 w2 = *reinterpret_cast<const float2*>(&wt[now.slot][2 * t]);
+        const uint32_t takes = picked.takes[now.slot] >> (2 * t);
 #pragma unroll
         for (int m = 0; m < DOWN_MT; m++) {
-            acc[m][0] = fmaf(w2.x, sum[m][0], acc[m][0]), acc[m][1] = fmaf(w2.y, sum[m][1], acc[m][1]);
-            acc[m][2] = fmaf(w2.x, sum[m][2], acc[m][2]), acc[m][3] = fmaf(w2.y, sum[m][3], acc[m][3]);
+            if (takes & 1) acc[m][0] = fmaf(w2.x, sum[m][0], acc[m][0]), acc[m][2] = fmaf(w2.x, sum[m][2], acc[m][2]);
+            if (takes & 2) acc[m][1] = fmaf(w2.y, sum[m][1], acc[m][1]), acc[m][3] = fmaf(w2.y, sum[m][3], acc[m][3]);
         }
         __syncwarp();                                           // (all lanes have read the place)
         now.next(slots, nb);
@@ -724,7 +727,6 @@ Weight weight(const void* codes, const void* scales, int N, int K, int group, in
     w.strips = (half + 15) / 16 * (pair ? 2 : 1), w.blocks = (K + 63) / 64, w.qgroups = (K + group - 1) / group;
     return w;
 }
-
 
 // Stages of a team beside the fragments of the rows: 0 where there is no room for two.
 template <int MODE, int NT, int GROUP>

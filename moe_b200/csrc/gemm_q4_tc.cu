@@ -216,9 +216,10 @@ gemm_q4_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant
                     if (lane >= o) upto += v;
                 }
                 if (g < p.G) s_prefix[g] = run + upto - n;
-                run += __shfl_sync(0xffffffffu, upto, 31);
+                run = min(run + __shfl_sync(0xffffffffu, upto, 31), 1 << 29);
             }
-            if (lane == 0) s_prefix[p.G] = run;
+            // (offsets that do not ascend may give more than the host checked: nothing is done then)
+            if (lane == 0) s_prefix[p.G] = run <= min(p.M, p.G) + p.M / p.bn ? run : 0;
         }
     }
     tc_fence_before();

@@ -159,12 +159,13 @@ __device__ __forceinline__ void quantize_unit(const T* __restrict__ w, const Sha
 template <typename T, int GROUP, bool FULL>
 __global__ void __launch_bounds__(256)
 quantize_kernel(const T* __restrict__ w, const Shape p, int vec, uint4* __restrict__ codes, uint32_t* __restrict__ scales, int* status) {
-    pdl_wait();                          // (the successor is let in when all is written: products read their weights before they wait)
+    pdl_wait();                          // (the successor is let in when all is written and to be seen: products read their weights before they wait)
     const int warp = threadIdx.x >> 5, u = ((int)blockIdx.x << p.kw) + (warp & ((1 << p.kw) - 1));
     if (u >= p.units) return;
     for (int g = blockIdx.z; g < p.G; g += gridDim.z)
         for (int strip = blockIdx.y * (8 >> p.kw) + (warp >> p.kw); strip < p.strips; strip += gridDim.y * (8 >> p.kw))
             quantize_unit<T, GROUP, FULL>(w, p, g, strip, u, vec, codes, scales, status);
+    __threadfence();
 }
 
 template <int GROUP>
@@ -204,7 +205,7 @@ __device__ __forceinline__ void dequantize_unit(const uint4* __restrict__ codes,
 template <int GROUP>
 __global__ void __launch_bounds__(256)
 dequantize_kernel(const uint4* __restrict__ codes, const uint32_t* __restrict__ scales, const Shape p, int vec, const q4::Bits bits, __nv_bfloat16* __restrict__ out) {
-    pdl_wait();                          // (the successor is let in when all is written: products read their weights before they wait)
+    pdl_wait();
     const int warp = threadIdx.x >> 5, u = ((int)blockIdx.x << p.kw) + (warp & ((1 << p.kw) - 1));
     if (u >= p.units) return;
     for (int g = blockIdx.z; g < p.G; g += gridDim.z)

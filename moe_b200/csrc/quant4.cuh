@@ -7,8 +7,7 @@
 // Rows come in strips of 16, k in blocks of 64.  A block of a strip is 512 bytes of codes, 16 for each lane of a warp: lane 4 r + t
 // holds rows r and r + 8 at k = 16 j + 4 t + {0, 1, 2, 3} in its 32-bit word j.  Those are the A fragment of an m16n8k16 product whose
 // k are taken in the order of the fragment (the B operand's are permuted alike: a lane's four k of 16 are neighbours, one 8-byte
-// load), and the registers that a warp hands to tensor memory with tcgen05.st.16x256b.  Word j, low to high: four times 4 bits of the
-// first k of a pair (rows r, r + 8 at k 4 t; rows r, r + 8 at 4 t + 2), then the same of the second (4 t + 1, 4 t + 3), each q + 8.
+// load or store).  Word j, low to high: four times 4 bits of the first k of a pair (rows r, r + 8 at k 4 t; rows r, r + 8 at 4 t + 2), then the same of the second (4 t + 1, 4 t + 3), each q + 8.
 //   codes   [G][strips][ceil(K / 64)][32][16 bytes]
 //   scales  [G][strips][ceil(K / group)][8][2] bfloat16: rows r and r + 8 beside one another
 // Rows beyond N have scale 0, k beyond K q = 0.  A pair (gate rows and up rows, N / 2 each) fills whole strips with either half.
@@ -17,7 +16,7 @@
 
 namespace q4 {
 
-constexpr int STRIP = 16, BLOCK_K = 64, BLOCK_BYTES = 512;
+constexpr int STRIP = 16;
 
 struct Weight {
     const uint4* codes;            // [G][strips][blocks][32]
@@ -79,12 +78,6 @@ __device__ __forceinline__ void mbar_arrive(uint32_t bar) { asm volatile("mbarri
 __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
     uint32_t ok;
     asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
-    return ok != 0;
-}
-// the same without suspending the thread
-__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
     return ok != 0;
 }
 // false: the barrier did not complete within limit_us (the site is recorded), or another role of the block gave up

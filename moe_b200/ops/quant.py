@@ -25,6 +25,7 @@ import torch
 from . import build, core
 
 GROUPS = (32, 64, 128)
+SIZE_MAX = 1 << 30
 EXPERTS_TOKENS = 8            # tokens that ``experts4`` takes
 FEW_ROWS = 16                 # rows (of a group: on average) up to which a product streams its weights through registers
 
@@ -69,8 +70,8 @@ class Weight4:
             G, N, K = shape
         else:
             raise core.KernelError(f"Weight4: the shape is (N, K) or (G, N, K), not {tuple(shape)}")
-        if G < 1 or N < 1 or K < 1:
-            raise core.KernelError(f"Weight4: a shape without elements, {tuple(shape)}")
+        if min(G, N, K) < 1 or max(G, N, K) > SIZE_MAX:
+            raise core.KernelError(f"Weight4: sizes from 1 to 2^30, not {tuple(shape)}")
         if group not in GROUPS:
             raise core.KernelError(f"Weight4: the group is one of {GROUPS}, not {group}")
         if pair and N % 2:
@@ -129,8 +130,11 @@ def _matrix(t: torch.Tensor, place: int, name: str, wide: bool):
         raise core.KernelError(f"{name}: expected a matrix of bfloat16{' or float32' if wide else ''} on cuda:{place}, got {t.dtype} {tuple(t.shape)} on {t.device}")
     rows, columns = t.shape
     pitch, step = t.stride()
-    if (step != 1 and columns > 1) or (rows > 1 and pitch < columns) or pitch > 0x7fffffff or rows > 0x7fffffff:
-        raise core.KernelError(f"{name}: expected dense rows that do not overlap, less than 2^31 elements apart, got strides {t.stride()} of {tuple(t.shape)}")
+    if rows <= 1:                 # (whatever torch says of the pitch)
+        pitch = columns
+    if (step != 1 and columns > 1) or pitch < columns or pitch > 0x7fffffff or rows >= 1 << 28:
+        raise core.KernelError(f"{name}: expected less than 2^28 dense rows that do not overlap, less than 2^31 elements apart, got strides {t.stride()} of "
+                               f"{tuple(t.shape)}")
     return rows, columns, pitch
 
 
@@ -140,8 +144,8 @@ def quantize(w: torch.Tensor, group: int = 64, *, pair: bool = False, status=Non
     core._chk(w, "w")
     core._dt(w)
     _here(w.get_device(), "quantize")
-    if w.dim() not in (2, 3) or not w.numel():
-        raise core.KernelError(f"quantize: a matrix or a stack of matrices, not {tuple(w.shape)}")
+    if w.dim() not in (2, 3) or not w.numel() or max(w.shape) > SIZE_MAX:
+        raise core.KernelError(f"quantize: a matrix or a stack of matrices of sizes from 1 to 2^30, not {tuple(w.shape)}")
     if group not in GROUPS:
         raise core.KernelError(f"quantize: the group is one of {GROUPS}, not {group}")
     G, N, K = (1, *w.shape) if w.dim() == 2 else w.shape

@@ -45,6 +45,15 @@ def test_a_weight_of_the_wrong_parts_is_refused(change):
         quant.Weight4(codes, scales, shape, group, pair)
 
 
+def test_sizes_that_the_kernels_do_not_count_are_refused():
+    from moe_b200.ops import core, quant
+
+    empty = torch.zeros(0, dtype=torch.uint8), torch.zeros(0, dtype=torch.bfloat16)
+    for shape in ((1 << 31, 8), (8, (1 << 30) + 1), (1 << 31, 8, 8)):
+        with pytest.raises(core.KernelError, match="sizes"):
+            quant.Weight4(*empty, shape)
+
+
 def test_no_cpu_path():
     from moe_b200.ops import core, quant
 

@@ -222,6 +222,25 @@ def test_offsets_out_of_range_touch_nothing_else(quant):
         assert bool((guard[:32] == 7).all()) and bool((guard[32 + M:] == 7).all())
 
 
+def test_offsets_that_go_up_and_down_touch_nothing_else(quant):
+    w4, W = weight(quant, (6, 40, 64))
+    for M in (90, 700):
+        x, guard = torch.randn(M, 64, device=DEV).to(BF), torch.full((M + 64, 40), 7.0, device=DEV)
+        quant.gemm4(x, w4, guard[32:32 + M], group_offsets=torch.tensor([0, M, 0, M, 0, M, 1], dtype=torch.int32, device=DEV), status=status())
+        torch.cuda.synchronize()
+        assert bool((guard[:32] == 7).all()) and bool((guard[32 + M:] == 7).all())
+
+
+@pytest.mark.parametrize("pitch", [0, 3, 8004])
+def test_one_row_whatever_its_pitch(quant, pitch):
+    """torch may say anything of the pitch of a single row."""
+    (stack, W), off = weight(quant, (2, 24, 8000)), torch.tensor([0, 0, 1], dtype=torch.int32, device=DEV)
+    row = torch.randn(8000, device=DEV).to(BF)
+    x, room = row.as_strided((1, 8000), (pitch, 1)), torch.empty(24, device=DEV)
+    quant.gemm4(x, stack, room.as_strided((1, 24), (pitch, 1)), group_offsets=off)
+    Q.check_product(room.view(1, 24), row.view(1, -1), W[1])
+
+
 @pytest.mark.parametrize("G_,M", [(1, 40), (1000, 900), (300, 6000)])
 def test_one_group_and_very_many(quant, G_, M):
     torch.manual_seed(M)
@@ -344,6 +363,23 @@ def test_a_token_that_is_no_number_keeps_to_itself(quant):
     assert bool(out[1].isnan().all()) and bool(out[3].isnan().any())
     y, size_ = plain_layer(x[rest], idx[rest], w[rest], GU, D)
     check_layer(out[rest], y, size_)
+
+
+def test_an_expert_that_is_no_number_stays_with_the_tokens_that_picked_it(quant):
+    T, H, E, size = 4, 128, 5, 80
+    torch.manual_seed(6)
+    for where in ("gate", "down"):
+        wu, wd = torch.randn(E, 2 * size, H, device=DEV) * H ** -0.5, torch.randn(E, H, size, device=DEV) * size ** -0.5
+        (wu if where == "gate" else wd)[2, 3, 5] = float("nan")
+        gu, d = quant.quantize(wu.to(BF), pair=True), quant.quantize(wd.to(BF))
+        x = torch.randn(T, H, device=DEV).to(BF)
+        idx = torch.tensor([[0, 1], [2, 0], [3, 1], [4, 3]], dtype=torch.int32, device=DEV)
+        w, out = torch.rand(T, 2, device=DEV), torch.empty(T, H, device=DEV)
+        assert quant.experts4(x, idx, w, gu, d, out)
+        rest = [0, 2, 3]
+        assert bool(out[1, 3].isnan())
+        y, size_ = plain_layer(x[rest], idx[rest], w[rest], quant.dequantize(gu).double().nan_to_num(), quant.dequantize(d).double().nan_to_num())
+        check_layer(out[rest], y, size_)
 
 
 def test_what_a_layer_does_not_take(quant):
