@@ -45,6 +45,17 @@ __device__ __forceinline__ void unpack(uint32_t w, const Bits& k, uint32_t (&a)[
 __device__ __forceinline__ float scale_lo(uint32_t s) { return __uint_as_float(s << 16); }            // row r
 __device__ __forceinline__ float scale_hi(uint32_t s) { return __uint_as_float(s & 0xffff0000u); }    // row r + 8
 
+// a[i] *= the scale of its row, exactly
+__device__ __forceinline__ void scale(uint32_t (&a)[4], uint32_t s) {
+    const uint32_t lo = __byte_perm(s, 0, 0x1010), hi = __byte_perm(s, 0, 0x3232);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const uint32_t m = (i & 1) ? hi : lo;
+        const __nv_bfloat162 y = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&a[i]), *reinterpret_cast<const __nv_bfloat162*>(&m));
+        a[i] = *reinterpret_cast<const uint32_t*>(&y);
+    }
+}
+
 // D = A B + C of one 16 x 16 tile of weights and eight columns of tokens
 __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float c0, float c1, float c2, float c3) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"

@@ -222,6 +222,31 @@ def test_offsets_out_of_range_touch_nothing_else(quant):
         assert bool((guard[:32] == 7).all()) and bool((guard[32 + M:] == 7).all())
 
 
+@pytest.mark.parametrize("rows", [[40, 0, 17, 64, 1, 33, 128, 20], [129, 70, 128, 0, 90, 200, 100, 99], [150, 90, 200, 128, 110, 90, 140, 130]])
+@pytest.mark.parametrize("N,dtype", [(512, torch.float32), (300, BF), (72, BF), (511, torch.float32)])
+def test_groups_of_many_rows(quant, rows, N, dtype):
+    """Either tile of the tensor-core form, whole and not, rows of the output in whole units and not; with a bias and an activation."""
+    torch.manual_seed(N + len(rows))
+    off = [0]
+    for r in rows:
+        off.append(off[-1] + r)
+    M, K, offsets = off[-1], 328, torch.tensor(off, dtype=torch.int32, device=DEV)
+    x, bias = torch.randn(M, K, device=DEV).to(BF), torch.randn(N, device=DEV)
+    w4, W = weight(quant, (len(rows), N, K))
+    pair4, P = weight(quant, (len(rows), 2 * N, K), 32, pair=True, seed=1)
+    for odd in (0, 3):
+        big = torch.full((M, N + 8 + odd), 7.0, dtype=dtype, device=DEV)
+        out = big[:, odd:N + odd]
+        for kw in (dict(bias=bias), dict(bias=bias, act="relu2"), dict(swiglu=True)):
+            st = status()
+            quant.gemm4(x, pair4 if "swiglu" in kw else w4, out, group_offsets=offsets, status=st, **kw)
+            fine(st)
+            for g, r in enumerate(rows):
+                if r:
+                    Q.check_product(out[off[g]:off[g + 1]], x[off[g]:off[g + 1]], P[g] if "swiglu" in kw else W[g], **kw)
+            assert bool((big[:, :odd] == 7).all()) and bool((big[:, N + odd:] == 7).all())
+
+
 def test_offsets_that_go_up_and_down_touch_nothing_else(quant):
     w4, W = weight(quant, (6, 40, 64))
     for M in (90, 700):
@@ -564,6 +589,34 @@ def test_a_wait_that_runs_out_is_reported_and_leaves_the_gpu_in_order(quant, for
         run()
     fine(st)
     check()
+
+
+@pytest.mark.parametrize("fault", [1, 2, 3])
+def test_a_wait_of_groups_that_runs_out(quant, fault):
+    from moe_b200.ops import core
+
+    torch.manual_seed(2)
+    rows, K, N = [40, 90, 0, 128, 60], 640, 300
+    off = torch.tensor([0, 40, 130, 130, 258, 318], dtype=torch.int32, device=DEV)
+    w4, W = weight(quant, (5, N, K))
+    st, x, out = status(), torch.randn(318, K, device=DEV).to(BF), torch.empty(318, N, device=DEV)
+    L = quant.lib()
+    L.moe_q4_set_wait_test(fault, 2000)
+    try:
+        quant.gemm4(x, w4, out, group_offsets=off, status=st)
+        torch.cuda.synchronize()
+    finally:
+        L.moe_q4_set_wait_test(0, 0)
+    assert int(st[0]) & 8, "the wait that ran out was not reported"
+    with pytest.raises(core.KernelError, match="4-bit weights"):
+        core.check_status(st)
+    quant.gemm4(x, w4, out, group_offsets=off, status=st)
+    fine(st)
+    at = 0
+    for g, r in enumerate(rows):
+        if r:
+            Q.check_product(out[at:at + r], x[at:at + r], W[g])
+        at += r
 
 
 # ------------------------------------------------------------------------------------------------ models
