@@ -87,6 +87,22 @@ def test_what_is_no_number_is_reported_and_stays_in_its_group(quant):
     assert torch.equal(v[~bad].double(), Q.plain_values(clean, 64)[~bad])
 
 
+@pytest.mark.parametrize("dtype", [BF, torch.float32])
+def test_weights_that_begin_anywhere(quant, dtype):
+    room = torch.randn(3 * 48 * 128 + 1, device=DEV).to(dtype)
+    for at in (0, 1):
+        w = room[at:at + 3 * 48 * 128].view(3, 48, 128)
+        back = torch.full((3 * 48 * 128 + 2,), 7.0, dtype=BF, device=DEV)
+        got = quant.dequantize(quant.quantize(w), back[at:at + 3 * 48 * 128].view(3, 48, 128))
+        assert torch.equal(got.double(), Q.plain_values(w, 64))
+        assert bool((back[:at] == 7).all()) and bool((back[at + 3 * 48 * 128:] == 7).all())
+
+
+def test_more_matrices_than_a_grid_has_blocks(quant):
+    w = torch.randn(66000, 2, 8, device=DEV)
+    assert torch.equal(quant.dequantize(quant.quantize(w, 32, pair=True)).double(), Q.plain_values(w, 32))
+
+
 # ------------------------------------------------------------------------------------------------ dense products
 @pytest.mark.parametrize("K", [1, 5, 64, 70, 200, 1411, 2048])
 @pytest.mark.parametrize("M", [1, 3, 8, 9, 16])
