@@ -569,8 +569,8 @@ struct DownArgs {
 template <int GROUP>
 struct DownRing {
     static constexpr int SCALES = GROUP == 32 ? 64 : 32, X = DOWN_MT * (512 + SCALES), SLOT = X + 2048, BYTES = DOWN_W * DOWN_DEPTH * SLOT;
-    static constexpr int RED_FLOATS = DOWN_W * DOWN_MT * 8 * 17;   // lies over the rings, and the other blocks' sums behind it
-    static_assert(RED_FLOATS * 4 + 8 * DOWN_MT * 128 * 4 <= BYTES, "sums");
+    static_assert(DOWN_W * DOWN_MT * 8 * 17 * 4 <= BYTES && DOWN_THREADS == DOWN_MT * 128, "sums");  // they lie over the rings
+    static constexpr int PARTS = 7 * DOWN_MT * 128 * 4;             // the other blocks' sums, behind the rings
 };
 
 template <int GROUP>
@@ -582,6 +582,7 @@ experts_down_kernel(const __grid_constant__ DownArgs p) {
     __shared__ float wk[PAIRS_MAX];
     __shared__ __align__(16) float wt[PAIRS_MAX + 1][FEW];      // a slot's weight of each token; the last one's: the shared expert's gate
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3, strip0 = blockIdx.x * DOWN_MT, rank = blockIdx.z;
+    if (p.S > 1) cluster_arrive();                              // (waited for below: this block's memory may be written to)
     // The picks were written at least two kernels ago (this one's predecessor let it in behind its own wait): they, and the weights, are
     // read before the wait.
     const int pairs = p.T * p.top_k;
@@ -700,18 +701,15 @@ experts_down_kernel(const __grid_constant__ DownArgs p) {
         for (int m = 0; m < DOWN_MT; m++) leave_sums<DOWN_MT>(red, warp, lane, m, acc[m]);
     __syncthreads();
     const int i = threadIdx.x, m = i >> 7, col = (i >> 4) & 7, f = i & 15, n = (strip0 + m) * 16 + f;
-    const bool live = i < DOWN_MT * 128;
-    float y = live ? sum_of<DOWN_W, DOWN_MT>(red, m, col, f) : 0.f;
+    float y = sum_of<DOWN_W, DOWN_MT>(red, m, col, f);         // (a thread an output)
     if (p.S > 1) {
-        const uint32_t part = smem_u32(smem) + D::RED_FLOATS * 4;
-        cluster_sync_all();                                     // (the first block's rings are free)
-        if (rank && live) st_cluster_f32(mapa_cluster(part + (rank * DOWN_MT * 128 + i) * 4, 0), y);
+        cluster_wait();
+        if (rank) st_cluster_f32(mapa_cluster(smem_u32(smem) + D::BYTES + ((rank - 1) * DOWN_MT * 128 + i) * 4, 0), y);
         cluster_sync_all();
         if (rank) return;
-        if (live)
-            for (int k = 1; k < p.S; k++) y += reinterpret_cast<const float*>(smem)[D::RED_FLOATS + k * DOWN_MT * 128 + i];
+        for (int k = 0; k < p.S - 1; k++) y += reinterpret_cast<const float*>(smem + D::BYTES)[k * DOWN_MT * 128 + i];
     }
-    if (live && col < p.T && n < p.H) {
+    if (col < p.T && n < p.H) {
         if (p.out_bf16)
             ((__nv_bfloat16*)p.out)[(size_t)col * p.ldo + n] = __float2bfloat16_rn(y);
         else
@@ -776,7 +774,7 @@ int run_experts(const Args& up, const DownArgs& down, cudaStream_t stream) {
     static q4::SmemLimit limit;
     if ((e = limit.lift((const void*)experts_down_kernel<GROUP>))) return e;
     return launch_pdl_cluster(experts_down_kernel<GROUP>, dim3((down.down.strips + DOWN_MT - 1) / DOWN_MT, 1, down.S), dim3(DOWN_THREADS),
-                              (size_t)DownRing<GROUP>::BYTES, stream, down.S, down);
+                              (size_t)(DownRing<GROUP>::BYTES + (down.S > 1 ? DownRing<GROUP>::PARTS : 0)), stream, down.S, down);
 }
 
 uint32_t g_wait_limit = WAIT_LIMIT_US;
