@@ -153,11 +153,12 @@ def quantize(w: torch.Tensor, group: int = 64, *, pair: bool = False, status=Non
     if pair and N % 2:
         raise core.KernelError("quantize: a pair has as many gate rows as up rows")
     strips = _strips(N, pair)
-    codes = torch.empty((G, strips, -(-K // 64), 8, 4, 4, 2, 2), dtype=torch.uint8, device=w.device)
-    scales = torch.empty((G, strips, -(-K // group), 8, 2), dtype=torch.bfloat16, device=w.device)
-    core._ok(lib().moe_q4_quantize(w.data_ptr(), core._dt(w), G, N, K, group, 1 if pair else 0, codes.data_ptr(), scales.data_ptr(),
-                                   _on(status, w.get_device(), "status", torch.int32), core._stream()), "quantize")
-    return Weight4(codes, scales, tuple(w.shape), group, pair)
+    device = w.device                     # (a tensor of one dimension takes two thirds of the host time of one of eight)
+    codes = torch.empty(G * strips * -(-K // 64) * 512, dtype=torch.uint8, device=device)
+    scales = torch.empty(G * strips * -(-K // group) * 16, dtype=torch.bfloat16, device=device)
+    core._ok((_lib or lib()).moe_q4_quantize(w.data_ptr(), core._dt(w), G, N, K, group, pair, codes.data_ptr(), scales.data_ptr(),
+                                             _on(status, w.get_device(), "status", torch.int32), core._stream()), "quantize")
+    return Weight4(codes, scales, w.shape, group, pair)
 
 
 def dequantize(w: Weight4, out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -167,8 +168,8 @@ def dequantize(w: Weight4, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         out = torch.empty(w.shape, dtype=torch.bfloat16, device=w.device)
     elif tuple(out.shape) != w.shape:
         raise core.KernelError(f"dequantize: out is {tuple(out.shape)}, the weight {w.shape}")
-    core._ok(lib().moe_q4_dequantize(*w.pointers, w.G, w.N, w.K, w.group, 1 if w.pair else 0,
-                                     _on(out, w.place, "out", torch.bfloat16), core._stream()), "dequantize")
+    core._ok((_lib or lib()).moe_q4_dequantize(*w.pointers, w.G, w.N, w.K, w.group, w.pair, _on(out, w.place, "out", torch.bfloat16), core._stream()),
+             "dequantize")
     return out
 
 
