@@ -3,10 +3,10 @@
 //   y[m, n] = sum_k x[m, k] q[n, k] s[n, k / group] (+ b[n]), or act(gate) * up of a pair's two rows.
 //
 // What should bound them is the stream of codes, 0.53 bytes an element; what does is the issue slots and the logic unit: 6.5 TB/s are 46
-// elements a cycle and SM, and turning eight codes into fragments takes 11 instructions a lane.  So the weights are the A operand of m16n8k16 products straight from the registers that they come in (a shift,
-// a mask and a subtraction a pair of elements), a product takes eight rows of x for the price of one, and the scale is applied to the sums
-// of a group's k (up to four products from zero, then one multiply-add an output), which also keeps the sums in plain 32-bit additions but
-// for those 64.  The warps that share a strip's k add their sums up through shared memory in the order of the warps.
+// elements a cycle and SM, and turning eight codes into fragments takes 11 instructions a lane.  So the weights are the A operand of m16n8k16 products
+// straight from the registers that they come in (a shift, a mask and a subtraction a pair of elements), a product takes eight rows of x for the
+// price of one, and the scale is applied to the sums of a group's k (up to four products from zero, then one multiply-add an output), which also
+// keeps the sums in plain 32-bit additions but for those 64.  The warps that share a strip's k add their sums up through shared memory in the order of the warps.
 //
 //   gemm_q4_direct_kernel    few strips: a block of eight warps a strip, codes and rows straight to registers, all asked for at once.  8 rows of
 //                            6,144 x 2,048 3.8 us, 1 row of 2,048 x 2,048 2.5
