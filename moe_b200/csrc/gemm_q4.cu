@@ -42,12 +42,25 @@ __device__ __forceinline__ uint2 row4(const __nv_bfloat16* row, int k, int K, in
     return make_uint2(e[0] | (e[1] << 16), e[2] | (e[3] << 16));
 }
 
-// acc += 64 k of MT strips against NT tiles of eight rows (x[n][j]: the B registers of 16 k), the group's scale on the sums of its k.  The strips'
-// products alternate: one waits for itself.
+// acc += 64 k of MT strips against NT tiles of eight rows (x[n][j]: the B registers of 16 k), the group's scale on the sums of its k, or, for more than two
+// tiles, on the weights (q s is a bfloat16), which saves the registers of a group's sums.  The strips' products alternate: one waits for itself.
 template <int MT, int NT, int GROUP>
 __device__ __forceinline__ void block_product(const uint4 (&code)[MT], const uint32_t (&sc)[MT][q4::Scales<GROUP>::N], const uint2 (&x)[NT][4], const q4::Bits& bits,
                                               float (&acc)[MT][NT][4]) {
     constexpr int SETS = q4::Scales<GROUP>::N, WORDS = 4 / SETS;
+    if constexpr (NT > 2) {
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+#pragma unroll
+            for (int m = 0; m < MT; m++) {
+                uint32_t a[4];
+                q4::unpack(q4::word(code[m], j), bits, a);
+                q4::scale(a, sc[m][j / WORDS]);
+#pragma unroll
+                for (int n = 0; n < NT; n++) q4::mma(acc[m][n], a, x[n][j].x, x[n][j].y, acc[m][n][0], acc[m][n][1], acc[m][n][2], acc[m][n][3]);
+            }
+        return;
+    }
 #pragma unroll
     for (int h = 0; h < SETS; h++) {
         float c[MT][NT][4];
@@ -183,12 +196,13 @@ __device__ __forceinline__ void put(const Args& p, int row, int n, float y) {
 
 // ---- few strips -----------------------------------------------------------------------------------------------------------------------------
 // Grid: strips of the output (of a pair: of one half).  Warp w takes blocks w, w + 8, ... of 64 k, DEPTH of them in flight; the codes are asked for
-// before the wait on the predecessor, the rows behind it and one block ahead.  (All four ahead cost registers: two blocks an SM instead of three,
-// us, 8 rows of 6,144 x 2,048 6.3 / 3.6, of a pair 11,264 x 2,048 6.7 / 4.8, of 2,048 x 5,632 4.8 / 5.6.)
+// before the wait on the predecessor, the rows behind it and one block ahead.  Three blocks an SM count for more than anything that their registers
+// could hold.  (us, two / three: 8 rows of 6,144 x 2,048, with all four blocks' rows ahead in the first, 6.3 / 3.6, of a pair 11,264 x 2,048 6.7 / 4.8,
+// of 2,048 x 5,632 4.8 / 5.6; 16 rows 8.9 / 6.5, 10.6 / 8.7, 9.0 / 8.8; 24 rows 8.9 / 8.4, 14.7 / 12.5, 12.5 / 12.0.)
 template <int MT, int NT, int GROUP>
-__global__ void __launch_bounds__(256, NT == 1 ? 3 : 2)
+__global__ void __launch_bounds__(256, 3)
 gemm_q4_direct_kernel(const __grid_constant__ Args p) {
-    constexpr int W = 8, DEPTH = 4, NS = q4::Scales<GROUP>::N;
+    constexpr int W = 8, DEPTH = MT == 2 && NT > 1 ? 2 : 4, NS = q4::Scales<GROUP>::N;
     __shared__ float red[W * MT * 8 * 17];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3, strip = blockIdx.x, blocks = p.w.blocks;
     const uint4* codes[MT];
@@ -263,7 +277,7 @@ gemm_q4_direct_kernel(const __grid_constant__ Args p) {
 }
 
 // ---- many strips ----------------------------------------------------------------------------------------------------------------------------
-// DENSE   one weight, up to 8 NT rows
+// DENSE   one weight, up to 8 NT rows, NT 1 to 3
 // GROUPED rows [offsets[g], offsets[g + 1]) meet weight g, eight at a time
 // EXPERTS the gate and up rows of a layer of routed experts: the eight rows of a unit are the step's tokens whatever the expert, so
 //         that nothing is gathered; the shared expert's strips come first.  What comes out lies as the B fragments of the next
@@ -749,6 +763,21 @@ int launch_stream(const Args& p, long long max_units, cudaStream_t stream) {
     return launch_pdl(kernel, dim3((unsigned)(max_units < sms ? max_units : sms)), dim3(STREAM_THREADS), (size_t)bytes, stream, p, stages);
 }
 
+// One weight, 8 NT rows (24: any number, in passes).  Streamed where a block a strip does not fit the SMs at once, three each, or, above eight rows, where there are
+// 1.5 units an SM.  (us, a block a strip / streamed: 8 rows of 6,144 x 2,048, 384 blocks, 3.5 / 5.1, of 7,168 x 2,048, 448, 5.5 / 5.1, of 12,288 x 2,048
+// 6.9 / 6.0, of 8,192 x 5,632 16.7 / 10.6, of a pair 11,264 x 2,048, 352, 4.9 / 5.9, of a pair 14,336 x 2,048, 448, 7.4 / 6.7; 16 rows of 6,144 x 2,048, 192 units, 6.3 / 7.4,
+// of a pair 11,264 x 2,048, 352, 8.9 / 8.3; 24 rows of the two 8.6 / 8.8, 12.6 / 10.2.)
+template <int NT, int GROUP>
+int run_dense(const Args& p, bool pair, cudaStream_t stream) {
+    const int half = pair ? p.w.strips / 2 : p.w.strips;
+    const long long units = pair ? half : (half + 1) / 2;
+    const int sms = q4::sm_count();
+    if (p.M <= 8 * NT && (half > 3 * sms || (NT > 1 && 2 * units >= 3 * sms)) && stream_stages<DENSE, NT, GROUP>(p.w.blocks))
+        return pair ? launch_stream<DENSE, NT, GROUP, true>(p, units, stream) : launch_stream<DENSE, NT, GROUP, false>(p, units, stream);
+    return pair ? launch_pdl(gemm_q4_direct_kernel<2, NT, GROUP>, dim3(half), 256, 0, stream, p)
+                : launch_pdl(gemm_q4_direct_kernel<1, NT, GROUP>, dim3(half), 256, 0, stream, p);
+}
+
 template <int GROUP>
 int run_gemm(const Args& p, bool pair, cudaStream_t stream) {
     const int half = pair ? p.w.strips / 2 : p.w.strips;
@@ -758,14 +787,8 @@ int run_gemm(const Args& p, bool pair, cudaStream_t stream) {
         if (pair) return launch_stream<GROUPED, 1, GROUP, true>(p, chunks * half, stream);
         return launch_stream<GROUPED, 1, GROUP, false>(p, chunks * ((half + 1) / 2), stream);
     }
-    const bool two = p.M > 8;
-    const long long units = pair ? half : (half + 1) / 2;
-    if (p.M <= (two ? 16 : 8) && units >= 4 * q4::sm_count() && (two ? stream_stages<DENSE, 2, GROUP>(p.w.blocks) : stream_stages<DENSE, 1, GROUP>(p.w.blocks)))
-        return pair ? (two ? launch_stream<DENSE, 2, GROUP, true>(p, units, stream) : launch_stream<DENSE, 1, GROUP, true>(p, units, stream))
-                    : (two ? launch_stream<DENSE, 2, GROUP, false>(p, units, stream) : launch_stream<DENSE, 1, GROUP, false>(p, units, stream));
-    const dim3 grid(half);
-    return pair ? (two ? launch_pdl(gemm_q4_direct_kernel<2, 2, GROUP>, grid, 256, 0, stream, p) : launch_pdl(gemm_q4_direct_kernel<2, 1, GROUP>, grid, 256, 0, stream, p))
-                : (two ? launch_pdl(gemm_q4_direct_kernel<1, 2, GROUP>, grid, 256, 0, stream, p) : launch_pdl(gemm_q4_direct_kernel<1, 1, GROUP>, grid, 256, 0, stream, p));
+    if (p.M <= 8) return run_dense<1, GROUP>(p, pair, stream);
+    return p.M <= 16 ? run_dense<2, GROUP>(p, pair, stream) : run_dense<3, GROUP>(p, pair, stream);
 }
 
 template <int GROUP>

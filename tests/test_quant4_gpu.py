@@ -105,7 +105,7 @@ def test_more_matrices_than_a_grid_has_blocks(quant):
 
 # ------------------------------------------------------------------------------------------------ dense products
 @pytest.mark.parametrize("K", [1, 5, 64, 70, 200, 1411, 2048])
-@pytest.mark.parametrize("M", [1, 3, 8, 9, 16])
+@pytest.mark.parametrize("M", [1, 3, 8, 9, 16, 17, 20, 24])
 def test_few_rows(quant, M, K):
     torch.manual_seed(M * K)
     for i, (N, group, dtype) in enumerate([(1, 64, torch.float32), (50, 32, BF), (257, 128, torch.float32)]):
@@ -129,7 +129,7 @@ def test_more_rows(quant, M):
         Q.check_product(out, x, W[0], bias=bias)
 
 
-@pytest.mark.parametrize("M", [1, 8, 11, 40, 130, 300])
+@pytest.mark.parametrize("M", [1, 8, 11, 23, 40, 130, 300])
 @pytest.mark.parametrize("act,param", [("silu", 0.0), ("gelu_tanh", 0.0), ("clamped_sigmoid", 1.5)])
 def test_gated_pairs(quant, M, act, param):
     torch.manual_seed(M)
@@ -152,7 +152,8 @@ def test_activations_of_an_ungated_product(quant, M, act):
     Q.check_product(out, x, W[0], act=act)
 
 
-@pytest.mark.parametrize("M,N,K", [(1, 20000, 200), (7, 20000, 264), (12, 20000, 136), (16, 40000, 72), (8, 19000, 7040)])
+@pytest.mark.parametrize("M,N,K", [(1, 20000, 200), (7, 20000, 264), (12, 20000, 136), (16, 40000, 72), (8, 19000, 7040), (17, 7200, 1000), (24, 20000, 333),
+                                   (19, 7200, 5000)])
 def test_so_many_features_that_the_weights_are_streamed(quant, M, N, K):
     torch.manual_seed(K)
     for pair in (False, True):
