@@ -22,7 +22,7 @@ from typing import Optional, Tuple
 
 import torch
 
-from . import build, core
+from . import build, core, tc
 
 GROUPS = (32, 64, 128)
 SIZE_MAX = 1 << 30
@@ -30,6 +30,7 @@ EXPERTS_TOKENS = 8            # tokens that ``experts4`` takes
 FEW_ROWS = 24                 # rows up to which a product streams its weights through registers
 GROUP_FEW_ROWS = 14           # the same of groups, on average
 
+_U8, _BF16, _F32 = torch.uint8, torch.bfloat16, torch.float32
 _lib = None
 
 
@@ -66,24 +67,25 @@ class Weight4:
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, shape: Tuple[int, ...], group: int = 64, pair: bool = False):
         if len(shape) == 2:
-            G, (N, K) = 1, shape
+            G = 1
+            N, K = shape
         elif len(shape) == 3:
             G, N, K = shape
         else:
             raise core.KernelError(f"Weight4: the shape is (N, K) or (G, N, K), not {tuple(shape)}")
-        if min(G, N, K) < 1 or max(G, N, K) > SIZE_MAX:
+        if not (0 < G <= SIZE_MAX and 0 < N <= SIZE_MAX and 0 < K <= SIZE_MAX):
             raise core.KernelError(f"Weight4: sizes from 1 to 2^30, not {tuple(shape)}")
         if group not in GROUPS:
             raise core.KernelError(f"Weight4: the group is one of {GROUPS}, not {group}")
         if pair and N % 2:
             raise core.KernelError("Weight4: a pair has as many gate rows as up rows")
         strips = G * _strips(N, pair)
+        nc, ns = strips * ((K + 63) // 64) * 512, strips * ((K + group - 1) // group) * 16
         pc, ps, place = codes.data_ptr(), scales.data_ptr(), codes.get_device()
-        if (codes.dtype is not torch.uint8 or scales.dtype is not torch.bfloat16 or codes.numel() != strips * -(-K // 64) * 512
-                or scales.numel() != strips * -(-K // group) * 16 or not codes.is_contiguous() or not scales.is_contiguous()
-                or pc % 16 or ps % 16 or scales.get_device() != place):
+        if (codes.dtype is not _U8 or scales.dtype is not _BF16 or codes.numel() != nc or scales.numel() != ns or not codes.is_contiguous()
+                or not scales.is_contiguous() or (pc | ps) & 15 or scales.get_device() != place):
             raise core.KernelError(f"Weight4: codes and scales of {tuple(shape)} in groups of {group} are contiguous uint8 and bfloat16 tensors "
-                                   f"of {strips * -(-K // 64) * 512} and {strips * -(-K // group) * 16} elements on one device")
+                                   f"of {nc} and {ns} elements on one device")
         self.codes, self.scales, self.shape, self.group, self.pair = codes, scales, tuple(shape), group, bool(pair)
         self.G, self.N, self.K, self.place, self.pointers = G, N, K, place, (pc, ps)
 
@@ -105,7 +107,7 @@ class Weight4:
 
 
 def _strips(N: int, pair: bool) -> int:
-    return 2 * -(-(N // 2) // 16) if pair else -(-N // 16)
+    return (N // 2 + 15) // 16 * 2 if pair else (N + 15) // 16
 
 
 def _here(place: int, what: str):
@@ -127,7 +129,8 @@ def _on(t: Optional[torch.Tensor], place: int, name: str, dtype, numel: Optional
 
 def _matrix(t: torch.Tensor, place: int, name: str, wide: bool):
     """(rows, columns, row pitch) of a matrix with dense rows, bfloat16 or (``wide``) float32."""
-    if (t.dtype is not torch.bfloat16 and not (wide and t.dtype is torch.float32)) or t.get_device() != place or t.dim() != 2:
+    dtype = t.dtype
+    if (dtype is not _BF16 and not (wide and dtype is _F32)) or t.get_device() != place or t.dim() != 2:
         raise core.KernelError(f"{name}: expected a matrix of bfloat16{' or float32' if wide else ''} on cuda:{place}, got {t.dtype} {tuple(t.shape)} on {t.device}")
     rows, columns = t.shape
     pitch, step = t.stride()
@@ -198,8 +201,8 @@ def gemm4(x: torch.Tensor, w: Weight4, out: torch.Tensor, *, swiglu: bool = Fals
         code = core.PLAIN_ACTS.get(act, 0)
     if group_offsets is None and w.G != 1:
         raise core.KernelError("gemm4: a stack needs group_offsets")
-    pb = _on(bias, place, "bias", torch.float32, N)
-    po = _on(group_offsets, place, "group_offsets", torch.int32, w.G + 1)
+    pb = None if bias is None else _on(bias, place, "bias", _F32, N)
+    po = None if group_offsets is None else _on(group_offsets, place, "group_offsets", torch.int32, w.G + 1)
     st = _on(status, place, "status", torch.int32)
     if not M:
         return out
@@ -212,10 +215,10 @@ def gemm4(x: torch.Tensor, w: Weight4, out: torch.Tensor, *, swiglu: bool = Fals
     done = -1
     for form in (few, not few):            # (what one does not take, -1, the other may)
         if form:
-            done = L.moe_gemm_q4(x.data_ptr(), ldx, M, pc, ps, w.G, w.N, K, w.group, w.pair, out.data_ptr(), out.dtype is torch.bfloat16, ldo, pb, po,
+            done = L.moe_gemm_q4(x.data_ptr(), ldx, M, pc, ps, w.G, w.N, K, w.group, w.pair, out.data_ptr(), out.dtype is _BF16, ldo, pb, po,
                                  code, act_param, st, core._stream())
         else:
-            done = L.moe_gemm_q4_tc(x.data_ptr(), ldx, M, pc, ps, w.G, w.N, K, w.group, w.pair, out.data_ptr(), out.dtype is torch.bfloat16, ldo, pb,
+            done = L.moe_gemm_q4_tc(x.data_ptr(), ldx, M, pc, ps, w.G, w.N, K, w.group, w.pair, out.data_ptr(), out.dtype is _BF16, ldo, pb,
                                     po, code, act_param, 1 if po is not None else _splits(M, N, w, place), st, core._stream())
         if done != -1:
             core._ok(done, "gemm4")
@@ -228,8 +231,6 @@ def _splits(M: int, N: int, w: Weight4, place: int) -> int:
     of that size finds room for every tile at once, 4 blocks of 64 k and more each.  (us, none / 2 / 3 / 4 / 8: 113 rows of 2,048 x 5,632, 16 tiles, 34.8 /
     20.8 / - / 13.0 / 20.5; 32 rows of 6,144 x 2,048, 48 tiles, 13.4 / 10.4 / 16.6 / 14.8 / 26.2: clusters of three or eight leave SMs of a GPC unused,
     and what does not fit at once takes a second round.)"""
-    from . import tc
-
     tiles, sms, blocks = -(-M // 256) * -(-N // (64 if w.pair else 128)), tc.num_sms(place), -(-w.K // 64)
     for splits in (4, 2):
         if tiles * splits <= sms * 9 // 10 and blocks >= 4 * splits:
@@ -279,7 +280,7 @@ def experts4(x: torch.Tensor, topk_idx: torch.Tensor, topk_w: torch.Tensor, gate
     slots = min(T * k, E)
     scratch = torch.empty((slots * -(-size // 64) + -(-shared // 64)) * 2048, dtype=torch.uint8, device=x.device)
     code = L.moe_experts_q4(x.data_ptr(), ldx, T, H, pi, pw, k, E, size, *gate_up.pointers, *down.pointers, shared, *s, pg, group, scratch.data_ptr(),
-                            scratch.numel(), out.data_ptr(), out.dtype is torch.bfloat16, ldo, ps, core._stream())
+                            scratch.numel(), out.data_ptr(), out.dtype is _BF16, ldo, ps, core._stream())
     if code == -1:
         return False
     core._ok(code, "experts4")
