@@ -278,7 +278,7 @@ gemm_q4_direct_kernel(const __grid_constant__ Args p) {
 
 // ---- many strips ----------------------------------------------------------------------------------------------------------------------------
 // DENSE   one weight, up to 8 NT rows, NT 1 to 3
-// GROUPED rows [offsets[g], offsets[g + 1]) meet weight g, eight at a time
+// GROUPED rows [offsets[g], offsets[g + 1]) meet weight g, 8 NT at a time
 // EXPERTS the gate and up rows of a layer of routed experts: the eight rows of a unit are the step's tokens whatever the expert, so
 //         that nothing is gathered; the shared expert's strips come first.  What comes out lies as the B fragments of the next
 //         product, as two bfloat16 terms (rounded to one, the layer's output would be as far off again as its own rounding).
@@ -783,6 +783,11 @@ int run_gemm(const Args& p, bool pair, cudaStream_t stream) {
     const int half = pair ? p.w.strips / 2 : p.w.strips;
     if (p.offsets) {
         const long long chunks = (long long)min(p.M, p.G) + p.M / 8;
+        // Two tiles of rows at a time where groups have more than nine on average.  (us, one / two: 60 experts of a pair 2,816 x 2,048 at 8 rows an expert 61 / 63, at 10
+        // 73 / 65, at 14 90 / 79; of 2,048 x 1,408 39 / 40, 45 / 42, 55 / 50.)
+        if (p.M > 9 * p.G && stream_stages<GROUPED, 2, GROUP>(p.w.blocks) && chunks * half <= 0x3fffffff)
+            return pair ? launch_stream<GROUPED, 2, GROUP, true>(p, chunks * half, stream)
+                        : launch_stream<GROUPED, 2, GROUP, false>(p, chunks * ((half + 1) / 2), stream);
         if (!stream_stages<GROUPED, 1, GROUP>(p.w.blocks) || chunks * half > 0x3fffffff) return -1;
         if (pair) return launch_stream<GROUPED, 1, GROUP, true>(p, chunks * half, stream);
         return launch_stream<GROUPED, 1, GROUP, false>(p, chunks * ((half + 1) / 2), stream);

@@ -210,7 +210,7 @@ def gemm4(x: torch.Tensor, w: Weight4, out: torch.Tensor, *, swiglu: bool = Fals
     L = _lib or lib()
     # Few rows stream the weights through registers, more go to the tensor core, whose tiles cost the same for 16 rows as for 100.  (us, this way / the
     # other: 17 rows of 6,144 x 2,048 7.3 / 10.2, 24 8.4 / 10.3, 32 in passes of 24 16 / 10.5; of 2,048 x 5,632 10.2 / 11.5, 12.0 / 11.5; of a pair
-    # 11,264 x 2,048 9.8 / 15.3, 10.2 / 15.4; of 40,960 x 2,048 20.9 / 38.2, 21.4 / 38.2.  60 experts of a pair 2,816 x 2,048 at 12 rows an expert 80 / 98, at 16 103 / 99; of 2,048 x 1,408 49 / 51, 61 / 51.)
+    # 11,264 x 2,048 9.8 / 15.3, 10.2 / 15.4; of 40,960 x 2,048 20.9 / 38.2, 21.4 / 38.2.  60 experts of a pair 2,816 x 2,048 at 14 rows an expert 79 / 98, at 16 93 / 99; of 2,048 x 1,408 50 / 51, 57 / 51.)
     few = M <= (FEW_ROWS if po is None else GROUP_FEW_ROWS * w.G)
     done = -1
     for form in (few, not few):            # (what one does not take, -1, the other may)

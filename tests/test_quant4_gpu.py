@@ -209,7 +209,7 @@ def test_a_product_right_behind_the_quantiser_of_its_weight(quant):
 
 
 # ------------------------------------------------------------------------------------------------ grouped products
-@pytest.mark.parametrize("rows", [[0, 3, 0, 0, 8, 9, 1, 0], [0] * 8, [17, 0, 40, 16, 1, 0, 100, 33], [300, 0, 1, 0, 0, 257, 64, 5], [0, 0, 0, 0, 0, 0, 0, 1]])
+@pytest.mark.parametrize("rows", [[0, 3, 0, 0, 8, 9, 1, 0], [0] * 8, [17, 0, 16, 33, 1, 0, 8, 25], [17, 0, 40, 16, 1, 0, 100, 33], [300, 0, 1, 0, 0, 257, 64, 5], [0, 0, 0, 0, 0, 0, 0, 1]])
 @pytest.mark.parametrize("pair", [False, True])
 def test_groups(quant, rows, pair):
     """Groups with and without rows, rows in front of the first group and behind the last: those stay as they were."""
