@@ -14,7 +14,7 @@
 //                            151,936 x 2,048 37 us (4.5 TB/s; ALU 58 %, issue slots 64 %), 16 rows of a pair 40,960 x 3,584 26 us (2.9 TB/s: the products
 //                            of two tiles of rows do not overlap with the fragments' making), 256 rows of 60 experts 2,048 x 1,408 30 us (3.1 TB/s)
 //   experts_down_kernel      the second half of a layer of experts.  A layer of 60 experts of 1,408 and a shared one of 5,632, width 2,048: 1 token
-//                            17.3 us, 8 tokens 41.5 (ALU 52 and 43 % of either half)
+//                            18.2 us, 8 tokens 44.7
 #include "quant4.cuh"
 
 namespace {
@@ -180,7 +180,7 @@ struct Args {
     float act_param;
     const int* idx;                // EXPERTS: the picks, [M, top_k]
     int top_k, E;
-    uint8_t *frag, *sfrag;         // EXPERTS: [slot][frag_blocks] of 2 KB, see experts_down_kernel; the shared expert's
+    uint8_t *frag, *sfrag;         // EXPERTS: [slot][frag_blocks] of TERMS_BLOCK bytes, see experts_down_kernel; the shared expert's
     int frag_blocks;
     q4::Bits bits;
     q4::Waits waits;
@@ -281,13 +281,14 @@ gemm_q4_direct_kernel(const __grid_constant__ Args p) {
 // GROUPED rows [offsets[g], offsets[g + 1]) meet weight g, 8 NT at a time
 // EXPERTS the gate and up rows of a layer of routed experts: the eight rows of a unit are the step's tokens whatever the expert, so
 //         that nothing is gathered; the shared expert's strips come first.  What comes out lies as the B fragments of the next
-//         product, as two bfloat16 terms (rounded to one, the layer's output would be as far off again as its own rounding).
+//         product, as three bfloat16 terms that together are the 32-bit number.
 //
 // A unit is two strips (a pair's gate and up strip, or neighbours) and up to 8 NT rows.  A block takes a run of neighbouring units; its five teams of
 // four warps take them in turn, and the warps of a team every fourth block of 64 k.  One more warp a team has its codes copied (cp.async.bulk) into
 // stages of KC blocks, across the borders of units.  The fragments of the rows lie in shared memory for all teams; where the
 // rows change (GROUPED), all teams meet.
 enum { DENSE = 0, GROUPED = 1, EXPERTS = 2 };
+constexpr int TERMS_BLOCK = 3072;      // EXPERTS: bytes of 64 k of eight rows in three terms, see experts_down_kernel
 constexpr int GROUPS_MAX = 1024, TEAM_W = 4, TEAMS = 5, KC = 8, STREAM_THREADS = TEAMS * (TEAM_W + 1) * 32, STAGES_MAX = 8;
 
 template <int NT, int GROUP>
@@ -545,13 +546,25 @@ gemm_q4_stream_kernel(const __grid_constant__ Args p, const int stages) {
                         const bool takes = col < p.M && (v.slot < 0 || ((picked.takes[v.slot] >> col) & 1));
                         float a = 0.f;
                         if (takes) a = glu_mul(ACT_SILU, 0.f, sum_of<TEAM_W, 2>(sums, 0, col, f), sum_of<TEAM_W, 2>(sums, 1, col, f));
-                        const __nv_bfloat16 h = __float2bfloat16_rn(a), l = __float2bfloat16_rn(a - __bfloat162float(h));
-                        uint8_t* to = (v.slot < 0 ? p.sfrag : p.frag + (size_t)v.slot * p.frag_blocks * 2048) + (size_t)v.strip * 512;
-                        __nv_bfloat16* e = reinterpret_cast<__nv_bfloat16*>(to + (col * 4 + (f >> 2)) * 16) + (f & 3);
-                        e[0] = h, e[4] = l;
+                        // a = t[0] + t[1] + t[2]: each cuts eight bits of mantissa off what is left (nothing is rounded, but for what lies below 2^-133)
+                        float left = a;
+                        uint16_t t[3];
+#pragma unroll
+                        for (int k = 0; k < 3; k++) {
+                            const uint32_t cut = __float_as_uint(left) & 0xffff0000u;
+                            t[k] = (uint16_t)(cut >> 16), left = isinf(left) ? 0.f : left - __uint_as_float(cut);
+                        }
+                        const int at = col * 4 + (f >> 2);
+                        uint8_t* to = (v.slot < 0 ? p.sfrag : p.frag + (size_t)v.slot * p.frag_blocks * TERMS_BLOCK) + (size_t)(v.strip >> 2) * TERMS_BLOCK;
+                        uint16_t *first = reinterpret_cast<uint16_t*>(to + (v.strip & 3) * 512 + at * 16) + (f & 3),
+                                 *last = reinterpret_cast<uint16_t*>(to + 2048 + (v.strip & 2) * 256 + at * 16 + (v.strip & 1) * 8) + (f & 3);
+                        first[0] = t[0], first[4] = t[1], *last = t[2];
                         // the strips that fill the last block of 64
                         if (v.strip == (v.slot < 0 ? shared_units : half) - 1)
-                            for (int z = v.strip + 1; z & 3; z++) *reinterpret_cast<uint32_t*>(to + (size_t)(z - v.strip) * 512 + i * 4) = 0u;
+                            for (int z = v.strip + 1; z & 3; z++) {
+                                *reinterpret_cast<uint32_t*>(to + (z & 3) * 512 + i * 4) = 0u;
+                                if (i < 64) *reinterpret_cast<uint32_t*>(to + 2048 + (z & 2) * 256 + (i >> 1) * 16 + (z & 1) * 8 + (i & 1) * 4) = 0u;
+                            }
                         continue;
                     }
                     if (n >= p.N || n8 * 8 + col >= rows) continue;
@@ -568,11 +581,13 @@ gemm_q4_stream_kernel(const __grid_constant__ Args p, const int stages) {
 // ---- the down products of a layer of routed experts ---------------------------------------------------------------------------------------
 //   out_t = sum_e w_te Wd_e a_te + gate_t Wd_s a_t,  w_te the sum of t's weights for expert e
 // Four strips of the output go through ALL picked experts and the shared one, w_te on the sums of each block of 64 k: nothing is left to
-// combine.  Tokens that did not pick an expert meet it with the zeros that the first kernel left, and its sums stay out of theirs (a scale may be NaN).  A block of 64 k of the rows is 2 KB: for each 16 k a
-// B fragment of 32 lanes x (four k rounded to bfloat16, what that left rounded likewise).  Grid: (fours of strips, 1, S); the S blocks of a unit are
+// combine.  Tokens that did not pick an expert meet it with the zeros that the first kernel left, and its sums stay out of theirs (a scale may be NaN).  A block of 64 k of the rows is 3 KB: for each
+// 16 k a B fragment of 32 lanes x (four k's first terms, their second terms), and behind the four of them the third terms, 8 bytes a lane.  (With two terms, rounded, the
+// layer's 32-bit output was 2.4e-6 of its norm off, ten times what its sums leave: 1 token 17.3 us, 8 tokens 41.6.  32-bit rows that become three terms in registers
+// here: 18.9, 47.0.)  Grid: (fours of strips, 1, S); the S blocks of a unit are
 // a cluster and share its blocks of 64 k; the first of them adds their sums up in order.  A warp takes every sixteenth block and copies for itself
 // into a ring of its own (cp.async: its pieces of 512 bytes and less are too small for bulk copies, of which an SM issued one in ten to twenty cycles).
-constexpr int DOWN_W = 16, DOWN_MT = 4, DOWN_DEPTH = 3, DOWN_THREADS = DOWN_W * 32;
+constexpr int DOWN_W = 16, DOWN_MT = 4, DOWN_DEPTH = 2, DOWN_THREADS = DOWN_W * 32;
 struct DownArgs {
     Weight down, shared;           // shared.codes null: none
     const uint8_t *frag, *sfrag;
@@ -586,7 +601,7 @@ struct DownArgs {
 };
 template <int GROUP>
 struct DownRing {
-    static constexpr int SCALES = GROUP == 32 ? 64 : 32, X = DOWN_MT * (512 + SCALES), SLOT = X + 2048, BYTES = DOWN_W * DOWN_DEPTH * SLOT;
+    static constexpr int SCALES = GROUP == 32 ? 64 : 32, X = DOWN_MT * (512 + SCALES), SLOT = X + TERMS_BLOCK, BYTES = DOWN_W * DOWN_DEPTH * SLOT;
     static_assert(DOWN_W * DOWN_MT * 8 * 17 * 4 <= BYTES && DOWN_THREADS == DOWN_MT * 128, "sums");  // they lie over the rings
     static constexpr int PARTS = 7 * DOWN_MT * 128 * 4;             // the other blocks' sums, behind the rings
 };
@@ -640,9 +655,9 @@ experts_down_kernel(const __grid_constant__ DownArgs p) {
         }
     };
     auto copy_rows = [&](uint32_t to, Place at) {
-        const uint8_t* from = (at.slot < slots ? p.frag + (size_t)at.slot * nb * 2048 : p.sfrag) + (size_t)at.b * 2048 + lane * 16;
+        const uint8_t* from = (at.slot < slots ? p.frag + (size_t)at.slot * nb * TERMS_BLOCK : p.sfrag) + (size_t)at.b * TERMS_BLOCK + lane * 16;
 #pragma unroll
-        for (int j = 0; j < 4; j++) copy16(to + D::X + j * 512 + lane * 16, from + j * 512);
+        for (int j = 0; j < 6; j++) copy16(to + D::X + j * 512 + lane * 16, from + j * 512);
     };
     Place now;
     now.slot = min((lo + warp) / nb, slots), now.b = lo + warp - now.slot * nb;
@@ -675,22 +690,26 @@ experts_down_kernel(const __grid_constant__ DownArgs p) {
         copy_wait<DOWN_DEPTH - 1>();
         __syncwarp();                                           // (the scales were copied by other lanes)
         float c[DOWN_MT][4], sum[DOWN_MT][4];
-        uint4 code[DOWN_MT];
+        uint4 code[DOWN_MT], third;
 #pragma unroll
         for (int m = 0; m < DOWN_MT; m++) code[m] = lds16(at + m * 512 + lane * 16);
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            const uint4 x = lds16(at + D::X + j * 512 + lane * 16);
+            const uint4 two = lds16(at + D::X + j * 512 + lane * 16);
+            if (j % 2 == 0) third = lds16(at + D::X + 2048 + j * 256 + lane * 16);
+            const uint2 x[3] = {make_uint2(two.x, two.y), make_uint2(two.z, two.w), j % 2 ? make_uint2(third.z, third.w) : make_uint2(third.x, third.y)};
             const bool fresh = GROUP == 32 ? j % 2 == 0 : j == 0, last = GROUP == 32 ? j % 2 == 1 : j == 3;
 #pragma unroll
             for (int m = 0; m < DOWN_MT; m++) {
                 uint32_t a[4];
                 q4::unpack(q4::word(code[m], j), p.bits, a);
-                if (fresh)
-                    q4::mma(c[m], a, x.x, x.y, 0.f, 0.f, 0.f, 0.f);
-                else
-                    q4::mma(c[m], a, x.x, x.y, c[m][0], c[m][1], c[m][2], c[m][3]);
-                q4::mma(c[m], a, x.z, x.w, c[m][0], c[m][1], c[m][2], c[m][3]);
+#pragma unroll
+                for (int i = 0; i < 3; i++) {
+                    if (fresh && i == 0)
+                        q4::mma(c[m], a, x[i].x, x[i].y, 0.f, 0.f, 0.f, 0.f);
+                    else
+                        q4::mma(c[m], a, x[i].x, x[i].y, c[m][0], c[m][1], c[m][2], c[m][3]);
+                }
             }
             if (last)
 #pragma unroll
@@ -841,7 +860,7 @@ MOE_API int moe_gemm_q4(const void* x, int ldx, int M, const void* codes, const 
 }
 
 // x: [T, H] bfloat16, row pitch ldx; idx, wk: [T, top_k]; gate: [T] or null; gu [E, 2 size, H] and sgu [2 shared, H] pairs, down [E, H, size], sdown
-// [H, shared]; shared 0: no shared expert; scratch: 2 KB for each 64 features of the experts that may be picked
+// [H, shared]; shared 0: no shared expert; scratch: 3 KB for each 64 features of the experts that may be picked
 // (min(T top_k, E)) and of the shared one.  Returns -1 for what it does not take: more than 8 tokens, 1,024 experts or 128 picks, rows that shared
 // memory does not hold (H beyond 6,000 or so).
 MOE_API int moe_experts_q4(const void* x, int ldx, int T, int H, const int* idx, const float* wk, int top_k, int E, int size, const void* gu_codes,
@@ -859,8 +878,8 @@ MOE_API int moe_experts_q4(const void* x, int ldx, int T, int H, const int* idx,
     up.w = weight(gu_codes, gu_scales, 2 * size, H, group, 1), d.down = weight(down_codes, down_scales, H, size, group, 0);
     if (shared > 0) up.shared = weight(sgu_codes, sgu_scales, 2 * shared, H, group, 1), d.shared = weight(sdown_codes, sdown_scales, H, shared, group, 0);
     const long long slots = (long long)T * top_k < E ? (long long)T * top_k : E;
-    up.frag = (uint8_t*)scratch, up.frag_blocks = d.down.blocks, up.sfrag = up.frag + slots * d.down.blocks * 2048;
-    if (scratch_bytes < (slots * d.down.blocks + (shared + 63) / 64) * 2048) return (int)cudaErrorInvalidValue;
+    up.frag = (uint8_t*)scratch, up.frag_blocks = d.down.blocks, up.sfrag = up.frag + slots * d.down.blocks * TERMS_BLOCK;
+    if (scratch_bytes < (slots * d.down.blocks + (shared + 63) / 64) * TERMS_BLOCK) return (int)cudaErrorInvalidValue;
     d.frag = up.frag, d.sfrag = up.sfrag, d.bits = up.bits;
     d.T = T, d.H = H, d.E = E, d.top_k = top_k, d.idx = idx, d.wk = wk, d.gate = gate, d.out = out, d.out_bf16 = out_bf16, d.ldo = ldo;
     // blocks of a cluster: one block an SM, but five blocks of 64 k a warp are done sooner than two cluster barriers

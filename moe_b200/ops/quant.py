@@ -278,7 +278,7 @@ def experts4(x: torch.Tensor, topk_idx: torch.Tensor, topk_w: torch.Tensor, gate
         return True
     L = _lib or lib()
     slots = min(T * k, E)
-    scratch = torch.empty((slots * -(-size // 64) + -(-shared // 64)) * 2048, dtype=torch.uint8, device=x.device)
+    scratch = torch.empty((slots * -(-size // 64) + -(-shared // 64)) * 3072, dtype=torch.uint8, device=x.device)
     code = L.moe_experts_q4(x.data_ptr(), ldx, T, H, pi, pw, k, E, size, *gate_up.pointers, *down.pointers, shared, *s, pg, group, scratch.data_ptr(),
                             scratch.numel(), out.data_ptr(), out.dtype is _BF16, ldo, ps, core._stream())
     if code == -1:
