@@ -495,7 +495,8 @@ gemm_q4_stream_kernel(const __grid_constant__ Args p, const int stages) {
             uint32_t xa = xs + tw * NT * 1024 + lane * 16;
             int left = blocks - tw;                      // blocks from this warp's first on
             for (int st = 0; st < unit_stages; st++) {
-                ok = q4::mbar_wait(smem_u32(&s_bars[team][0][s]), parity, &s_abort, p.waits.limit_us, p.waits.status, 0x64);
+                // (a lane may give up where another is let through: the warp goes on, to products that all of it has to reach, or gives up, as a whole)
+                ok = __all_sync(0xffffffffu, q4::mbar_wait(smem_u32(&s_bars[team][0][s]), parity, &s_abort, p.waits.limit_us, p.waits.status, 0x64));
                 if (!ok) break;
                 const uint32_t at = base + s * S::STAGE + tw * 512 + lane * 16, as = base + s * S::STAGE + 2 * S::CODES + r * 4;
 #pragma unroll

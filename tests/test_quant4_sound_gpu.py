@@ -53,3 +53,32 @@ def test_what_lies_between_a_layers_products_keeps_32_bits(quant, T, group):
         fine(st)
         far = (out.double() - y).abs()
         assert bool((far <= 2.0 ** -20 * y.abs() + 1e-37).all()), f"{what}: {float((far / y.abs().clamp_min(1e-37)).max()):.3g} of an output"
+
+
+# ------------------------------------------------------------------------------------------------ waits
+@pytest.mark.parametrize("per", [3, 12])
+@pytest.mark.parametrize("pair", [False, True])
+def test_a_wait_of_streamed_groups_that_runs_out(quant, pair, per):
+    """Groups of few rows, one and two tiles of rows at a time: every team of every block gives up on several runs of units, and as a whole."""
+    from moe_b200.ops import core
+
+    torch.manual_seed(per)
+    groups, K, N = 9, 328, 640
+    off = torch.arange(0, groups * per + 1, per, dtype=torch.int32, device=DEV)
+    w4, W = weight(quant, (groups, N, K), pair=pair)
+    st, x, out = status(), torch.randn(groups * per, K, device=DEV).to(BF), torch.empty(groups * per, N // 2 if pair else N, device=DEV)
+    run = lambda: quant.gemm4(x, w4, out, swiglu=pair, group_offsets=off, status=st)  # noqa: E731
+    L = quant.lib()
+    L.moe_q4_set_wait_test(1, 2000)
+    try:
+        run()
+        torch.cuda.synchronize()
+    finally:
+        L.moe_q4_set_wait_test(0, 0)
+    assert int(st[0]) & 8, "the wait that ran out was not reported"
+    with pytest.raises(core.KernelError, match="4-bit weights"):
+        core.check_status(st)
+    run()
+    fine(st)
+    for g in range(groups):
+        Q.check_product(out[g * per:(g + 1) * per], x[g * per:(g + 1) * per], W[g], swiglu=pair)
