@@ -200,6 +200,9 @@ WAIT_ROLES = {
     0x4: "MMA issuer: a loaded stage", 0x5: "epilogue: a finished accumulator",
     0x6: "converter: a free stage", 0x8: "MMA issuer: its last product",
 }
+WAIT_ROLES_STREAM = {
+    0x1: "copies: a free stage", 0x2: "copies: their own in flight", 0x3: "copies: the step's picks", 0x4: "products: a loaded stage",
+}
 WAIT_ROLES_ATTENTION = {
     0x1: "producer: a free key stage", 0x2: "producer: a free value stage", 0x3: "producer: its own copies in flight",
     0x4: "MMA issuer: the queries", 0x5: "MMA issuer: a key tile",
@@ -210,7 +213,7 @@ WAIT_ROLES_ATTENTION = {
 
 def wait_site(code: int) -> str:
     kernel, role = code & 0xf0, code & 0xf
-    roles = WAIT_ROLES_ATTENTION if kernel == 0x40 else WAIT_ROLES
+    roles = {0x40: WAIT_ROLES_ATTENTION, 0x60: WAIT_ROLES_STREAM}.get(kernel, WAIT_ROLES)
     return f"{WAIT_SITES.get(kernel, 'kernel ?')}, {roles.get(role, 'wait ?')} (site 0x{code:02x})"
 
 
