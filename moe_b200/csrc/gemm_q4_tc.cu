@@ -536,10 +536,10 @@ uint32_t g_wait_limit = WAIT_LIMIT_US;
 int g_test_fault = 0;
 
 template <int GROUP, bool PAIR, bool WIDE>
-int launch(const CUtensorMap& map, const Args& p, unsigned ctas, cudaStream_t stream) {
+int launch(const CUtensorMap& map, const Args& p, unsigned ctas, bool early, cudaStream_t stream) {
     static q4::SmemLimit limit;
     if (const int e = limit.lift((const void*)gemm_q4_tc_kernel<GROUP, PAIR, WIDE>)) return e;
-    return launch_pdl_cluster(gemm_q4_tc_kernel<GROUP, PAIR, WIDE>, dim3(ctas, 1, p.splits), dim3(Form<WIDE>::THREADS), (size_t)(p.stages * p.stage_bytes + 1024), stream, p.splits, map, p);
+    return launch_pdl_if(early, gemm_q4_tc_kernel<GROUP, PAIR, WIDE>, dim3(ctas, 1, p.splits), dim3(Form<WIDE>::THREADS), (size_t)(p.stages * p.stage_bytes + 1024), stream, p.splits, map, p);
 }
 
 }  // namespace
@@ -547,7 +547,7 @@ int launch(const CUtensorMap& map, const Args& p, unsigned ctas, cudaStream_t st
 // The same product as moe_gemm_q4 by the kernel above.  Returns -1, with nothing launched, for what it does not take: K or a row pitch of x that is no
 // multiple of 8, an unaligned x, more than 1,024 groups.
 MOE_API int moe_gemm_q4_tc(const void* x, int ldx, int M, const void* codes, const void* scales, int G, int N, int K, int group, int pair, void* out,
-                           int out_bf16, int ldo, const float* bias, const int* offsets, int act, float act_param, int splits, int* status, cudaStream_t stream) {
+                           int out_bf16, int ldo, const float* bias, const int* offsets, int act, float act_param, int splits, int early, int* status, cudaStream_t stream) {
     if (M <= 0 || N <= 0) return 0;
     if (!x || !codes || !scales || !out || K <= 0 || G <= 0 || (G > 1 && !offsets) || (pair && N % 2)) return (int)cudaErrorInvalidValue;
     if (K % 8 || ldx % 8 || ((uintptr_t)x & 15) || G > MAX_GROUPS || !encode_fn()) return -1;
@@ -587,8 +587,8 @@ MOE_API int moe_gemm_q4_tc(const void* x, int ldx, int M, const void* codes, con
     p.splits = (p.w.blocks + p.kb_per_split - 1) / p.kb_per_split;
     const unsigned ctas = p.splits > 1 ? (unsigned)tiles : (unsigned)(tiles < sms ? tiles : sms);
 #define GO(GR)                                                                                                  \
-    (wide ? (pair ? launch<GR, true, true>(map, p, ctas, stream) : launch<GR, false, true>(map, p, ctas, stream)) \
-          : (pair ? launch<GR, true, false>(map, p, ctas, stream) : launch<GR, false, false>(map, p, ctas, stream)))
+    (wide ? (pair ? launch<GR, true, true>(map, p, ctas, early, stream) : launch<GR, false, true>(map, p, ctas, early, stream)) \
+          : (pair ? launch<GR, true, false>(map, p, ctas, early, stream) : launch<GR, false, false>(map, p, ctas, early, stream)))
     switch (group) {
         case 32: return GO(32);
         case 64: return GO(64);

@@ -164,13 +164,12 @@ constexpr int quantize_blocks = GROUP == 128 ? 3 : FULL && sizeof(T) == 2 ? 6 : 
 template <typename T, int GROUP, bool FULL>
 __global__ void __launch_bounds__(256, (quantize_blocks<T, GROUP, FULL>))
 quantize_kernel(const T* __restrict__ w, const Shape p, int vec, uint4* __restrict__ codes, uint32_t* __restrict__ scales, int* status) {
-    pdl_wait();                          // (the successor is let in when all is written and to be seen: products read their weights before they wait)
+    pdl_wait();
     const int warp = threadIdx.x >> 5, u = ((int)blockIdx.x << p.kw) + (warp & ((1 << p.kw) - 1));
     if (u >= p.units) return;
     for (int g = blockIdx.z; g < p.G; g += gridDim.z)
         for (int strip = blockIdx.y * (8 >> p.kw) + (warp >> p.kw); strip < p.strips; strip += gridDim.y * (8 >> p.kw))
             quantize_unit<T, GROUP, FULL>(w, p, g, strip, u, vec, codes, scales, status);
-    __threadfence();
 }
 
 template <int GROUP>

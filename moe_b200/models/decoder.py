@@ -103,6 +103,7 @@ class DecoderModel:
             bind(j)
         bind(self.final_norm)
         bind(self.head, embedding=self.embedding)
+        rt.settle()
         self.num_parameters = sum(
             int(torch.tensor(ts.shape).prod()) for ts in expected_tensors(spec).values()
         )

@@ -41,9 +41,9 @@ def lib():
         P, I, F, LL = c_void_p, c_int, c_float, c_longlong
         for name, args in (("moe_q4_quantize", [P, I, I, I, I, I, I, P, P, P, P]),
                            ("moe_q4_dequantize", [P, P, I, I, I, I, I, P, P]),
-                           ("moe_gemm_q4", [P, I, I, P, P, I, I, I, I, I, P, I, I, P, P, I, F, P, P]),
-                           ("moe_gemm_q4_tc", [P, I, I, P, P, I, I, I, I, I, P, I, I, P, P, I, F, I, P, P]),
-                           ("moe_experts_q4", [P, I, I, I, P, P, I, I, I, P, P, P, P, I, P, P, P, P, P, I, P, LL, P, I, I, P, P])):
+                           ("moe_gemm_q4", [P, I, I, P, P, I, I, I, I, I, P, I, I, P, P, I, F, I, P, P]),
+                           ("moe_gemm_q4_tc", [P, I, I, P, P, I, I, I, I, I, P, I, I, P, P, I, F, I, I, P, P]),
+                           ("moe_experts_q4", [P, I, I, I, P, P, I, I, I, P, P, P, P, I, P, P, P, P, P, I, P, LL, P, I, I, I, P, P])):
             fn = getattr(L, name)
             fn.argtypes, fn.restype = args, c_int
         L.moe_q4_set_wait_test.argtypes, L.moe_q4_set_wait_test.restype = [I, c_uint], None
@@ -61,9 +61,13 @@ class Weight4:
     [.., strip, block, r, t, j, h, p] holds k = 64 block + 16 j + 4 t + 2 p + h of rows r (low four bits) and r + 8 (high four bits) of the
     strip, each as q + 8.  ``scales``: bfloat16 [G, strips, ceil(K / group), 8, 2], rows r and r + 8 beside one another, each of at most five
     significant bits.  Rows beyond N have scale 0, elements beyond K q = 0.  With ``pair`` the rows are a gated feed-forward's, N / 2 of
-    the gate and N / 2 of up, and either half fills whole strips; a pair is what products with ``swiglu`` take."""
+    the gate and N / 2 of up, and either half fills whole strips; a pair is what products with ``swiglu`` take.
 
-    __slots__ = ("codes", "scales", "shape", "group", "pair", "G", "N", "K", "place", "pointers")
+    Products read a weight before the kernel in front of them on their stream has ended, as soon as that cannot be the one that wrote it: from a
+    weight's second product on a stream on, or on any stream behind ``settle``.  So ``codes`` and ``scales`` may be written (on the product's stream, or ordered
+    before it) right until the weight's first product, and not after it: who writes other ones into the same tensors makes another ``Weight4`` of them."""
+
+    __slots__ = ("codes", "scales", "shape", "group", "pair", "G", "N", "K", "place", "pointers", "read_on")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, shape: Tuple[int, ...], group: int = 64, pair: bool = False):
         if len(shape) == 2:
@@ -88,6 +92,7 @@ class Weight4:
                                    f"of {nc} and {ns} elements on one device")
         self.codes, self.scales, self.shape, self.group, self.pair = codes, scales, tuple(shape), group, bool(pair)
         self.G, self.N, self.K, self.place, self.pointers = G, N, K, place, (pc, ps)
+        self.read_on = ()             # the streams that have had a product of this weight; None: all may be taken to
 
     @property
     def device(self) -> torch.device:
@@ -97,6 +102,11 @@ class Weight4:
     def dtype(self) -> str:
         """(No ``torch.dtype``: whoever asks whether a weight is bfloat16 is told no.)"""
         return "int4"
+
+    def settle(self) -> None:
+        """Waits until the device has done what it was given, the writing of this weight with it."""
+        torch.cuda.synchronize(self.device)
+        self.read_on = None
 
     @property
     def nbytes(self) -> int:
@@ -140,6 +150,19 @@ def _matrix(t: torch.Tensor, place: int, name: str, wide: bool):
         raise core.KernelError(f"{name}: expected less than 2^28 dense rows that do not overlap, less than 2^31 elements apart, got strides {t.stride()} of "
                                f"{tuple(t.shape)}")
     return rows, columns, pitch
+
+
+def _early(w: Weight4, stream: int) -> bool:
+    return w.read_on is None or stream in w.read_on
+
+
+def _has_read(w: Weight4, stream: int):
+    """(Not what is captured: a graph's launches say nothing of the stream that it was captured on.)"""
+    if w.read_on is not None and stream not in w.read_on and not _capturing():
+        w.read_on = (*w.read_on, stream)
+
+
+_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", torch.cuda.is_current_stream_capturing)
 
 
 def quantize(w: torch.Tensor, group: int = 64, *, pair: bool = False, status=None) -> Weight4:
@@ -207,7 +230,8 @@ def gemm4(x: torch.Tensor, w: Weight4, out: torch.Tensor, *, swiglu: bool = Fals
     if not M:
         return out
     pc, ps = w.pointers
-    L = _lib or lib()
+    L, stream = _lib or lib(), core._stream()
+    early = _early(w, stream)
     # Few rows stream the weights through registers, more go to the tensor core, whose tiles cost the same for 16 rows as for 100.  (us, this way / the
     # other: 17 rows of 6,144 x 2,048 7.3 / 10.2, 24 8.4 / 10.3, 32 in passes of 24 16 / 10.5; of 2,048 x 5,632 10.2 / 11.5, 12.0 / 11.5; of a pair
     # 11,264 x 2,048 9.8 / 15.3, 10.2 / 15.4; of 40,960 x 2,048 20.9 / 38.2, 21.4 / 38.2.  60 experts of a pair 2,816 x 2,048 at 14 rows an expert 79 / 98, at 16 93 / 99; of 2,048 x 1,408 50 / 51, 57 / 51.)
@@ -216,12 +240,14 @@ def gemm4(x: torch.Tensor, w: Weight4, out: torch.Tensor, *, swiglu: bool = Fals
     for form in (few, not few):            # (what one does not take, -1, the other may)
         if form:
             done = L.moe_gemm_q4(x.data_ptr(), ldx, M, pc, ps, w.G, w.N, K, w.group, w.pair, out.data_ptr(), out.dtype is _BF16, ldo, pb, po,
-                                 code, act_param, st, core._stream())
+                                 code, act_param, early, st, stream)
         else:
             done = L.moe_gemm_q4_tc(x.data_ptr(), ldx, M, pc, ps, w.G, w.N, K, w.group, w.pair, out.data_ptr(), out.dtype is _BF16, ldo, pb,
-                                    po, code, act_param, 1 if po is not None else _splits(M, N, w, place), st, core._stream())
+                                    po, code, act_param, 1 if po is not None else _splits(M, N, w, place), early, st, stream)
         if done != -1:
             core._ok(done, "gemm4")
+            if not early:
+                _has_read(w, stream)
             return out
     raise core.KernelError("gemm4: a stack of more than 1,024 weights, or one of K beyond 5,500 or so with rows that are no whole 16-byte units")
 
@@ -276,13 +302,18 @@ def experts4(x: torch.Tensor, topk_idx: torch.Tensor, topk_w: torch.Tensor, gate
         return False
     if not T:
         return True
-    L = _lib or lib()
+    L, stream = _lib or lib(), core._stream()
+    weights = (gate_up, down) if shared_gate_up is None else (gate_up, down, shared_gate_up, shared_down)
+    early = all(_early(w, stream) for w in weights)
     slots = min(T * k, E)
     scratch = torch.empty((slots * -(-size // 64) + -(-shared // 64)) * 3072, dtype=torch.uint8, device=x.device)
     code = L.moe_experts_q4(x.data_ptr(), ldx, T, H, pi, pw, k, E, size, *gate_up.pointers, *down.pointers, shared, *s, pg, group, scratch.data_ptr(),
-                            scratch.numel(), out.data_ptr(), out.dtype is _BF16, ldo, ps, core._stream())
+                            scratch.numel(), out.data_ptr(), out.dtype is _BF16, ldo, early, ps, stream)
     if code == -1:
         return False
     core._ok(code, "experts4")
+    if not early:
+        for w in weights:
+            _has_read(w, stream)
     core.launches += 1            # (two kernels)
     return True

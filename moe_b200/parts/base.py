@@ -118,6 +118,7 @@ class Runtime:
         if weight_group not in (0, 32, 64, 128):
             raise ValueError(f"weights in 4 bits have groups of 32, 64 or 128, not {weight_group}")
         self.weight_group = int(weight_group)
+        self._fresh = []               # matrices in 4 bits that were not waited for yet, see ``settle``
         self.device = torch.device(device)
         self.compute_dtype = compute_dtype
         self.forked = False            # see ``beside``
@@ -153,6 +154,11 @@ class Runtime:
 
     def empty(self, shape, dtype=None) -> torch.Tensor:
         return torch.empty(shape, dtype=dtype or self.compute_dtype, device=self.device)
+
+    def settle(self) -> None:
+        """Waits for what a model's binding launched, its matrices in 4 bits among it: every step's products may then read them early."""
+        while self._fresh:
+            self._fresh.pop().settle()
 
     def check(self) -> None:
         from ..ops import core
@@ -230,7 +236,9 @@ class Part:
         from ..ops import quant
 
         self.in_4_bits = True
-        return quant.quantize(w.contiguous(), rt.weight_group, pair=pair, status=rt.status)
+        held = quant.quantize(w.contiguous(), rt.weight_group, pair=pair, status=rt.status)
+        rt._fresh.append(held)
+        return held
 
     def step_bytes(self, num_tokens: int, rt: Runtime) -> float:
         """Bytes of ``step_elements``: a part that holds its matrices in 4 bits counts all its elements so."""
