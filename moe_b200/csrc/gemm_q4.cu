@@ -892,4 +892,12 @@ MOE_API int moe_experts_q4(const void* x, int ldx, int T, int H, const int* idx,
 #undef GO
 }
 
+// Whether shared memory holds what groups of few rows need of rows of K elements (layer: what the first kernel of a layer of experts needs).
+MOE_API int moe_q4_holds_rows(int K, int group, int layer) {
+    const int blocks = (K + 63) / 64;
+#define GO(GR) (layer ? stream_stages<EXPERTS, 1, GR>(blocks) : stream_stages<GROUPED, 1, GR>(blocks)) > 0
+    BY_GROUP(GO);
+#undef GO
+}
+
 void q4::few_rows_wait_test(int fault, uint32_t wait_limit) { g_test_fault = fault, g_wait_limit = wait_limit; }

@@ -4,7 +4,7 @@ The bfloat16 path uses the tcgen05 kernel (``tc.gemm_tc``) wherever activations 
 weight are both bfloat16 and the shape qualifies, and the plain kernel otherwise (a
 weight stored in 32-bit, a width that is no multiple of 8).  The float32 path always
 uses the plain kernel, which is true 32-bit arithmetic.  A weight may be a ``quant.Weight4`` (held in 4
-bits), with bfloat16 activations: ``quant.gemm4`` takes every such product.
+bits), with bfloat16 activations: ``quant.gemm4`` takes every such product, rows that are no whole 16-byte units among them.
 """
 from __future__ import annotations
 
@@ -26,7 +26,7 @@ def linear(rt, a: torch.Tensor, w: torch.Tensor, *, bias: Optional[torch.Tensor]
     of a branch (``Runtime.beside``): the other branch wants the SMs that the splits would fill"""
     out = torch.empty((a.shape[0], w.shape[0]), dtype=out_dtype, device=a.device)
     if isinstance(w, Weight4):
-        return gemm4(a, w, out, bias=bias, status=rt.status)
+        return gemm4(a, w, out, bias=bias, any_rows=True, status=rt.status)
     if _use_tc(rt, a, w):
         from . import tc
 
@@ -44,7 +44,7 @@ def swiglu_linear(rt, a: torch.Tensor, w_gate_up: torch.Tensor, act: str = "silu
     M, inter = a.shape[0], w_gate_up.shape[0] // 2
     out = torch.empty((M, inter), dtype=rt.compute_dtype, device=a.device)
     if isinstance(w_gate_up, Weight4):
-        return gemm4(a, w_gate_up, out, swiglu=True, status=rt.status, act=act, act_param=act_param)
+        return gemm4(a, w_gate_up, out, swiglu=True, any_rows=True, status=rt.status, act=act, act_param=act_param)
     if _use_tc(rt, a, w_gate_up):
         from . import tc
 
@@ -74,7 +74,7 @@ def grouped_swiglu_linear(rt, a: torch.Tensor, w_gate_up: torch.Tensor, group_of
     act = torch.empty((num_rows, inter), dtype=rt.compute_dtype, device=a.device)
     if isinstance(w_gate_up, Weight4):
         xs = a if rows is None else gathered if gathered is not None else _gather(rt, a, rows, num_rows)
-        return gemm4(xs, w_gate_up, act, swiglu=True, group_offsets=group_offsets, status=rt.status)
+        return gemm4(xs, w_gate_up, act, swiglu=True, group_offsets=group_offsets, any_rows=True, status=rt.status)
     if _use_tc(rt, a, w_gate_up) and a.shape[1] % 8 == 0:
         from . import tc
 
@@ -93,7 +93,7 @@ def grouped_linear(rt, a: torch.Tensor, w: torch.Tensor, group_offsets: torch.Te
     ``early_offsets``: see ``tc.gemm_tc``."""
     out = torch.empty((num_rows, w.shape[1]), dtype=torch.float32, device=a.device)
     if isinstance(w, Weight4):
-        return gemm4(a, w, out, group_offsets=group_offsets, status=rt.status)
+        return gemm4(a, w, out, group_offsets=group_offsets, any_rows=True, status=rt.status)
     if _use_tc(rt, a, w):
         from . import tc
 

@@ -29,6 +29,7 @@ SIZE_MAX = 1 << 30
 EXPERTS_TOKENS = 8            # tokens that ``experts4`` takes
 FEW_ROWS = 24                 # rows up to which a product streams its weights through registers
 GROUP_FEW_ROWS = 14           # the same of groups, on average
+GROUPS_A_LAUNCH = 1024        # groups that one launch of a grouped product takes
 
 _U8, _BF16, _F32 = torch.uint8, torch.bfloat16, torch.float32
 _lib = None
@@ -46,6 +47,7 @@ def lib():
                            ("moe_experts_q4", [P, I, I, I, P, P, I, I, I, P, P, P, P, I, P, P, P, P, P, I, P, LL, P, I, I, I, P, P])):
             fn = getattr(L, name)
             fn.argtypes, fn.restype = args, c_int
+        L.moe_q4_holds_rows.argtypes, L.moe_q4_holds_rows.restype = [I, I, I], c_int
         L.moe_q4_set_wait_test.argtypes, L.moe_q4_set_wait_test.restype = [I, c_uint], None
         L.moe_q4_set_pdl.argtypes, L.moe_q4_set_pdl.restype = [I], None
         if os.environ.get("MOE_B200_PDL", "1") == "0":      # programmatic dependent launch off
@@ -200,12 +202,16 @@ def dequantize(w: Weight4, out: Optional[torch.Tensor] = None) -> torch.Tensor:
 
 
 def gemm4(x: torch.Tensor, w: Weight4, out: torch.Tensor, *, swiglu: bool = False, bias: Optional[torch.Tensor] = None,
-          group_offsets: Optional[torch.Tensor] = None, act: str = "silu", act_param: float = 0.0, status=None) -> torch.Tensor:
+          group_offsets: Optional[torch.Tensor] = None, act: str = "silu", act_param: float = 0.0, any_rows: bool = False, status=None) -> torch.Tensor:
     """out = x w^T (+ bias), or act(x gate^T) * (x up^T) with ``swiglu`` and a pair; ``act``: as in ``tc.gemm_tc``.
 
     x: bfloat16 [M, K], dense rows of any pitch; out: float32 or bfloat16 [M, N] (a pair: [M, N / 2]), dense rows of any pitch.
     A stack needs ``group_offsets`` (int32 [G + 1], ascending): rows [offsets[g], offsets[g + 1]) of x meet w[g]; rows that no group
-    has are left as they were."""
+    has are left as they were.
+
+    The tensor cores take rows of x in whole 16-byte units (K and the pitch multiples of 8, an aligned first row).  Of others, ``any_rows`` copies those that
+    only they take, or take at once; without it a dense product of many such rows reads the weight once for every 24 of them, and groups with K beyond 5,500
+    or so are refused."""
     place = x.get_device()
     _here(place, "gemm4")
     M, K, ldx = _matrix(x, place, "x", False)
@@ -229,27 +235,38 @@ def gemm4(x: torch.Tensor, w: Weight4, out: torch.Tensor, *, swiglu: bool = Fals
     st = _on(status, place, "status", torch.int32)
     if not M:
         return out
-    pc, ps = w.pointers
     L, stream = _lib or lib(), core._stream()
     early = _early(w, stream)
     # Few rows stream the weights through registers, more go to the tensor core, whose tiles cost the same for 16 rows as for 100.  (us, this way / the
     # other: 17 rows of 6,144 x 2,048 7.3 / 10.2, 24 8.4 / 10.3, 32 in passes of 24 16 / 10.5; of 2,048 x 5,632 10.2 / 11.5, 12.0 / 11.5; of a pair
     # 11,264 x 2,048 9.8 / 15.3, 10.2 / 15.4; of 40,960 x 2,048 20.9 / 38.2, 21.4 / 38.2.  60 experts of a pair 2,816 x 2,048 at 14 rows an expert 79 / 98, at 16 93 / 99; of 2,048 x 1,408 50 / 51, 57 / 51.)
     few = M <= (FEW_ROWS if po is None else GROUP_FEW_ROWS * w.G)
-    done = -1
-    for form in (few, not few):            # (what one does not take, -1, the other may)
-        if form:
-            done = L.moe_gemm_q4(x.data_ptr(), ldx, M, pc, ps, w.G, w.N, K, w.group, w.pair, out.data_ptr(), out.dtype is _BF16, ldo, pb, po,
-                                 code, act_param, early, st, stream)
-        else:
-            done = L.moe_gemm_q4_tc(x.data_ptr(), ldx, M, pc, ps, w.G, w.N, K, w.group, w.pair, out.data_ptr(), out.dtype is _BF16, ldo, pb,
-                                    po, code, act_param, 1 if po is not None else _splits(M, N, w, place), early, st, stream)
-        if done != -1:
-            core._ok(done, "gemm4")
-            if not early:
-                _has_read(w, stream)
-            return out
-    raise core.KernelError("gemm4: a stack of more than 1,024 weights, or one of K beyond 5,500 or so with rows that are no whole 16-byte units")
+    if any_rows and (K % 8 or ldx % 8 or x.data_ptr() % 16) and not (few and (po is None or L.moe_q4_holds_rows(K, w.group, 0))):
+        few, ldx = False, (K + 7) // 8 * 8           # (as many blocks and groups of k as before: the weight's elements there are zeros)
+        whole = torch.zeros(M, ldx, dtype=_BF16, device=x.device)
+        whole[:, :K] = x
+        x, K = whole, ldx
+    strips = _strips(w.N, w.pair)
+    for g in range(0, w.G, GROUPS_A_LAUNCH):
+        pc, ps = w.pointers
+        if g:                              # further groups of a large stack
+            pc, ps, po = pc + g * strips * -(-K // 64) * 512, ps + g * strips * -(-K // w.group) * 32, po + 4 * GROUPS_A_LAUNCH
+        groups = min(w.G - g, GROUPS_A_LAUNCH)
+        for form in (few, not few):        # (what one does not take, -1, the other may)
+            if form:
+                done = L.moe_gemm_q4(x.data_ptr(), ldx, M, pc, ps, groups, w.N, K, w.group, w.pair, out.data_ptr(), out.dtype is _BF16, ldo, pb, po,
+                                     code, act_param, early or g > 0, st, stream)
+            else:
+                done = L.moe_gemm_q4_tc(x.data_ptr(), ldx, M, pc, ps, groups, w.N, K, w.group, w.pair, out.data_ptr(), out.dtype is _BF16, ldo, pb,
+                                        po, code, act_param, 1 if po is not None else _splits(M, N, w, place), early or g > 0, st, stream)
+            if done != -1:
+                break
+        if done == -1:
+            raise core.KernelError("gemm4: a stack of K beyond 5,500 or so with rows that are no whole 16-byte units (any_rows copies them)")
+        core._ok(done, "gemm4")
+    if not early:
+        _has_read(w, stream)
+    return out
 
 
 def _splits(M: int, N: int, w: Weight4, place: int) -> int:

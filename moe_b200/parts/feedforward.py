@@ -74,7 +74,7 @@ def act_linear(rt, a, w_up, act, out=None):
     if out is None:
         out = torch.empty((a.shape[0], w_up.shape[0]), dtype=rt.compute_dtype, device=a.device)
     if isinstance(w_up, Weight4):
-        return gemm4(a, w_up, out, status=rt.status, act=act)
+        return gemm4(a, w_up, out, any_rows=True, status=rt.status, act=act)
     if rt.is_bf16 and a.dtype == torch.bfloat16 and w_up.dtype == torch.bfloat16:
         from ..ops import tc
 

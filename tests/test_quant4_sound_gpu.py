@@ -5,6 +5,7 @@ from __future__ import annotations
 import pytest
 import torch
 
+import gpu_util as G
 import quant4_util as Q
 from test_quant4_gpu import BF, DEV, fine, quant, status, weight  # noqa: F401  (quant: a fixture)
 
@@ -194,3 +195,80 @@ def test_a_models_weights_are_settled(quant):
     model = moe_b200.random_model(helpers.CONFIG_A, seed=1, weights="int4")
     held = [w for b in model.blocks for p in b.parts() for w in vars(p).values() if isinstance(w, quant.Weight4)]
     assert held and all(w.read_on is None for w in held)
+
+
+# ------------------------------------------------------------------------------------------------ sizes that no tile divides, stacks of any size
+@pytest.mark.parametrize("rows", [[1, 0, 1], [40, 0, 17], [200, 150, 3]])
+@pytest.mark.parametrize("K,pitch", [(7999, 8000), (7999, 7999), (6000, 6001), (131, 131), (136, 139)])
+def test_groups_of_rows_that_are_no_whole_units(quant, K, pitch, rows):
+    torch.manual_seed(K + rows[0])
+    off, M = torch.tensor([0, *rows], dtype=torch.int32, device=DEV).cumsum(0).to(torch.int32), sum(rows)
+    x = torch.randn(M, pitch, device=DEV).to(BF)[:, :K]
+    for pair in (False, True):
+        w4, W = weight(quant, (3, 48, K), 32 if K == 131 else 128, pair=pair)
+        st, out = status(), torch.full((M, 24 if pair else 48), float("nan"), device=DEV)
+        quant.gemm4(x, w4, out, swiglu=pair, group_offsets=off, any_rows=True, status=st)
+        fine(st)
+        for g in range(3):
+            a, b = int(off[g]), int(off[g + 1])
+            if a < b:
+                Q.check_product(out[a:b], x[a:b], W[g], swiglu=pair)
+
+
+@pytest.mark.parametrize("M", [1, 24, 25, 300])
+@pytest.mark.parametrize("K,pitch,at", [(131, 131, 0), (128, 137, 5), (1001, 1008, 0), (64, 64, 1)])
+def test_dense_rows_that_are_no_whole_units(quant, M, K, pitch, at):
+    torch.manual_seed(M + K)
+    x = torch.randn(M * pitch + at, device=DEV).to(BF)[at:].view(M, pitch)[:, :K]
+    w4, W = weight(quant, (77, K))
+    st, bias = status(), torch.randn(77, device=DEV)
+    out = quant.gemm4(x, w4, torch.empty(M, 77, device=DEV), bias=bias, any_rows=True, status=st)
+    fine(st)
+    Q.check_product(out, x, W[0], bias=bias)
+
+
+@pytest.mark.parametrize("M", [700, 60000])
+def test_a_stack_of_more_groups_than_a_launch_takes(quant, M):
+    """In several launches; rows in front of the first group and behind the last stay as they were."""
+    G_, N, K = 2500, 24, 72
+    torch.manual_seed(M)
+    w4, W = weight(quant, (G_, N, K), 32)
+    off = torch.cat([torch.tensor([3]), torch.randint(3, M - 2, (G_ - 1,)).sort().values, torch.tensor([M - 2])])
+    x, st = torch.randn(M, K, device=DEV).to(BF), status()
+    out = quant.gemm4(x, w4, torch.full((M, N), 7.0, device=DEV), group_offsets=off.to(torch.int32).to(DEV), status=st)
+    fine(st)
+    assert bool((out[:3] == 7).all()) and bool((out[M - 2:] == 7).all())
+    group = torch.bucketize(torch.arange(3, M - 2), off[1:], right=True).to(DEV)
+    xs = x[3:M - 2].double()
+    y, mag = torch.empty(M - 5, N, dtype=torch.float64, device=DEV), torch.empty(M - 5, N, dtype=torch.float64, device=DEV)
+    for a in range(0, M - 5, 4096):
+        w = W[group[a:a + 4096]]
+        y[a:a + 4096], mag[a:a + 4096] = torch.einsum("mk,mnk->mn", xs[a:a + 4096], w), torch.einsum("mk,mnk->mn", xs[a:a + 4096].abs(), w.abs())
+    bound = (K / 16 + 80) * 2.0 ** -23 * mag + 2.0 ** -23 * y.abs()
+    assert bool(((out[3:M - 2].double() - y).abs() <= bound).all())
+
+
+def test_a_model_whose_experts_no_tile_divides(quant):
+    """Rows between the experts' products of 5,503 elements: too long for the products of few rows, no whole units for the tensor cores."""
+    import helpers
+    import moe_b200
+
+    config = {**helpers.CONFIG_A, "moe_intermediate_size": 5503, "num_hidden_layers": 2}
+    held, same = [moe_b200.random_model(config, seed=3, weights="int4") for _ in range(2)]
+    rows = []
+    for b in same.blocks:                 # the same numbers in bfloat16
+        for p in b.parts():
+            for name, w in list(vars(p).items()):
+                if isinstance(w, quant.Weight4):
+                    setattr(p, name, quant.dequantize(w))
+            if hasattr(p, "whole_in_4_bits"):
+                p.whole_in_4_bits = False
+    for model in (held, same):
+        engine = moe_b200.Engine(model, max_tokens=512)
+        slots = [engine.new_sequence() for _ in range(2)]
+        got = [engine.step(slots, [list(range(20)), list(range(5, 40))], [[19], [34]]).float().clone()]
+        got.append(engine.step(slots, [[3], [4]], [[0], [0]]).float().clone())
+        model.rt.check()
+        rows.append(torch.stack(got))
+    far = float((rows[0] - rows[1]).abs().max() / rows[1].abs().max())
+    assert far < G.TOL_CUT_BF16, far
