@@ -230,8 +230,8 @@ class Part:
 
     def hold(self, rt: Runtime, w: torch.Tensor, pair: bool = False):
         """What the part keeps of a matrix (or a stack of them) that only products read: the tensor, or where the model holds its weights in 4
-        bits, and this one came in bfloat16, its ``Weight4``.  ``pair``: gate rows and up rows of a gated feed-forward."""
-        if not rt.weight_group or w.dtype != torch.bfloat16:
+        bits its ``Weight4``, whether the checkpoint has 16 or 32 bits of it.  ``pair``: gate rows and up rows of a gated feed-forward."""
+        if not rt.weight_group:
             return w
         from ..ops import quant
 

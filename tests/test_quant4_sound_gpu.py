@@ -7,7 +7,7 @@ import torch
 
 import gpu_util as G
 import quant4_util as Q
-from test_quant4_gpu import BF, DEV, fine, quant, status, weight  # noqa: F401  (quant: a fixture)
+from test_quant4_gpu import BF, DEV, _designs as designs, fine, quant, status, weight  # noqa: F401  (quant: a fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -272,3 +272,84 @@ def test_a_model_whose_experts_no_tile_divides(quant):
         rows.append(torch.stack(got))
     far = float((rows[0] - rows[1]).abs().max() / rows[1].abs().max())
     assert far < G.TOL_CUT_BF16, far
+
+
+# ------------------------------------------------------------------------------------------------ models
+def parts_of(model):
+    """Every part of every block, those inside others too."""
+    found = []
+
+    def add(p):
+        found.append(p)
+        for _, sub in getattr(p, "subs", []):
+            add(sub)
+
+    for b in model.blocks:
+        for p in b.parts():
+            add(p)
+    return found
+
+
+def held_by(part, quant):
+    return {n: w for n, w in vars(part).items() if isinstance(w, quant.Weight4)}
+
+
+def logits_of(model, prompts, steps=3):
+    import moe_b200
+
+    vocab = model.spec.vocab_size
+    engine = moe_b200.Engine(model, max_tokens=4096)
+    slots = [engine.new_sequence() for _ in prompts]
+    got = [engine.step(slots, prompts, [[len(p) - 1] for p in prompts]).float().clone()]
+    for i in range(steps):
+        got.append(engine.step(slots, [[(7 * i + j) % vocab] for j in range(len(slots))], [[0]] * len(slots)).float().clone())
+    model.rt.check()
+    return torch.cat(got)
+
+
+DESIGNS = [n for n, _ in designs()]
+
+
+@pytest.mark.parametrize("which", range(len(DESIGNS)), ids=DESIGNS)
+def test_a_model_of_32_bit_weights_is_held_in_4_bits(quant, which, monkeypatch):
+    """Quantised from the 32-bit values; against the same model whose matrices are the 4-bit ones' values in bfloat16."""
+    import moe_b200
+    from moe_b200.parts.base import Part
+
+    _, config = designs()[which]
+    held = moe_b200.random_model(config, seed=6, stored_dtype="float32", weights="int4")
+    assert any(held_by(p, quant) for p in parts_of(held))
+    with monkeypatch.context() as m:
+        m.setattr(Part, "hold", lambda self, rt, w, pair=False: quant.dequantize(quant.quantize(w.contiguous(), 64, pair=pair)))
+        same = moe_b200.random_model(config, seed=6, stored_dtype="float32")
+    gen = torch.Generator().manual_seed(which)
+    prompts = [torch.randint(0, held.spec.vocab_size, (n,), generator=gen).tolist() for n in (9, 1, 30)]
+    a, b = logits_of(held, prompts), logits_of(same, prompts)
+    far = float((a - b).abs().max() / b.abs().max())
+    assert far < G.TOL_CUT_BF16, far
+
+
+@pytest.mark.parametrize("dtype", ["float16", "float32"])
+def test_a_folder_of_another_float_type_is_held_in_4_bits(quant, dtype, tmp_path, model_dirs):
+    """Every matrix is what the quantiser makes of the stored numbers."""
+    import moe_b200
+    from moe_b200.weights.safetensors_io import write_safetensors
+    from moe_b200.weights.store import SafetensorsStore
+
+    d = model_dirs.get("A", "float32", seed=2, std=0.02)
+    if dtype == "float16":
+        import shutil
+
+        store = SafetensorsStore(d)
+        tensors = {n: store.raw(n).to(torch.float16) for n in store.names()}
+        d16 = tmp_path / "half"
+        d16.mkdir()
+        shutil.copy(f"{d}/config.json", d16 / "config.json")
+        write_safetensors(str(d16 / "model.safetensors"), tensors)
+        d = str(d16)
+    store = SafetensorsStore(d)
+    model = moe_b200.load_model(d, weights="int4")
+    for i, b in enumerate(model.blocks):
+        assert {"wqkv", "wo"} <= set(held_by(b.mixer, quant)) and {"w_gu", "w_down", "ws_gu", "ws_down"} <= set(held_by(b.ffn, quant))
+        stored = store.raw(f"model.layers.{i}.self_attn.o_proj.weight").float()
+        assert torch.equal(quant.dequantize(b.mixer.wo).double().cpu(), Q.plain_values(stored, 64))
