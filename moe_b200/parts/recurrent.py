@@ -92,7 +92,7 @@ class WKVMixer(Part):
         self.mu = torch.stack([tensors[n["mu_" + s]].to(torch.float32) for s in _STREAMS]).contiguous()
         ws = [tensors[n[s]] for s in ("r", "k", "v", "g")]
         dt = ws[0].dtype if all(w.dtype == ws[0].dtype for w in ws) else torch.float32
-        self.w_rkvg = torch.stack([w.to(dt) for w in ws]).contiguous()          # [4, inner, hidden]
+        self.w_rkvg = self.hold(rt, torch.stack([w.to(dt) for w in ws]).contiguous())          # [4, inner, hidden]
         # the decay's two small projections stay 32-bit arithmetic in both dtypes
         w1 = tensors[n["w1"]]
         self.w1 = w1.to(torch.float32).contiguous()

@@ -307,10 +307,9 @@ def logits_of(model, prompts, steps=3):
     return torch.cat(got)
 
 
-DESIGNS = [n for n, _ in designs()]
 
 
-@pytest.mark.parametrize("which", range(len(DESIGNS)), ids=DESIGNS)
+@pytest.mark.parametrize("which", range(len(designs())), ids=[n for n, _ in designs()])
 def test_a_model_of_32_bit_weights_is_held_in_4_bits(quant, which, monkeypatch):
     """Quantised from the 32-bit values; against the same model whose matrices are the 4-bit ones' values in bfloat16."""
     import moe_b200
@@ -353,3 +352,42 @@ def test_a_folder_of_another_float_type_is_held_in_4_bits(quant, dtype, tmp_path
         assert {"wqkv", "wo"} <= set(held_by(b.mixer, quant)) and {"w_gu", "w_down", "ws_gu", "ws_down"} <= set(held_by(b.ffn, quant))
         stored = store.raw(f"model.layers.{i}.self_attn.o_proj.weight").float()
         assert torch.equal(quant.dequantize(b.mixer.wo).double().cpu(), Q.plain_values(stored, 64))
+
+
+def all_designs():
+    import importlib
+
+    import helpers
+
+    found = [("qwen " + n, c) for n, c in helpers.CONFIGS.items()]
+    for u in ("supevik", "fogapel", "zosipel", "divadra", "ditazen", "kulanex"):
+        m = importlib.import_module(u + "_util")
+        found += [(f"{u} {n}", m.config_dict(n)) for n in ("mix", "lean", "ones", "wide", "odd") if n in m.CONFIGS]
+    return found
+
+
+# What a part keeps in 16 bits: routers, the narrow products behind a decay's logits (``w1_3``: as three copies), a latent's products a head
+IN_16_BITS = {"w_router", "w_router3", "w1_3", "w_low1", "w_low2", "w_qc", "w_cv"}
+
+
+@pytest.mark.parametrize("which", range(len(all_designs())), ids=[n for n, _ in all_designs()])
+def test_the_matrices_of_a_model_are_held_in_4_bits(quant, which, monkeypatch):
+    """All that the parts multiply by, and prompts so long that routers, norms and branches take their forms of many tokens, against the same model whose
+    matrices are the 4-bit ones' values in bfloat16."""
+    import moe_b200
+    from moe_b200.parts.base import Part
+
+    _, config = all_designs()[which]
+    held = moe_b200.random_model(config, seed=8, weights="int4")
+    for p in parts_of(held):
+        assert p.category not in ("mixer", "ffn") or hasattr(p, "subs") or held_by(p, quant), p.kind
+        left = {n for n, w in vars(p).items() if isinstance(w, torch.Tensor) and w.dtype == BF and w.dim() > 1}
+        assert left <= IN_16_BITS, (p.kind, left)
+    with monkeypatch.context() as m:
+        m.setattr(Part, "hold", lambda self, rt, w, pair=False: quant.dequantize(quant.quantize(w.contiguous(), 64, pair=pair)))
+        same = moe_b200.random_model(config, seed=8)
+    gen = torch.Generator().manual_seed(which)
+    prompts = [torch.randint(0, held.spec.vocab_size, (n,), generator=gen).tolist() for n in (9, 290, 1)]
+    a, b = logits_of(held, prompts), logits_of(same, prompts)
+    far = float((a - b).abs().max() / b.abs().max())
+    assert far < G.TOL_CUT_BF16, far
