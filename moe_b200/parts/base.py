@@ -225,8 +225,8 @@ class Part:
             n += k
         return float(n)
 
-    # whether the part holds its matrices in 4 bits (``hold``)
-    in_4_bits = False
+    # elements that the part holds in 4 bits (``hold``)
+    held_elements = 0
 
     def hold(self, rt: Runtime, w: torch.Tensor, pair: bool = False):
         """What the part keeps of a matrix (or a stack of them) that only products read: the tensor, or where the model holds its weights in 4
@@ -235,15 +235,19 @@ class Part:
             return w
         from ..ops import quant
 
-        self.in_4_bits = True
+        self.held_elements = self.held_elements + w.numel()
         held = quant.quantize(w.contiguous(), rt.weight_group, pair=pair, status=rt.status)
         rt._fresh.append(held)
         return held
 
     def step_bytes(self, num_tokens: int, rt: Runtime) -> float:
-        """Bytes of ``step_elements``: a part that holds its matrices in 4 bits counts all its elements so."""
-        each = 0.5 + 2.0 / rt.weight_group if self.in_4_bits else 2 if rt.is_bf16 else 4
-        return self.step_elements(num_tokens) * each
+        """Bytes of ``step_elements``, those that are held in 4 bits counted so."""
+        return self._bytes(self.step_elements(num_tokens), self.held_elements, rt)
+
+    @staticmethod
+    def _bytes(elements: float, held: float, rt: Runtime) -> float:
+        held = min(held, elements)     # (rows of zeros that fill a matrix up are held, and no element of the model's)
+        return (elements - held) * (2 if rt.is_bf16 else 4) + (held * (0.5 + 2.0 / rt.weight_group) if held else 0)
 
     def bind(self, tensors: Dict[str, torch.Tensor], rt: Runtime) -> None:
         """Take ownership of the loaded tensors (re-laying them out is allowed)."""

@@ -274,6 +274,10 @@ class RoutedExperts(Part):
     def step_elements(self, num_tokens):
         """The router, the shared expert, and the experts that ``num_tokens`` tokens are expected to
         touch if each picks ``top_k`` of them evenly: E (1 - (1 - k/E)^tokens)."""
+        return sum(self._step_elements(num_tokens))
+
+    def _step_elements(self, num_tokens):
+        """(those that every token reads, those of the experts)"""
         dense = sparse = 0
         for ts in self.tensors().values():
             n = 1
@@ -283,8 +287,12 @@ class RoutedExperts(Part):
                 sparse += n
             else:
                 dense += n
-        touched = 1.0 - (1.0 - self.k / self.E) ** max(num_tokens, 0)
-        return dense + sparse * touched
+        return dense, sparse * (1.0 - (1.0 - self.k / self.E) ** max(num_tokens, 0))
+
+    def step_bytes(self, num_tokens, rt):
+        dense, sparse = self._step_elements(num_tokens)
+        experts = 3 * self.E * self.size * self.hidden if self.held_elements else 0        # (held with the shared expert, if at all)
+        return self._bytes(dense, self.held_elements - experts, rt) + self._bytes(sparse, experts, rt)
 
     def bind(self, tensors, rt):
         super().bind(tensors, rt)

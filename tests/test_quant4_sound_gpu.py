@@ -391,3 +391,31 @@ def test_the_matrices_of_a_model_are_held_in_4_bits(quant, which, monkeypatch):
     a, b = logits_of(held, prompts), logits_of(same, prompts)
     far = float((a - b).abs().max() / b.abs().max())
     assert far < G.TOL_CUT_BF16, far
+
+
+@pytest.mark.parametrize("which", range(len(all_designs())), ids=[n for n, _ in all_designs()])
+def test_the_bytes_of_a_step_are_those_that_are_held(quant, which):
+    """Elements in 4 bits at theirs, all others at 16; so many tokens that every expert is read, and one."""
+    import moe_b200
+    from moe_b200 import cli
+
+    _, config = all_designs()[which]
+    group = (32, 64, 128)[which % 3]
+    model = moe_b200.random_model(config, seed=8, weights="int4", weight_group=group)
+    each = 0.5 + 2 / group
+    for p in parts_of(model):
+        if hasattr(p, "subs"):
+            continue
+        held = held_by(p, quant)
+        full = p.step_elements(1 << 20)
+        # (up to seven rows of zeros a matrix are held beside the model's own, and differential attention lays some rows out twice: what a step counts are the model's)
+        in4 = min(full, sum(w.G * w.N * w.K for w in held.values()))
+        room = 2 * sum(7 * w.K for w in held.values())
+        assert abs(p.step_bytes(1 << 20, model.rt) - ((full - in4) * 2 + in4 * each)) <= room, p.kind
+        if p.kind == "routed_experts":
+            experts = p.w_gu.N * p.w_gu.K * p.E + p.w_down.N * p.w_down.K * p.E
+            want = (full - in4) * 2 + (in4 - experts) * each + experts * each * p.k / p.E
+            assert abs(p.step_bytes(1, model.rt) - want) <= 1e-9 * want
+    rest, _ = cli.step_bytes(model, [10])
+    blocks = sum(p.step_bytes(1, model.rt) for e in model.spec.schedule for p in model.blocks[e.layer].parts())
+    assert rest > blocks > 0
