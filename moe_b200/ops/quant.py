@@ -281,6 +281,12 @@ def _splits(M: int, N: int, w: Weight4, place: int) -> int:
     return 1
 
 
+def takes_experts(tokens: int, top_k: int, gate_up: Weight4) -> bool:
+    """Whether ``experts4`` takes so many tokens and picks through these experts."""
+    return (tokens <= EXPERTS_TOKENS and gate_up.G <= GROUPS_A_LAUNCH and tokens * top_k <= 128
+            and bool((_lib or lib()).moe_q4_holds_rows(gate_up.K, gate_up.group, 1)))
+
+
 def experts4(x: torch.Tensor, topk_idx: torch.Tensor, topk_w: torch.Tensor, gate_up: Weight4, down: Weight4, out: torch.Tensor, *,
              shared_gate_up: Optional[Weight4] = None, shared_down: Optional[Weight4] = None, shared_gate: Optional[torch.Tensor] = None,
              status=None) -> bool:
@@ -291,7 +297,8 @@ def experts4(x: torch.Tensor, topk_idx: torch.Tensor, topk_w: torch.Tensor, gate
     x: bfloat16 [T, H]; topk_idx int32 and topk_w float32 [T, k]; gate_up: a pair's stack [E, 2 I, H], down: [E, H, I]; the shared expert's two
     likewise without the stack, shared_gate float32 [T] (None: 1); out: float32 or bfloat16 [T, H].  An index of -1 is no pick
     (all of a row's: zeros but for the shared expert), any other outside [0, E) is reported through ``status`` and taken for none.  False, with
-    nothing launched, for more tokens, more than 1,024 experts or 128 picks, or rows that shared memory does not hold (H beyond 6,000 or so)."""
+    nothing launched, for what ``takes_experts`` says no to: more tokens, more than 1,024 experts or 128 picks, or rows that shared memory does not hold (H beyond
+    6,000 or so)."""
     place = x.get_device()
     _here(place, "experts4")
     T, H, ldx = _matrix(x, place, "x", False)
@@ -315,7 +322,7 @@ def experts4(x: torch.Tensor, topk_idx: torch.Tensor, topk_w: torch.Tensor, gate
         raise core.KernelError("experts4: the weights of a layer have one group size")
     pi, pw = _on(topk_idx, place, "topk_idx", torch.int32), _on(topk_w, place, "topk_w", torch.float32)
     pg, ps = _on(shared_gate, place, "shared_gate", torch.float32, T), _on(status, place, "status", torch.int32)
-    if T > EXPERTS_TOKENS or E > 1024 or T * k > 128:
+    if not takes_experts(T, k, gate_up):
         return False
     if not T:
         return True
@@ -326,8 +333,6 @@ def experts4(x: torch.Tensor, topk_idx: torch.Tensor, topk_w: torch.Tensor, gate
     scratch = torch.empty((slots * -(-size // 64) + -(-shared // 64)) * 3072, dtype=torch.uint8, device=x.device)
     code = L.moe_experts_q4(x.data_ptr(), ldx, T, H, pi, pw, k, E, size, *gate_up.pointers, *down.pointers, shared, *s, pg, group, scratch.data_ptr(),
                             scratch.numel(), out.data_ptr(), out.dtype is _BF16, ldo, early, ps, stream)
-    if code == -1:
-        return False
     core._ok(code, "experts4")
     if not early:
         for w in weights:

@@ -15,7 +15,7 @@ import torch
 
 from ..ops import core
 from ..ops.linear import grouped_linear, grouped_swiglu_linear, linear, swiglu_linear
-from ..ops.quant import EXPERTS_TOKENS, Weight4, experts4, gemm4
+from ..ops.quant import Weight4, experts4, gemm4, takes_experts
 from .base import Activations, LazyDelta, Part, TensorSpec, register_part
 
 
@@ -442,13 +442,11 @@ class RoutedExperts(Part):
     def _whole_in_4_bits(self, rt, h, batch, routed):
         """Router (where ``routed`` does not bring its picks), then all experts, the shared one and the combine; None where they do not fit."""
         T = h.act.shape[0]
-        if not self.whole_in_4_bits or T > EXPERTS_TOKENS or self.weight_input or h.act.dtype != torch.bfloat16:
+        if not self.whole_in_4_bits or self.weight_input or h.act.dtype != torch.bfloat16 or not takes_experts(T, self.k, self.w_gu):
             return None
         topk_idx, topk_w, sg = routed[:3] if routed is not None else self.route(rt, h, batch)
         out = rt.empty((T, self.hidden), torch.float32)
-        if not experts4(h.act, topk_idx, topk_w, self.w_gu, self.w_down, out, shared_gate_up=self.ws_gu, shared_down=self.ws_down, shared_gate=sg,
-                        status=rt.status):
-            return None
+        experts4(h.act, topk_idx, topk_w, self.w_gu, self.w_down, out, shared_gate_up=self.ws_gu, shared_down=self.ws_down, shared_gate=sg, status=rt.status)
         self._record(topk_idx, topk_w)
         return out
 

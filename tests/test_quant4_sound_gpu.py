@@ -419,3 +419,41 @@ def test_the_bytes_of_a_step_are_those_that_are_held(quant, which):
     rest, _ = cli.step_bytes(model, [10])
     blocks = sum(p.step_bytes(1, model.rt) for e in model.spec.schedule for p in model.blocks[e.layer].parts())
     assert rest > blocks > 0
+
+
+@pytest.mark.parametrize("change", [dict(hidden_size=6400, num_experts=300), dict(num_experts=1100), dict(num_experts=300, num_experts_per_tok=20)])
+def test_a_layer_that_its_kernels_do_not_take_is_routed_once(quant, change, monkeypatch):
+    """Too wide, too many experts, or too many picks for the layer of few tokens: the products take it one by one, from the picks of one router."""
+    import helpers
+    import moe_b200
+    from moe_b200.ops import core
+
+    config = {**helpers.CONFIG_A, **change}
+    model = moe_b200.random_model(config, seed=4, weights="int4")
+    ffn = model.blocks[0].ffn
+    tokens = 8
+    assert not quant.takes_experts(tokens, ffn.k, ffn.w_gu) and quant.takes_experts(1, 2, quant.quantize(torch.ones(4, 32, 64, device=DEV), pair=True))
+    x = torch.randn(tokens, model.spec.hidden_size, device=DEV)
+
+    class H:
+        act, f32, split = x.to(BF), x, None
+
+    calls, rt = [], model.rt
+    for name in ("router", "route_dispatch", "router_topk"):
+        real = getattr(core, name)
+        monkeypatch.setattr(core, name, lambda *a, _real=real, _name=name, **kw: (calls.append(_name), _real(*a, **kw))[1])
+    out = ffn.forward(rt, H, type("B", (), dict(seq_of_token=None))())
+    rt.check()
+    assert len(calls) == 1, calls
+    topk_idx, topk_w, sg = ffn.route(rt, H, type("B", (), dict(seq_of_token=None))())
+    GU, D = [quant.dequantize(w).double() for w in (ffn.w_gu, ffn.w_down)]
+    SGU, SD = [quant.dequantize(w).double() for w in (ffn.ws_gu, ffn.ws_down)]
+    # (between the two products bfloat16 rows: 2^-8 of each term)
+    mag, want = torch.zeros_like(out, dtype=torch.float64), torch.zeros_like(out, dtype=torch.float64)
+    for t in range(tokens):
+        pairs = [(GU[e], D[e], float(f)) for e, f in zip(topk_idx[t].tolist(), topk_w[t].tolist())] + [(SGU, SD, 1.0 if sg is None else float(sg[t]))]
+        for gu, d, f in pairs:
+            a = Q.gated("silu", *(gu @ H.act[t].double()).chunk(2))
+            want[t] += f * (d @ a)
+            mag[t] += f * (d.abs() @ a.abs())
+    assert bool(((out.double() - want).abs() <= 2.0 ** -7 * mag + 1e-30).all())
