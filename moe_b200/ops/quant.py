@@ -3,7 +3,7 @@
 A ``Weight4`` stands for a matrix [N, K] or a stack of them [G, N, K].  ``group`` (32, 64 or 128) neighbouring elements of a
 row share a scale s = max |w| / 7 rounded to five significant bits; an element is q s with q = w / s rounded, a whole number from -7 to 7.  q s
 has at most eight significant bits, so it is a bfloat16: a product over a ``Weight4`` is the product over ``dequantize`` of it, but for the
-order of the 32-bit sums.  0.5 + 2 / group bytes an element.
+order of the 32-bit sums (and silu's exponential, quicker for many rows: 2 + 1.2 |g| ulp).  0.5 + 2 / group bytes an element.
 
     w4 = quantize(w, group=64)                 # w: float32 or bfloat16, on the device
     gemm4(x, w4, out, bias=b)                  # out = x w^T (+ b); x bfloat16 [M, K], any M

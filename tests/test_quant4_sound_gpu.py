@@ -457,3 +457,36 @@ def test_a_layer_that_its_kernels_do_not_take_is_routed_once(quant, change, monk
             want[t] += f * (d @ a)
             mag[t] += f * (d.abs() @ a.abs())
     assert bool(((out.double() - want).abs() <= 2.0 ** -7 * mag + 1e-30).all())
+
+
+# ------------------------------------------------------------------------------------------------ the gate's function
+@pytest.mark.parametrize("M,groups", [(4, 0), (20, 0), (64, 0), (300, 0), (200, 4), (1200, 4)])
+def test_gates_far_from_zero(quant, M, groups):
+    """Every form at gates down to -100 and up to 100 whose sums are exact (one element of x is not zero), so that only silu(g) u is off.  Few rows: an exponential of 2 ulp
+    and three roundings, below 2^-20 of it; the divisor is infinite from -88.73 on, and the zero that is left off by 88.73 e^-88.73 = 2.6e-37 < 2^-121 at most.  The tensor
+    cores' epilogue: an exponential of 2 + 1.2 |g| ulp, a quotient of 2, two roundings, (5 + 1.2 |g|) 2^-23; zero from a divisor of 2^126 on, 88 2^-126 < 2^-119."""
+    K, half = 64, 512
+    gen = torch.Generator(device=DEV)
+    gen.manual_seed(M)
+    G_ = max(groups, 1)
+    w = torch.zeros(G_, 2 * half, K, device=DEV)
+    w[:, :half, 9] = torch.linspace(-7, 7, half, device=DEV).round()              # whole numbers up to 7: held as they are
+    w[:, half:, 9] = torch.randint(1, 8, (G_, half), device=DEV, generator=gen).float()
+    w[:, :, 20] = 7                       # (the scale of every group of 64 is 1; x is zero there)
+    shape = w.shape if groups else w.shape[1:]
+    w4 = quant.quantize(w.reshape(shape), pair=True)
+    assert torch.equal(quant.dequantize(w4).float().reshape(w.shape), w)
+    x = torch.zeros(M, K, dtype=BF, device=DEV)
+    x[:, 9] = torch.linspace(0.01, 14.3, M, device=DEV).to(BF)
+    off = torch.arange(0, M + 1, M // groups, dtype=torch.int32, device=DEV) if groups else None
+    st, out = status(), torch.empty(M, half, device=DEV)
+    quant.gemm4(x, w4, out, swiglu=True, group_offsets=off, status=st)
+    fine(st)
+    each = w.double().repeat_interleave(M // G_, dim=0) if groups else w.double().expand(M, -1, -1)
+    g, u = [x[:, 9].double().unsqueeze(1) * each[:, h * half:(h + 1) * half, 9] for h in (0, 1)]
+    y = g * torch.sigmoid(g) * u
+    assert float(g.min()) < -99 and float(g.max()) > 99
+    few = M <= quant.FEW_ROWS
+    far = (out.double() - y).abs()
+    room = 2.0 ** -20 * y.abs() + u.abs() * 2.0 ** -121 if few else (5 + 1.2 * g.abs()) * 2.0 ** -23 * y.abs() + u.abs() * 2.0 ** -119
+    assert bool((far <= room).all()), float((far / room).max())
