@@ -46,7 +46,8 @@ def load_model(model_dir: str, dtype="bfloat16", device="cuda", weights=None, we
 
     ``weights="int4"`` (with dtype bfloat16): the matrices of attention, recurrent mixers and feed-forwards, routed experts among them, are held in
     4 bits, ``weight_group`` (32, 64 or 128) neighbouring elements of a row to a scale (``ops.quant``), whatever floating type the folder stores them in;
-    embedding, output projection, joins, routers, norms, a latent's products a head and the narrow products behind a decay's logits stay as they are."""
+    embedding, output projection, joins, routers, norms, a latent's products a head and the narrow products behind a decay's logits stay as they are.
+    Raises ``ops.core.KernelError`` where one of them is an infinity or a NaN."""
     from .models import DecoderModel
 
     arch, typed = parse_config(read_config_json(model_dir))

@@ -139,6 +139,7 @@ def _load(path: str, opt, device="cuda"):
     """The model of the command: a folder, or with ``--random CONFIG.json`` random weights of that
     configuration drawn on the device from ``--seed`` (nothing is written)."""
     import moe_b200
+    from .ops.core import KernelError
 
     dtype = opt.get("dtype", "bfloat16")
     # (``info`` says what a folder holds, and loads on the CPU, which has no 4-bit weights)
@@ -149,7 +150,7 @@ def _load(path: str, opt, device="cuda"):
                 cfg = json.load(f)
             return moe_b200.random_model(cfg, seed=_num(opt, "seed", 0, int), dtype=dtype, device=device, **held)
         return moe_b200.load_model(path, dtype=dtype, device=device, **held)
-    except (moe_b200.ConfigError, moe_b200.WeightError, ValueError, OSError) as e:
+    except (moe_b200.ConfigError, moe_b200.WeightError, KernelError, ValueError, OSError) as e:      # (KernelError: a weight that is to be held in 4 bits is no number)
         fail(e)
 
 

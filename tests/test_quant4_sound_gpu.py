@@ -490,3 +490,26 @@ def test_gates_far_from_zero(quant, M, groups):
     far = (out.double() - y).abs()
     room = 2.0 ** -20 * y.abs() + u.abs() * 2.0 ** -121 if few else (5 + 1.2 * g.abs()) * 2.0 ** -23 * y.abs() + u.abs() * 2.0 ** -119
     assert bool((far <= room).all()), float((far / room).max())
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_a_folder_with_a_weight_that_is_no_number_is_refused_in_a_line(quant, bad, tmp_path, model_dirs, capsys):
+    import shutil
+
+    import moe_b200
+    from moe_b200 import cli
+    from moe_b200.ops import core
+    from moe_b200.weights.safetensors_io import write_safetensors
+    from moe_b200.weights.store import SafetensorsStore
+
+    d = model_dirs.get("A", "bfloat16", seed=2, std=0.02)
+    store = SafetensorsStore(d)
+    tensors = {n: store.raw(n).clone() for n in store.names()}
+    tensors["model.layers.1.self_attn.o_proj.weight"][3, 5] = bad
+    shutil.copy(f"{d}/config.json", tmp_path / "config.json")
+    write_safetensors(str(tmp_path / "model.safetensors"), tensors)
+    with pytest.raises(core.KernelError, match="not finite"):
+        moe_b200.load_model(str(tmp_path), weights="int4")
+    with pytest.raises(SystemExit):
+        cli.main(["run", str(tmp_path), "--ids", "5", "-n", "1", "--weights", "int4"])
+    assert "not finite" in capsys.readouterr().err
