@@ -142,9 +142,11 @@ def _load(path: str, opt, device="cuda"):
     from .ops.core import KernelError
 
     dtype = opt.get("dtype", "bfloat16")
-    # (``info`` says what a folder holds, and loads on the CPU, which has no 4-bit weights)
-    held = {} if device == "cpu" else dict(weights=opt.get("weights"), weight_group=_num(opt, "weight-group", 64, int))
+    held = dict(weights=opt.get("weights"), weight_group=_num(opt, "weight-group", 64, int))
     try:
+        if device == "cpu":      # (``info`` says what a folder holds, and loads on the CPU, which has no 4-bit weights)
+            moe_b200._weight_group(*held.values())
+            held = {}
         if "random" in opt:
             with open(opt["random"], encoding="utf-8") as f:
                 cfg = json.load(f)

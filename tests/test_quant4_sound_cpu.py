@@ -19,3 +19,14 @@ def test_a_wait_is_called_by_its_own_name():
         text = core.wait_site(site)
         assert word in text and "MMA" not in text and "few rows" in text, text
     assert "MMA issuer" in core.wait_site(0x53)
+
+
+@pytest.mark.parametrize("options", [["--weights", "int3"], ["--weights", "int4", "--weight-group", "48"]])
+def test_info_refuses_weights_that_there_are_none_of(model_dirs, options, capsys):
+    from moe_b200 import cli
+
+    d = model_dirs.get("A", "bfloat16", seed=1, std=0.02)
+    with pytest.raises(SystemExit):
+        cli.main(["info", d, *options])
+    assert "weight" in capsys.readouterr().err
+    assert cli.main(["info", d, "--weights", "int4"]) == 0
