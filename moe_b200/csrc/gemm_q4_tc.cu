@@ -38,7 +38,7 @@ using q4::Weight;
 
 constexpr int BK = 64, BN = 256, NBUF = 2, STAGES_MAX = 8;
 constexpr int BOX = 64, BOX_BYTES = BOX * BK * 2, ROOM = 200 * 1024;      // ROOM: bytes for stages
-constexpr int TMEM_COLS = 512, MAX_GROUPS = 1024, MAX_CLUSTER = 8;
+constexpr int TMEM_COLS = 512, MAX_GROUPS = 1024, MAX_CLUSTER = 4;
 static_assert(NBUF * BN <= TMEM_COLS, "tensor memory");
 // WIDE: 256 features, the MMA's columns, x 128 rows; else 128 features, the MMA's lanes, x up to 256 rows
 template <bool WIDE>
@@ -547,7 +547,7 @@ int launch(const CUtensorMap& map, const Args& p, unsigned ctas, bool early, cud
 }  // namespace
 
 // The same product as moe_gemm_q4 by the kernel above.  Returns -1, with nothing launched, for what it does not take: K or a row pitch of x that is no
-// multiple of 8, an unaligned x, more than 1,024 groups.
+// multiple of 8, an unaligned x, more than 1,024 groups.  splits: CTAs of a cluster that share a dense tile's k, 1 to 4.
 MOE_API int moe_gemm_q4_tc(const void* x, int ldx, int M, const void* codes, const void* scales, int G, int N, int K, int group, int pair, void* out,
                            int out_bf16, int ldo, const float* bias, const int* offsets, int act, float act_param, int splits, int early, int* status, cudaStream_t stream) {
     if (M <= 0 || N <= 0) return 0;
