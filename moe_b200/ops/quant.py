@@ -139,6 +139,13 @@ def _on(t: Optional[torch.Tensor], place: int, name: str, dtype, numel: Optional
     return t.data_ptr()
 
 
+def _status(t: Optional[torch.Tensor], place: int):
+    """(Faults and, beside them, where the first wait ran out.)"""
+    if t is not None and t.numel() < 2:
+        raise core.KernelError("status: expected what core.new_status makes")
+    return _on(t, place, "status", torch.int32)
+
+
 def _matrix(t: torch.Tensor, place: int, name: str, wide: bool):
     """(rows, columns, row pitch) of a matrix with dense rows, bfloat16 or (``wide``) float32."""
     dtype = t.dtype
@@ -185,7 +192,7 @@ def quantize(w: torch.Tensor, group: int = 64, *, pair: bool = False, status=Non
     codes = torch.empty(G * strips * -(-K // 64) * 512, dtype=torch.uint8, device=device)
     scales = torch.empty(G * strips * -(-K // group) * 16, dtype=torch.bfloat16, device=device)
     core._ok((_lib or lib()).moe_q4_quantize(w.data_ptr(), core._dt(w), G, N, K, group, pair, codes.data_ptr(), scales.data_ptr(),
-                                             _on(status, w.get_device(), "status", torch.int32), core._stream()), "quantize")
+                                             _status(status, w.get_device()), core._stream()), "quantize")
     return Weight4(codes, scales, w.shape, group, pair)
 
 
@@ -232,7 +239,7 @@ def gemm4(x: torch.Tensor, w: Weight4, out: torch.Tensor, *, swiglu: bool = Fals
         raise core.KernelError("gemm4: a stack needs group_offsets")
     pb = None if bias is None else _on(bias, place, "bias", _F32, N)
     po = None if group_offsets is None else _on(group_offsets, place, "group_offsets", torch.int32, w.G + 1)
-    st = _on(status, place, "status", torch.int32)
+    st = _status(status, place)
     if not M:
         return out
     L, stream = _lib or lib(), core._stream()
@@ -321,7 +328,7 @@ def experts4(x: torch.Tensor, topk_idx: torch.Tensor, topk_w: torch.Tensor, gate
     if down.group != group:
         raise core.KernelError("experts4: the weights of a layer have one group size")
     pi, pw = _on(topk_idx, place, "topk_idx", torch.int32), _on(topk_w, place, "topk_w", torch.float32)
-    pg, ps = _on(shared_gate, place, "shared_gate", torch.float32, T), _on(status, place, "status", torch.int32)
+    pg, ps = _on(shared_gate, place, "shared_gate", torch.float32, T), _status(status, place)
     if not takes_experts(T, k, gate_up):
         return False
     if not T:

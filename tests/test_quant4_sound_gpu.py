@@ -513,3 +513,16 @@ def test_a_folder_with_a_weight_that_is_no_number_is_refused_in_a_line(quant, ba
     with pytest.raises(SystemExit):
         cli.main(["run", str(tmp_path), "--ids", "5", "-n", "1", "--weights", "int4"])
     assert "not finite" in capsys.readouterr().err
+
+
+def test_a_status_without_room_for_what_is_reported_is_refused(quant):
+    from moe_b200.ops import core
+
+    (w4, _), (pair, _), (down, _) = weight(quant, (32, 64)), weight(quant, (2, 32, 64), pair=True), weight(quant, (2, 64, 16))
+    x, idx, w = torch.zeros(2, 64, dtype=BF, device=DEV), torch.zeros(2, 1, dtype=torch.int32, device=DEV), torch.ones(2, 1, device=DEV)
+    for n in (0, 1):
+        small = torch.zeros(n, dtype=torch.int32, device=DEV)
+        for call in (lambda: quant.quantize(torch.ones(32, 64, device=DEV), status=small), lambda: quant.gemm4(x, w4, torch.empty(2, 32, device=DEV), status=small),
+                     lambda: quant.experts4(x, idx, w, pair, down, torch.empty(2, 64, device=DEV), status=small)):
+            with pytest.raises(core.KernelError, match="status"):
+                call()
