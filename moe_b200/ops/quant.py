@@ -105,9 +105,14 @@ class Weight4:
         """(No ``torch.dtype``: whoever asks whether a weight is bfloat16 is told no.)"""
         return "int4"
 
+    def __reduce__(self):
+        """(A copy, or what is stored and read back, has tensors of its own: their addresses, and what has read them.)"""
+        return Weight4, (self.codes, self.scales, self.shape, self.group, self.pair)
+
     def settle(self) -> None:
         """Waits until the device has done what it was given, the writing of this weight with it."""
-        torch.cuda.synchronize(self.device)
+        if self.place >= 0:
+            torch.cuda.synchronize(self.device)
         self.read_on = None
 
     @property

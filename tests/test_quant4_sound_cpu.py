@@ -30,3 +30,19 @@ def test_info_refuses_weights_that_there_are_none_of(model_dirs, options, capsys
         cli.main(["info", d, *options])
     assert "weight" in capsys.readouterr().err
     assert cli.main(["info", d, "--weights", "int4"]) == 0
+
+
+def test_a_copy_of_a_weight_is_a_weight_of_its_own_tensors():
+    """Copied, and stored and read back: the addresses that kernels are given are those of the copy's tensors, and nobody has read them yet."""
+    import copy
+    import pickle
+
+    import test_quant4_cpu as T
+
+    w = T._w((3, 32, 70), 32, pair=True)
+    w.settle()
+    for c in (copy.deepcopy(w), pickle.loads(pickle.dumps(w))):
+        assert c.pointers == (c.codes.data_ptr(), c.scales.data_ptr()) and c.codes.data_ptr() != w.codes.data_ptr()
+        assert (c.shape, c.group, c.pair, c.place) == (w.shape, w.group, w.pair, w.place) and c.read_on == ()
+        assert bool((c.codes == w.codes).all())
+    assert copy.copy(w).codes is w.codes
