@@ -249,10 +249,10 @@ static inline int launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, si
     return (int)cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
 }
 
-// The same with thread-block clusters of `cluster_z` CTAs along grid.z (1: no clusters), and where `early` is false without the attribute.
+// The same with thread-block clusters of `cluster_z` CTAs along grid.z (1: no clusters).
 template <typename... KArgs, typename... Args>
-static inline int launch_pdl_if(bool early, void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
-                                int cluster_z, Args... args) {
+static inline int launch_pdl_cluster(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
+                                     int cluster_z, Args... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = block;
@@ -265,7 +265,7 @@ static inline int launch_pdl_if(bool early, void (*kernel)(KArgs...), dim3 grid,
         attr[n].val.clusterDim.x = 1, attr[n].val.clusterDim.y = 1, attr[n].val.clusterDim.z = (unsigned)cluster_z;
         n++;
     }
-    if (early && g_pdl_enabled) {
+    if (g_pdl_enabled) {
         attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
         attr[n].val.programmaticStreamSerializationAllowed = 1;
         n++;
@@ -273,11 +273,6 @@ static inline int launch_pdl_if(bool early, void (*kernel)(KArgs...), dim3 grid,
     cfg.attrs = attr;
     cfg.numAttrs = n;
     return (int)cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
-}
-template <typename... KArgs, typename... Args>
-static inline int launch_pdl_cluster(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
-                                     int cluster_z, Args... args) {
-    return launch_pdl_if(true, kernel, grid, block, smem, stream, cluster_z, args...);
 }
 
 // ---- thread-block clusters -------------------------------------------------------------------

@@ -182,6 +182,7 @@ struct Args {
     int top_k, E;
     uint8_t *frag, *sfrag;         // EXPERTS: [slot][frag_blocks] of TERMS_BLOCK bytes, see experts_down_kernel; the shared expert's
     int frag_blocks;
+    int early;                     // the weights may be read before what is in front of this launch has ended
     q4::Bits bits;
     q4::Waits waits;
 };
@@ -213,7 +214,8 @@ gemm_q4_direct_kernel(const __grid_constant__ Args p) {
         codes[m] = p.w.codes + s * blocks * 32 + lane;
         scales[m] = p.w.scales + s * p.w.qgroups * 8;
     }
-    bool waited = false;
+    bool waited = !p.early;
+    if (waited) pdl_sync();
     for (int row0 = 0; row0 < p.M; row0 += 8 * NT) {
         uint4 code[DEPTH][MT];
         uint32_t sc[DEPTH][MT][NS];
@@ -402,6 +404,7 @@ gemm_q4_stream_kernel(const __grid_constant__ Args p, const int stages) {
     if (warp >= TEAMS * TEAM_W) {
         // ---- copies of team q ---------------------------------------------------------------------------------------------------------------
         if (lane || p.waits.test_fault == 1) return;
+        if (MODE != GROUPED && !p.early) pdl_wait();
         const int q = warp - TEAMS * TEAM_W;
         int u = u0 + q, end = u0 < u1 ? run_end(u0) : u0, s = 0, it = 0;
         bool waits = MODE == EXPERTS;                    // for the picks
@@ -617,8 +620,8 @@ experts_down_kernel(const __grid_constant__ DownArgs p) {
     __shared__ __align__(16) float wt[PAIRS_MAX + 1][FEW];      // a slot's weight of each token; the last one's: the shared expert's gate
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3, strip0 = blockIdx.x * DOWN_MT, rank = blockIdx.z;
     if (p.S > 1) cluster_arrive();                              // (waited for below: this block's memory may be written to)
-    // The picks were written at least two kernels ago (this one's predecessor let it in behind its own wait): they, and the weights, are
-    // read before the wait.
+    // The picks and the weights were written at least two kernels ago (this one's predecessor let it in behind its own wait): they are read before the
+    // wait.
     const int pairs = p.T * p.top_k;
     if (warp == 0)
         find_picked(p.idx, p.T, p.top_k, p.E, nullptr, picked, lane);
@@ -774,13 +777,13 @@ int stream_stages(int blocks) {
 
 // max_units: the units of the launch, or more (blocks without one leave at once)
 template <int MODE, int NT, int GROUP, bool PAIR>
-int launch_stream(const Args& p, long long max_units, bool early, cudaStream_t stream) {
+int launch_stream(const Args& p, long long max_units, cudaStream_t stream) {
     const int stages = stream_stages<MODE, NT, GROUP>(p.w.blocks), bytes = Stream<NT, GROUP>::bytes(p.w.blocks, stages);
     auto kernel = gemm_q4_stream_kernel<MODE, NT, GROUP, PAIR>;
     static q4::SmemLimit limit;
     if (const int e = limit.lift((const void*)kernel)) return e;
     const int sms = q4::sm_count();
-    return launch_pdl_if(early, kernel, dim3((unsigned)(max_units < sms ? max_units : sms)), dim3(STREAM_THREADS), (size_t)bytes, stream, 1, p, stages);
+    return launch_pdl(kernel, dim3((unsigned)(max_units < sms ? max_units : sms)), dim3(STREAM_THREADS), (size_t)bytes, stream, p, stages);
 }
 
 // One weight, 8 NT rows (24: any number, in passes).  Streamed where a block a strip does not fit the SMs at once, three each, or, above eight rows, where there are
@@ -788,40 +791,40 @@ int launch_stream(const Args& p, long long max_units, bool early, cudaStream_t s
 // 6.9 / 6.0, of 8,192 x 5,632 16.7 / 10.6, of a pair 11,264 x 2,048, 352, 4.9 / 5.9, of a pair 14,336 x 2,048, 448, 7.4 / 6.7; 16 rows of 6,144 x 2,048, 192 units, 6.3 / 7.4,
 // of a pair 11,264 x 2,048, 352, 8.9 / 8.3; 24 rows of the two 8.6 / 8.8, 12.6 / 10.2.)
 template <int NT, int GROUP>
-int run_dense(const Args& p, bool pair, bool early, cudaStream_t stream) {
+int run_dense(const Args& p, bool pair, cudaStream_t stream) {
     const int half = pair ? p.w.strips / 2 : p.w.strips;
     const long long units = pair ? half : (half + 1) / 2;
     const int sms = q4::sm_count();
     if (p.M <= 8 * NT && (half > 3 * sms || (NT > 1 && 2 * units >= 3 * sms)) && stream_stages<DENSE, NT, GROUP>(p.w.blocks))
-        return pair ? launch_stream<DENSE, NT, GROUP, true>(p, units, early, stream) : launch_stream<DENSE, NT, GROUP, false>(p, units, early, stream);
-    return pair ? launch_pdl_if(early, gemm_q4_direct_kernel<2, NT, GROUP>, dim3(half), dim3(256), 0, stream, 1, p)
-                : launch_pdl_if(early, gemm_q4_direct_kernel<1, NT, GROUP>, dim3(half), dim3(256), 0, stream, 1, p);
+        return pair ? launch_stream<DENSE, NT, GROUP, true>(p, units, stream) : launch_stream<DENSE, NT, GROUP, false>(p, units, stream);
+    return pair ? launch_pdl(gemm_q4_direct_kernel<2, NT, GROUP>, dim3(half), 256, 0, stream, p)
+                : launch_pdl(gemm_q4_direct_kernel<1, NT, GROUP>, dim3(half), 256, 0, stream, p);
 }
 
 template <int GROUP>
-int run_gemm(const Args& p, bool pair, bool early, cudaStream_t stream) {
+int run_gemm(const Args& p, bool pair, cudaStream_t stream) {
     const int half = pair ? p.w.strips / 2 : p.w.strips;
     if (p.offsets) {
         const long long chunks = (long long)min(p.M, p.G) + p.M / 8;
         // Two tiles of rows at a time where groups have more than nine on average.  (us, one / two: 60 experts of a pair 2,816 x 2,048 at 8 rows an expert 61 / 63, at 10
         // 73 / 65, at 14 90 / 79; of 2,048 x 1,408 39 / 40, 45 / 42, 55 / 50.)
         if (p.M > 9 * p.G && stream_stages<GROUPED, 2, GROUP>(p.w.blocks) && chunks * half <= 0x3fffffff)
-            return pair ? launch_stream<GROUPED, 2, GROUP, true>(p, chunks * half, early, stream)
-                        : launch_stream<GROUPED, 2, GROUP, false>(p, chunks * ((half + 1) / 2), early, stream);
+            return pair ? launch_stream<GROUPED, 2, GROUP, true>(p, chunks * half, stream)
+                        : launch_stream<GROUPED, 2, GROUP, false>(p, chunks * ((half + 1) / 2), stream);
         if (!stream_stages<GROUPED, 1, GROUP>(p.w.blocks) || chunks * half > 0x3fffffff) return -1;
-        if (pair) return launch_stream<GROUPED, 1, GROUP, true>(p, chunks * half, early, stream);
-        return launch_stream<GROUPED, 1, GROUP, false>(p, chunks * ((half + 1) / 2), early, stream);
+        if (pair) return launch_stream<GROUPED, 1, GROUP, true>(p, chunks * half, stream);
+        return launch_stream<GROUPED, 1, GROUP, false>(p, chunks * ((half + 1) / 2), stream);
     }
-    if (p.M <= 8) return run_dense<1, GROUP>(p, pair, early, stream);
-    return p.M <= 16 ? run_dense<2, GROUP>(p, pair, early, stream) : run_dense<3, GROUP>(p, pair, early, stream);
+    if (p.M <= 8) return run_dense<1, GROUP>(p, pair, stream);
+    return p.M <= 16 ? run_dense<2, GROUP>(p, pair, stream) : run_dense<3, GROUP>(p, pair, stream);
 }
 
 template <int GROUP>
-int run_experts(const Args& up, const DownArgs& down, bool early, cudaStream_t stream) {
+int run_experts(const Args& up, const DownArgs& down, cudaStream_t stream) {
     if (!stream_stages<EXPERTS, 1, GROUP>(up.w.blocks)) return -1;
     const long long pairs = (long long)up.M * up.top_k, slots = pairs < up.E ? pairs : up.E;
     const long long units = slots * (up.w.strips / 2) + (up.shared.codes ? up.shared.strips / 2 : 0);
-    int e = launch_stream<EXPERTS, 1, GROUP, true>(up, units, early, stream);
+    int e = launch_stream<EXPERTS, 1, GROUP, true>(up, units, stream);
     if (e) return e;
     static q4::SmemLimit limit;
     if ((e = limit.lift((const void*)experts_down_kernel<GROUP>))) return e;
@@ -855,15 +858,15 @@ MOE_API int moe_gemm_q4(const void* x, int ldx, int M, const void* codes, const 
     p.w = weight(codes, scales, N, K, group, pair);
     p.x = (const __nv_bfloat16*)x, p.ldx = ldx, p.M = M, p.vec = K % 4 == 0 && ldx % 4 == 0 && ((uintptr_t)x & 7) == 0;
     p.out = out, p.out_bf16 = out_bf16, p.ldo = ldo, p.bias = bias, p.offsets = offsets, p.G = G, p.N = pair ? N / 2 : N;
-    p.act = act, p.act_param = act_param, p.bits = q4::bits(), p.waits = q4::Waits{status, g_wait_limit, g_test_fault};
-#define GO(GR) run_gemm<GR>(p, pair != 0, early != 0, stream)
+    p.act = act, p.act_param = act_param, p.early = early, p.bits = q4::bits(), p.waits = q4::Waits{status, g_wait_limit, g_test_fault};
+#define GO(GR) run_gemm<GR>(p, pair != 0, stream)
     BY_GROUP(GO);
 #undef GO
 }
 
 // x: [T, H] bfloat16, row pitch ldx; idx, wk: [T, top_k]; gate: [T] or null; gu [E, 2 size, H] and sgu [2 shared, H] pairs, down [E, H, size], sdown
 // [H, shared]; shared 0: no shared expert; scratch: 3 KB for each 64 features of the experts that may be picked
-// (min(T top_k, E)) and of the shared one; early: as above, for all four.  Returns -1 for what it does not take: more than 8 tokens, 1,024 experts or 128 picks, rows that shared
+// (min(T top_k, E)) and of the shared one; early: as above, of the pairs (the second kernel waits for the first in any case).  Returns -1 for what it does not take: more than 8 tokens, 1,024 experts or 128 picks, rows that shared
 // memory does not hold (H beyond 6,000 or so).
 MOE_API int moe_experts_q4(const void* x, int ldx, int T, int H, const int* idx, const float* wk, int top_k, int E, int size, const void* gu_codes,
                            const void* gu_scales, const void* down_codes, const void* down_scales, int shared, const void* sgu_codes,
@@ -876,7 +879,7 @@ MOE_API int moe_experts_q4(const void* x, int ldx, int T, int H, const int* idx,
     Args up = {};
     DownArgs d = {};
     up.x = (const __nv_bfloat16*)x, up.ldx = ldx, up.vec = H % 4 == 0 && ldx % 4 == 0 && ((uintptr_t)x & 7) == 0, up.M = T;
-    up.idx = idx, up.top_k = top_k, up.E = E, up.bits = q4::bits(), up.waits = q4::Waits{status, g_wait_limit, g_test_fault};
+    up.idx = idx, up.top_k = top_k, up.E = E, up.early = early, up.bits = q4::bits(), up.waits = q4::Waits{status, g_wait_limit, g_test_fault};
     up.w = weight(gu_codes, gu_scales, 2 * size, H, group, 1), d.down = weight(down_codes, down_scales, H, size, group, 0);
     if (shared > 0) up.shared = weight(sgu_codes, sgu_scales, 2 * shared, H, group, 1), d.shared = weight(sdown_codes, sdown_scales, H, shared, group, 0);
     const long long slots = (long long)T * top_k < E ? (long long)T * top_k : E;
@@ -887,7 +890,7 @@ MOE_API int moe_experts_q4(const void* x, int ldx, int T, int H, const int* idx,
     // blocks of a cluster: one block an SM, but five blocks of 64 k a warp are done sooner than two cluster barriers
     const long long most = slots * d.down.blocks + (shared > 0 ? d.shared.blocks : 0);
     d.S = most <= 5 * DOWN_W ? 1 : max(1, min(8, q4::sm_count() / ((d.down.strips + DOWN_MT - 1) / DOWN_MT)));
-#define GO(GR) run_experts<GR>(up, d, early != 0, stream)
+#define GO(GR) run_experts<GR>(up, d, stream)
     BY_GROUP(GO);
 #undef GO
 }

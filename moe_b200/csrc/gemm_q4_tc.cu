@@ -63,6 +63,7 @@ struct Args {
     int act;
     float act_param;
     int* status;
+    int early;                     // the weight may be read before what is in front of this launch has ended
     uint32_t wait_limit;
     q4::Bits bits;
     int test_fault;                // 0; the wait test: 1 nothing is loaded, 2 no product is issued, 3 no value is formed
@@ -306,6 +307,7 @@ gemm_q4_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant
 
     if (warp < DEQUANT_WARPS) {
         // ---- codes to values: block `it` of the CTA's sequence by the warps of team it % TEAMS -----------------------------------------
+        if (!p.offsets && !p.early) pdl_wait();
         const int q = warp % F::TEAM, r = lane >> 2, half = PAIR ? p.w.strips / 2 : p.w.strips;
         uint4 code[PREFETCH][2];
         q4::Scales<GROUP> sc[PREFETCH][2];
@@ -538,10 +540,10 @@ uint32_t g_wait_limit = WAIT_LIMIT_US;
 int g_test_fault = 0;
 
 template <int GROUP, bool PAIR, bool WIDE>
-int launch(const CUtensorMap& map, const Args& p, unsigned ctas, bool early, cudaStream_t stream) {
+int launch(const CUtensorMap& map, const Args& p, unsigned ctas, cudaStream_t stream) {
     static q4::SmemLimit limit;
     if (const int e = limit.lift((const void*)gemm_q4_tc_kernel<GROUP, PAIR, WIDE>)) return e;
-    return launch_pdl_if(early, gemm_q4_tc_kernel<GROUP, PAIR, WIDE>, dim3(ctas, 1, p.splits), dim3(Form<WIDE>::THREADS), (size_t)(p.stages * p.stage_bytes + 1024), stream, p.splits, map, p);
+    return launch_pdl_cluster(gemm_q4_tc_kernel<GROUP, PAIR, WIDE>, dim3(ctas, 1, p.splits), dim3(Form<WIDE>::THREADS), (size_t)(p.stages * p.stage_bytes + 1024), stream, p.splits, map, p);
 }
 
 }  // namespace
@@ -564,7 +566,7 @@ MOE_API int moe_gemm_q4_tc(const void* x, int ldx, int M, const void* codes, con
     p.N = pair ? N / 2 : N;
     p.w.strips = (p.N + 15) / 16 * (pair ? 2 : 1), p.w.blocks = (K + 63) / 64, p.w.qgroups = (K + group - 1) / group;
     p.out = out, p.out_bf16 = out_bf16, p.ldo = ldo, p.bias = bias, p.offsets = offsets, p.G = G, p.M = M;
-    p.act = act, p.act_param = act_param, p.status = status, p.wait_limit = g_wait_limit, p.test_fault = g_test_fault, p.bits = q4::bits();
+    p.act = act, p.act_param = act_param, p.early = early, p.status = status, p.wait_limit = g_wait_limit, p.test_fault = g_test_fault, p.bits = q4::bits();
     // Groups that mostly fit 128 rows take the wide tile.  (us, narrow / wide: 60 experts of a pair 2,816 x 2,048 at 34 rows an expert 126 / 101, at 100 137 / 109,
     // at 136, where most have a second tile, 149 / 177; of 2,048 x 1,408 69 / 52, 73 / 61, 76 / 86.  A dense product of 64 rows of 6,144 x 2,048 in the better
     // number of splits 11.1 / 10.8, of 113 rows 12.1 / 12.4: the narrow one throughout.)
@@ -589,8 +591,8 @@ MOE_API int moe_gemm_q4_tc(const void* x, int ldx, int M, const void* codes, con
     p.splits = (p.w.blocks + p.kb_per_split - 1) / p.kb_per_split;
     const unsigned ctas = p.splits > 1 ? (unsigned)tiles : (unsigned)(tiles < sms ? tiles : sms);
 #define GO(GR)                                                                                                  \
-    (wide ? (pair ? launch<GR, true, true>(map, p, ctas, early, stream) : launch<GR, false, true>(map, p, ctas, early, stream)) \
-          : (pair ? launch<GR, true, false>(map, p, ctas, early, stream) : launch<GR, false, false>(map, p, ctas, early, stream)))
+    (wide ? (pair ? launch<GR, true, true>(map, p, ctas, stream) : launch<GR, false, true>(map, p, ctas, stream)) \
+          : (pair ? launch<GR, true, false>(map, p, ctas, stream) : launch<GR, false, false>(map, p, ctas, stream)))
     switch (group) {
         case 32: return GO(32);
         case 64: return GO(64);

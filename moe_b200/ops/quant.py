@@ -109,6 +109,14 @@ class Weight4:
         """(A copy, or what is stored and read back, has tensors of its own: their addresses, and what has read them.)"""
         return Weight4, (self.codes, self.scales, self.shape, self.group, self.pair)
 
+    def _parts(self, groups: int):
+        """(so many neighbouring matrices of a stack, the first one's number)"""
+        codes, scales = self.codes.view(self.G, -1), self.scales.view(self.G, -1)
+        for g in range(0, self.G, groups):
+            part = Weight4(codes[g:g + groups], scales[g:g + groups], (min(groups, self.G - g), self.N, self.K), self.group, self.pair)
+            part.read_on = self.read_on
+            yield part, g
+
     def settle(self) -> None:
         """Waits until the device has done what it was given, the writing of this weight with it."""
         if self.place >= 0:
@@ -144,9 +152,9 @@ def _on(t: Optional[torch.Tensor], place: int, name: str, dtype, numel: Optional
     return t.data_ptr()
 
 
-def _status(t: Optional[torch.Tensor], place: int):
+def _status(t: torch.Tensor, place: int):
     """(Faults and, beside them, where the first wait ran out.)"""
-    if t is not None and t.numel() < 2:
+    if t.numel() < 2:
         raise core.KernelError("status: expected what core.new_status makes")
     return _on(t, place, "status", torch.int32)
 
@@ -166,14 +174,11 @@ def _matrix(t: torch.Tensor, place: int, name: str, wide: bool):
     return rows, columns, pitch
 
 
-def _early(w: Weight4, stream: int) -> bool:
-    return w.read_on is None or stream in w.read_on
-
-
 def _has_read(w: Weight4, stream: int):
     """(Not what is captured: a graph's launches say nothing of the stream that it was captured on.)"""
-    if w.read_on is not None and stream not in w.read_on and not _capturing():
-        w.read_on = (*w.read_on, stream)
+    read_on = w.read_on
+    if read_on is not None and stream not in read_on and not _capturing():
+        w.read_on = read_on + (stream,)
 
 
 _capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", torch.cuda.is_current_stream_capturing)
@@ -197,7 +202,7 @@ def quantize(w: torch.Tensor, group: int = 64, *, pair: bool = False, status=Non
     codes = torch.empty(G * strips * -(-K // 64) * 512, dtype=torch.uint8, device=device)
     scales = torch.empty(G * strips * -(-K // group) * 16, dtype=torch.bfloat16, device=device)
     core._ok((_lib or lib()).moe_q4_quantize(w.data_ptr(), core._dt(w), G, N, K, group, pair, codes.data_ptr(), scales.data_ptr(),
-                                             _status(status, w.get_device()), core._stream()), "quantize")
+                                             None if status is None else _status(status, w.get_device()), core._stream()), "quantize")
     return Weight4(codes, scales, w.shape, group, pair)
 
 
@@ -244,11 +249,16 @@ def gemm4(x: torch.Tensor, w: Weight4, out: torch.Tensor, *, swiglu: bool = Fals
         raise core.KernelError("gemm4: a stack needs group_offsets")
     pb = None if bias is None else _on(bias, place, "bias", _F32, N)
     po = None if group_offsets is None else _on(group_offsets, place, "group_offsets", torch.int32, w.G + 1)
-    st = _status(status, place)
+    st = None if status is None else _status(status, place)
     if not M:
         return out
-    L, stream = _lib or lib(), core._stream()
-    early = _early(w, stream)
+    if w.G > GROUPS_A_LAUNCH:
+        for part, g in w._parts(GROUPS_A_LAUNCH):
+            gemm4(x, part, out, swiglu=swiglu, bias=bias, group_offsets=group_offsets[g:g + part.G + 1], act=act, act_param=act_param, any_rows=any_rows, status=status)
+        return out
+    L, stream, read_on = _lib or lib(), core._stream(), w.read_on
+    early = read_on is None or stream in read_on
+    pc, ps = w.pointers
     # Few rows stream the weights through registers, more go to the tensor core, whose tiles cost the same for 16 rows as for 100.  (us, this way / the
     # other: 17 rows of 6,144 x 2,048 7.3 / 10.2, 24 8.4 / 10.3, 32 in passes of 24 16 / 10.5; of 2,048 x 5,632 10.2 / 11.5, 12.0 / 11.5; of a pair
     # 11,264 x 2,048 9.8 / 15.3, 10.2 / 15.4; of 40,960 x 2,048 20.9 / 38.2, 21.4 / 38.2.  60 experts of a pair 2,816 x 2,048 at 14 rows an expert 79 / 98, at 16 93 / 99; of 2,048 x 1,408 50 / 51, 57 / 51.)
@@ -258,27 +268,20 @@ def gemm4(x: torch.Tensor, w: Weight4, out: torch.Tensor, *, swiglu: bool = Fals
         whole = torch.zeros(M, ldx, dtype=_BF16, device=x.device)
         whole[:, :K] = x
         x, K = whole, ldx
-    strips = _strips(w.N, w.pair)
-    for g in range(0, w.G, GROUPS_A_LAUNCH):
-        pc, ps = w.pointers
-        if g:                              # further groups of a large stack
-            pc, ps, po = pc + g * strips * -(-K // 64) * 512, ps + g * strips * -(-K // w.group) * 32, po + 4 * GROUPS_A_LAUNCH
-        groups = min(w.G - g, GROUPS_A_LAUNCH)
-        for form in (few, not few):        # (what one does not take, -1, the other may)
-            if form:
-                done = L.moe_gemm_q4(x.data_ptr(), ldx, M, pc, ps, groups, w.N, K, w.group, w.pair, out.data_ptr(), out.dtype is _BF16, ldo, pb, po,
-                                     code, act_param, early or g > 0, st, stream)
-            else:
-                done = L.moe_gemm_q4_tc(x.data_ptr(), ldx, M, pc, ps, groups, w.N, K, w.group, w.pair, out.data_ptr(), out.dtype is _BF16, ldo, pb,
-                                        po, code, act_param, 1 if po is not None else _splits(M, N, w, place), early or g > 0, st, stream)
-            if done != -1:
-                break
-        if done == -1:
-            raise core.KernelError("gemm4: a stack of K beyond 5,500 or so with rows that are no whole 16-byte units (any_rows copies them)")
-        core._ok(done, "gemm4")
-    if not early:
-        _has_read(w, stream)
-    return out
+    done = -1
+    for form in (few, not few):            # (what one does not take, -1, the other may)
+        if form:
+            done = L.moe_gemm_q4(x.data_ptr(), ldx, M, pc, ps, w.G, w.N, K, w.group, w.pair, out.data_ptr(), out.dtype is _BF16, ldo, pb, po,
+                                 code, act_param, early, st, stream)
+        else:
+            done = L.moe_gemm_q4_tc(x.data_ptr(), ldx, M, pc, ps, w.G, w.N, K, w.group, w.pair, out.data_ptr(), out.dtype is _BF16, ldo, pb,
+                                    po, code, act_param, 1 if po is not None else _splits(M, N, w, place), early, st, stream)
+        if done != -1:
+            core._ok(done, "gemm4")
+            if not early:
+                _has_read(w, stream)
+            return out
+    raise core.KernelError("gemm4: a stack of K beyond 5,500 or so with rows that are no whole 16-byte units (any_rows copies them)")
 
 
 def _splits(M: int, N: int, w: Weight4, place: int) -> int:
@@ -333,14 +336,14 @@ def experts4(x: torch.Tensor, topk_idx: torch.Tensor, topk_w: torch.Tensor, gate
     if down.group != group:
         raise core.KernelError("experts4: the weights of a layer have one group size")
     pi, pw = _on(topk_idx, place, "topk_idx", torch.int32), _on(topk_w, place, "topk_w", torch.float32)
-    pg, ps = _on(shared_gate, place, "shared_gate", torch.float32, T), _status(status, place)
+    pg, ps = _on(shared_gate, place, "shared_gate", torch.float32, T), None if status is None else _status(status, place)
     if not takes_experts(T, k, gate_up):
         return False
     if not T:
         return True
     L, stream = _lib or lib(), core._stream()
     weights = (gate_up, down) if shared_gate_up is None else (gate_up, down, shared_gate_up, shared_down)
-    early = all(_early(w, stream) for w in weights)
+    early = all(w.read_on is None or stream in w.read_on for w in weights)
     slots = min(T * k, E)
     scratch = torch.empty((slots * -(-size // 64) + -(-shared // 64)) * 3072, dtype=torch.uint8, device=x.device)
     code = L.moe_experts_q4(x.data_ptr(), ldx, T, H, pi, pw, k, E, size, *gate_up.pointers, *down.pointers, shared, *s, pg, group, scratch.data_ptr(),
