@@ -16,6 +16,7 @@ called while a CUDA graph is captured.
 """
 from __future__ import annotations
 
+import functools
 import os
 from ctypes import c_float, c_int, c_longlong, c_uint, c_void_p
 from typing import Optional, Tuple
@@ -174,11 +175,14 @@ def _matrix(t: torch.Tensor, place: int, name: str, wide: bool):
     return rows, columns, pitch
 
 
-def _has_read(w: Weight4, stream: int):
+def _have_read(stream: int, *weights: Weight4):
     """(Not what is captured: a graph's launches say nothing of the stream that it was captured on.)"""
-    read_on = w.read_on
-    if read_on is not None and stream not in read_on and not _capturing():
-        w.read_on = read_on + (stream,)
+    if _capturing():
+        return
+    for w in weights:
+        read_on = w.read_on
+        if read_on is not None and stream not in read_on:
+            w.read_on = read_on + (stream,)
 
 
 _capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", torch.cuda.is_current_stream_capturing)
@@ -222,7 +226,8 @@ def gemm4(x: torch.Tensor, w: Weight4, out: torch.Tensor, *, swiglu: bool = Fals
           group_offsets: Optional[torch.Tensor] = None, act: str = "silu", act_param: float = 0.0, any_rows: bool = False, status=None) -> torch.Tensor:
     """out = x w^T (+ bias), or act(x gate^T) * (x up^T) with ``swiglu`` and a pair; ``act``: as in ``tc.gemm_tc``.
 
-    x: bfloat16 [M, K], dense rows of any pitch; out: float32 or bfloat16 [M, N] (a pair: [M, N / 2]), dense rows of any pitch.
+    x: bfloat16 [M, K], dense rows of any pitch, of magnitudes below 2^119 (few rows meet the codes before the scale); out: float32 or bfloat16 [M, N] (a pair:
+    [M, N / 2]), dense rows of any pitch.
     A stack needs ``group_offsets`` (int32 [G + 1], ascending): rows [offsets[g], offsets[g + 1]) of x meet w[g]; rows that no group
     has are left as they were.
 
@@ -263,7 +268,7 @@ def gemm4(x: torch.Tensor, w: Weight4, out: torch.Tensor, *, swiglu: bool = Fals
     # other: 17 rows of 6,144 x 2,048 7.3 / 10.2, 24 8.4 / 10.3, 32 in passes of 24 16 / 10.5; of 2,048 x 5,632 10.2 / 11.5, 12.0 / 11.5; of a pair
     # 11,264 x 2,048 9.8 / 15.3, 10.2 / 15.4; of 40,960 x 2,048 20.9 / 38.2, 21.4 / 38.2.  60 experts of a pair 2,816 x 2,048 at 14 rows an expert 79 / 98, at 16 93 / 99; of 2,048 x 1,408 50 / 51, 57 / 51.)
     few = M <= (FEW_ROWS if po is None else GROUP_FEW_ROWS * w.G)
-    if any_rows and (K % 8 or ldx % 8 or x.data_ptr() % 16) and not (few and (po is None or L.moe_q4_holds_rows(K, w.group, 0))):
+    if any_rows and (K % 8 or ldx % 8 or x.data_ptr() % 16) and not (few and (po is None or _holds_rows(K, w.group, False))):
         few, ldx = False, (K + 7) // 8 * 8           # (as many blocks and groups of k as before: the weight's elements there are zeros)
         whole = torch.zeros(M, ldx, dtype=_BF16, device=x.device)
         whole[:, :K] = x
@@ -279,7 +284,7 @@ def gemm4(x: torch.Tensor, w: Weight4, out: torch.Tensor, *, swiglu: bool = Fals
         if done != -1:
             core._ok(done, "gemm4")
             if not early:
-                _has_read(w, stream)
+                _have_read(stream, w)
             return out
     raise core.KernelError("gemm4: a stack of K beyond 5,500 or so with rows that are no whole 16-byte units (any_rows copies them)")
 
@@ -296,10 +301,15 @@ def _splits(M: int, N: int, w: Weight4, place: int) -> int:
     return 1
 
 
+@functools.lru_cache(maxsize=None)
+def _holds_rows(K: int, group: int, layer: bool) -> bool:
+    """Whether shared memory holds what groups of few rows (``layer``: a layer of experts) need of rows so long."""
+    return bool((_lib or lib()).moe_q4_holds_rows(K, group, layer))
+
+
 def takes_experts(tokens: int, top_k: int, gate_up: Weight4) -> bool:
     """Whether ``experts4`` takes so many tokens and picks through these experts."""
-    return (tokens <= EXPERTS_TOKENS and gate_up.G <= GROUPS_A_LAUNCH and tokens * top_k <= 128
-            and bool((_lib or lib()).moe_q4_holds_rows(gate_up.K, gate_up.group, 1)))
+    return tokens <= EXPERTS_TOKENS and gate_up.G <= GROUPS_A_LAUNCH and tokens * top_k <= 128 and _holds_rows(gate_up.K, gate_up.group, True)
 
 
 def experts4(x: torch.Tensor, topk_idx: torch.Tensor, topk_w: torch.Tensor, gate_up: Weight4, down: Weight4, out: torch.Tensor, *,
@@ -343,14 +353,15 @@ def experts4(x: torch.Tensor, topk_idx: torch.Tensor, topk_w: torch.Tensor, gate
         return True
     L, stream = _lib or lib(), core._stream()
     weights = (gate_up, down) if shared_gate_up is None else (gate_up, down, shared_gate_up, shared_down)
-    early = all(w.read_on is None or stream in w.read_on for w in weights)
+    early = True
+    for w in weights:
+        early = early and (w.read_on is None or stream in w.read_on)
     slots = min(T * k, E)
     scratch = torch.empty((slots * -(-size // 64) + -(-shared // 64)) * 3072, dtype=torch.uint8, device=x.device)
     code = L.moe_experts_q4(x.data_ptr(), ldx, T, H, pi, pw, k, E, size, *gate_up.pointers, *down.pointers, shared, *s, pg, group, scratch.data_ptr(),
                             scratch.numel(), out.data_ptr(), out.dtype is _BF16, ldo, early, ps, stream)
     core._ok(code, "experts4")
     if not early:
-        for w in weights:
-            _has_read(w, stream)
+        _have_read(stream, *weights)
     core.launches += 1            # (two kernels)
     return True
