@@ -2,19 +2,19 @@
 //
 //   y[m, n] = sum_k x[m, k] q[n, k] s[n, k / group] (+ b[n]), or act(gate) * up of a pair's two rows.
 //
-// What should bound them is the stream of codes, 0.53 bytes an element; what does is the issue slots and the logic unit: 6.5 TB/s are 46
-// elements a cycle and SM, and turning eight codes into fragments takes 11 instructions a lane.  So the weights are the A operand of m16n8k16 products
+// What should bound them is the stream of codes, 0.53 bytes an element; for one row of a long matrix it is the issue slots and the logic unit (without forming
+// fragments 27 us of 37): 6.5 TB/s are 46 elements a cycle and SM, and turning eight codes into fragments takes 11 instructions a lane.  So the weights are the A operand of m16n8k16 products
 // straight from the registers that they come in (a shift, a mask and a subtraction a pair of elements), a product takes eight rows of x for the
 // price of one, and the scale is applied to the sums of a group's k (up to four products from zero, then one multiply-add an output), which also
 // keeps the sums in plain 32-bit additions but for those 64.  The warps that share a strip's k add their sums up through shared memory in the order of the warps.
 //
 //   gemm_q4_direct_kernel    few strips: a block of eight warps a strip, codes and rows straight to registers, all asked for at once.  8 rows of
-//                            6,144 x 2,048 3.8 us, 1 row of 2,048 x 2,048 2.5
+//                            6,144 x 2,048 3.5 us (with a bias 3.6), 1 row of 2,048 x 2,048 2.4
 //   gemm_q4_stream_kernel    many: one block an SM, its codes by bulk copies into stages, the rows' fragments in shared memory.  1 row of
-//                            151,936 x 2,048 37 us (4.5 TB/s; ALU 58 %, issue slots 64 %), 16 rows of a pair 40,960 x 3,584 26 us (2.9 TB/s: the products
-//                            of two tiles of rows do not overlap with the fragments' making), 256 rows of 60 experts 2,048 x 1,408 30 us (3.1 TB/s)
+//                            151,936 x 2,048 37 us (4.5 TB/s; ALU 58 %, issue slots 64 %), 16 rows of a pair 40,960 x 3,584 26 us (2.9 TB/s: two rounds of units
+//                            with 86 % of the teams' places used, two stages a team at this K; without fragments and products 20.7), 256 rows of 60 experts 2,048 x 1,408 30 us (3.1 TB/s)
 //   experts_down_kernel      the second half of a layer of experts.  A layer of 60 experts of 1,408 and a shared one of 5,632, width 2,048: 1 token
-//                            18.2 us, 8 tokens 44.7
+//                            18.2 us, 8 tokens 44.6
 #include "quant4.cuh"
 
 namespace {
@@ -198,7 +198,7 @@ __device__ __forceinline__ void put(const Args& p, int row, int n, float y) {
 // ---- few strips -----------------------------------------------------------------------------------------------------------------------------
 // Grid: strips of the output (of a pair: of one half).  Warp w takes blocks w, w + 8, ... of 64 k, DEPTH of them in flight; the codes are asked for
 // before the wait on the predecessor, the rows behind it and one block ahead.  Three blocks an SM count for more than anything that their registers
-// could hold.  (us, two / three: 8 rows of 6,144 x 2,048, with all four blocks' rows ahead in the first, 6.3 / 3.6, of a pair 11,264 x 2,048 6.7 / 4.8,
+// could hold.  (us of one set of runs, two / three: 8 rows of 6,144 x 2,048, with all four blocks' rows ahead in the first, 6.3 / 3.6, of a pair 11,264 x 2,048 6.7 / 4.8,
 // of 2,048 x 5,632 4.8 / 5.6; 16 rows 8.9 / 6.5, 10.6 / 8.7, 9.0 / 8.8; 24 rows 8.9 / 8.4, 14.7 / 12.5, 12.5 / 12.0.)
 template <int MT, int NT, int GROUP>
 __global__ void __launch_bounds__(256, 3)
@@ -587,8 +587,8 @@ gemm_q4_stream_kernel(const __grid_constant__ Args p, const int stages) {
 // Four strips of the output go through ALL picked experts and the shared one, w_te on the sums of each block of 64 k: nothing is left to
 // combine.  Tokens that did not pick an expert meet it with the zeros that the first kernel left, and its sums stay out of theirs (a scale may be NaN).  A block of 64 k of the rows is 3 KB: for each
 // 16 k a B fragment of 32 lanes x (four k's first terms, their second terms), and behind the four of them the third terms, 8 bytes a lane.  (With two terms, rounded, the
-// layer's 32-bit output was 2.4e-6 of its norm off, ten times what its sums leave: 1 token 17.3 us, 8 tokens 41.6.  32-bit rows that become three terms in registers
-// here: 18.9, 47.0.)  Grid: (fours of strips, 1, S); the S blocks of a unit are
+// layer's 32-bit output was 2.4e-6 of its norm off, ten times what its sums leave: 1 token 17.3 us, 8 tokens 41.6, now 18.2, 44.6.  32-bit rows that become three terms
+// in registers here: 18.9, 47.0.)  Grid: (fours of strips, 1, S); the S blocks of a unit are
 // a cluster and share its blocks of 64 k; the first of them adds their sums up in order.  A warp takes every sixteenth block and copies for itself
 // into a ring of its own (cp.async: its pieces of 512 bytes and less are too small for bulk copies, of which an SM issued one in ten to twenty cycles).
 constexpr int DOWN_W = 16, DOWN_MT = 4, DOWN_DEPTH = 2, DOWN_THREADS = DOWN_W * 32;
@@ -787,7 +787,7 @@ int launch_stream(const Args& p, long long max_units, cudaStream_t stream) {
 }
 
 // One weight, 8 NT rows (24: any number, in passes).  Streamed where a block a strip does not fit the SMs at once, three each, or, above eight rows, where there are
-// 1.5 units an SM.  (us, a block a strip / streamed: 8 rows of 6,144 x 2,048, 384 blocks, 3.5 / 5.1, of 7,168 x 2,048, 448, 5.5 / 5.1, of 12,288 x 2,048
+// 1.5 units an SM.  (us of another, a block a strip / streamed: 8 rows of 6,144 x 2,048, 384 blocks, 3.5 / 5.1, of 7,168 x 2,048, 448, 5.5 / 5.1, of 12,288 x 2,048
 // 6.9 / 6.0, of 8,192 x 5,632 16.7 / 10.6, of a pair 11,264 x 2,048, 352, 4.9 / 5.9, of a pair 14,336 x 2,048, 448, 7.4 / 6.7; 16 rows of 6,144 x 2,048, 192 units, 6.3 / 7.4,
 // of a pair 11,264 x 2,048, 352, 8.9 / 8.3; 24 rows of the two 8.6 / 8.8, 12.6 / 10.2.)
 template <int NT, int GROUP>
@@ -866,7 +866,8 @@ MOE_API int moe_gemm_q4(const void* x, int ldx, int M, const void* codes, const 
 
 // x: [T, H] bfloat16, row pitch ldx; idx, wk: [T, top_k]; gate: [T] or null; gu [E, 2 size, H] and sgu [2 shared, H] pairs, down [E, H, size], sdown
 // [H, shared]; shared 0: no shared expert; scratch: 3 KB for each 64 features of the experts that may be picked
-// (min(T top_k, E)) and of the shared one; early: as above, of the pairs (the second kernel waits for the first in any case).  Returns -1 for what it does not take: more than 8 tokens, 1,024 experts or 128 picks, rows that shared
+// (min(T top_k, E)) and of the shared one; early: as above (the second kernel reads its weights early in any case: the first has waited for what
+// wrote them).  Returns -1 for what it does not take: more than 8 tokens, 1,024 experts or 128 picks, rows that shared
 // memory does not hold (H beyond 6,000 or so).
 MOE_API int moe_experts_q4(const void* x, int ldx, int T, int H, const int* idx, const float* wk, int top_k, int E, int size, const void* gu_codes,
                            const void* gu_scales, const void* down_codes, const void* down_scales, int shared, const void* sgu_codes,
