@@ -57,11 +57,15 @@ def swiglu_linear(rt, a: torch.Tensor, w_gate_up: torch.Tensor, act: str = "silu
 
 
 def _gather(rt, a: torch.Tensor, rows: torch.Tensor, n: int) -> torch.Tensor:
-    if a.shape[1] % 8 == 0 and a.stride(0) % 8 == 0:
-        from . import tc
+    """a[rows[:n]]; rows that are no whole 16-byte units go through a copy that has such, so that a bad index is reported whatever the width."""
+    from . import tc
 
-        return tc.gather_rows(a, rows, n, rt.status)
-    return a.index_select(0, rows[:n])
+    width = a.shape[1]
+    if width % 8 or a.stride(0) % 8 or a.data_ptr() % 16:
+        whole = torch.zeros((a.shape[0], (width + 7) // 8 * 8), dtype=a.dtype, device=a.device)
+        whole[:, :width] = a
+        a = whole
+    return tc.gather_rows(a, rows, n, rt.status)[:, :width]
 
 
 def grouped_swiglu_linear(rt, a: torch.Tensor, w_gate_up: torch.Tensor, group_offsets: torch.Tensor,

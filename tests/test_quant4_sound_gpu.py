@@ -526,3 +526,32 @@ def test_a_status_without_room_for_what_is_reported_is_refused(quant):
                      lambda: quant.experts4(x, idx, w, pair, down, torch.empty(2, 64, device=DEV), status=small)):
             with pytest.raises(core.KernelError, match="status"):
                 call()
+
+
+@pytest.mark.parametrize("H", [64, 100, 133])
+def test_a_gather_index_outside_its_tensor_is_reported_whatever_the_width(quant, H):
+    """Rows of no whole 16-byte units too: the other rows are what they are, and the context lives on."""
+    from moe_b200.ops import core
+    from moe_b200.ops.linear import grouped_swiglu_linear
+    from moe_b200.parts.base import Runtime
+
+    torch.manual_seed(H)
+    rt = Runtime(DEV, BF, 64)
+    w4, W = weight(quant, (3, 48, H), pair=True)
+    a = torch.randn(7, H, device=DEV).to(BF)
+    rows = torch.tensor([3, 0, 6, 6, 1, 2, 5, 4, 0], dtype=torch.int32, device=DEV)
+    off = torch.tensor([0, 4, 4, 9], dtype=torch.int32, device=DEV)
+    for bad in (None, -1, 7, 1 << 30):
+        at = rows.clone()
+        if bad is not None:
+            at[5] = bad
+        out = grouped_swiglu_linear(rt, a, w4, off, at, 9)
+        if bad is None:
+            rt.check()
+        else:
+            with pytest.raises(core.KernelError, match="gather"):
+                rt.check()
+        for g, (lo, hi) in enumerate(((0, 4), (4, 4), (4, 9))):
+            keep = [i for i in range(lo, hi) if bad is None or i != 5]
+            if keep:
+                Q.check_product(out[keep], a[rows[keep].long()], W[g], swiglu=True)
