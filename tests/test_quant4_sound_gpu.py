@@ -555,3 +555,16 @@ def test_a_gather_index_outside_its_tensor_is_reported_whatever_the_width(quant,
             keep = [i for i in range(lo, hi) if bad is None or i != 5]
             if keep:
                 Q.check_product(out[keep], a[rows[keep].long()], W[g], swiglu=True)
+
+
+def test_the_command_line_times_a_model_with_4_bit_weights(model_dirs, capsys):
+    from moe_b200 import cli
+
+    d = model_dirs.get("D", "bfloat16", seed=1, std=0.02)
+    said = []
+    for more in ([], ["--weights", "int4", "--weight-group", "128"]):
+        assert cli.main(["bench", d, "--tokens", "4", "--prompt-len", "9", "--batch", "3", *more]) == 0
+        said.append(capsys.readouterr().out)
+    assert all("roofline" in s and "tok/s" in s for s in said)
+    read = [s.split("roofline ")[1].split(" weights")[0] for s in said]
+    assert read[0] != read[1], read
